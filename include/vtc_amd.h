@@ -238,6 +238,64 @@ int vtc_profile_read(vtc_model* m, double* ms /*[VTC_PROF_CLASSES]*/, int64_t* l
                      double* flops /*[VTC_PROF_CLASSES]*/, double* bytes /*[VTC_PROF_CLASSES]*/);
 const char* vtc_profile_class_name(int32_t cls);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Operators: the pieces of an encoder variant (vtc_create_variant), for callers that run layers themselves or train them.
+ * No counterpart in the reference (its model code lives in segma).  They take a device index instead of a model, launch on
+ * `stream` (which belongs to that device), never allocate and never synchronise, so they may be captured into a graph and
+ * called from several threads; the caller's current device is left as it was.  Scratch memory is the caller's: its size comes
+ * from the matching _workspace call, it must be 256-byte aligned, and two calls that may run at the same time need two.
+ * The message of a failure is vtc_last_error(NULL) on the calling thread.  Sizes of zero are valid and launch nothing that
+ * reads them.  Bits of a result do not depend on the launch order (no atomics). */
+typedef enum { VTC_F32 = 0, VTC_F16 = 1, VTC_BF16 = 2 } vtc_dtype;
+typedef enum { VTC_ACT_NONE = 0, VTC_ACT_GELU = 1 /* x Phi(x) */, VTC_ACT_SILU = 2, VTC_ACT_SIGMOID = 3 } vtc_act;
+
+/* Rotary positions.  A pair (a, b) of a head at position p becomes amplitude * (a cos t - b sin t, a sin t + b cos t) with
+ * t = p * frequency[j]; inverse != 0 turns by -t (the gradient's direction).  Pairs are (j, j + rotary_dim / 2) (HALF) or
+ * (2j, 2j + 1) (INTERLEAVED) of the first rotary_dim elements; the rest of the head is copied.  Angles are reduced in 64 bits.
+ * Positions are [dev] int32 or int64 at positions[b * pos_batch + t * pos_row] + offset, or, with positions == NULL, t + offset.
+ * One or two tensors (q and k) of shape (batch, length, heads, head_dim) per call, element strides as given, the elements of a
+ * head contiguous; y may be x itself (same strides) or memory apart from it, and the elements of y must be distinct.  x may have
+ * strides of zero. */
+#define VTC_ROTARY_HALF 0
+#define VTC_ROTARY_INTERLEAVED 1
+typedef struct {
+  int32_t head_dim, rotary_dim; /* rotary_dim even, <= head_dim, <= 512 */
+  int32_t layout;
+  int32_t reserved;
+  double amplitude;
+  const double* frequency;      /* [host] rotary_dim / 2 radians per position; copied before the call returns */
+} vtc_rotary;
+typedef struct {
+  const void* x; /* [dev] */
+  void* y;       /* [dev] */
+  int64_t x_batch, x_row, x_head, y_batch, y_row, y_head;
+  int32_t heads;
+  int32_t reserved;
+} vtc_heads;
+int vtc_rotary_heads(int device, int dtype, const vtc_rotary* r, int64_t batch, int64_t length, const vtc_heads* tensors /*[host]*/,
+                     int32_t n_tensors, const void* positions /*[dev]*/, int32_t positions64, int64_t pos_batch, int64_t pos_row,
+                     int64_t offset, int32_t inverse, void* stream);
+
+/* Group norm with an activation (NONE, GELU, SILU) on channel-last rows (batch, length, channels), channels contiguous:
+ * y = act((x - mean) * rstd * weight + bias), statistics per (sample, group of channels / groups neighbours) over the real rows
+ * l < lengths[n] (lengths [dev] or NULL: all rows; values outside 0..length are clamped).  Rows behind a sample's length are not
+ * read and come out as zero, in y and in dx.  weight / bias may be NULL; they (and their gradients) are of the tensors' type, or
+ * fp32 with affine_f32 = 1.  mean / rstd [dev] [batch][groups] fp32 are written by the forward call and read by the backward one
+ * (0 and 0 for a sample without rows).  y may be x, dx may be dy or x (same strides). */
+typedef struct {
+  const void* p;      /* [dev] */
+  int64_t batch, row; /* element strides */
+} vtc_rows3;
+int64_t vtc_group_norm_act_workspace(int64_t batch, int64_t length, int32_t channels, int32_t groups, int32_t backward);
+int vtc_group_norm_act(int device, int dtype, const vtc_rows3* x, const vtc_rows3* y, int64_t batch, int64_t length, int32_t channels,
+                       int32_t groups, const void* weight /*[dev]*/, const void* bias /*[dev]*/, int32_t affine_f32, double eps, int32_t act,
+                       const int32_t* lengths /*[dev]*/, float* mean /*[dev]*/, float* rstd /*[dev]*/, void* workspace /*[dev]*/,
+                       int64_t workspace_bytes, void* stream);
+int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows3* dy, const vtc_rows3* x, const vtc_rows3* dx, int64_t batch,
+                                int64_t length, int32_t channels, int32_t groups, const void* weight, const void* bias, int32_t affine_f32,
+                                int32_t act, const int32_t* lengths, const float* mean, const float* rstd, void* dweight /*[dev] or NULL*/,
+                                void* dbias /*[dev] or NULL*/, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -69,9 +69,9 @@ __device__ __forceinline__ float gelu_f(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * p));
 }
 
-// Two elements at once with packed fp32 arithmetic (v_pk_mul_f32 / v_pk_fma_f32 / v_pk_add_f32: the same IEEE operations
-// in the same order, so the results are bit-identical to gelu_f).  tools/gelu_bench: 15.8 ns of SIMD time per 64 elements
-// against 21.3; what is left is mostly the two quarter-rate transcendentals (8.9 ns).
+// Two elements at once, the same IEEE operations in the same order as gelu_f (bit-identical to it).  The library is compiled
+// without the packed fp32 instructions (see the Makefile), so the pair runs as scalar operations: 21 ns of SIMD time per 64
+// elements, where v_pk_fma_f32 took 15.8; what is left is mostly the two quarter-rate transcendentals (8.9 ns).
 __device__ __forceinline__ void gelu2(float& a, float& b) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const f32x2 x = {a, b};

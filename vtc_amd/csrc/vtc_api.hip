@@ -24,6 +24,7 @@
 #include "flac_decode.h"
 #include "gemm.hip.h"
 #include "gemm256.hip.h"
+#include "ops.h"
 #include "posconv.hip.h"
 
 using namespace vtc;
@@ -79,6 +80,16 @@ struct LayerDev {
 struct ProfRec { int cls; double flops, bytes; hipEvent_t e0, e1; };
 
 }  // namespace
+
+int vtc::fail_handleless(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  try { g_create_error = buf; } catch (...) {}   // out of memory for the text: the code still says what happened
+  return code;
+}
 
 struct vtc_model {
   vtc_spec spec{};

@@ -53,6 +53,21 @@ class VtcWeights(C.Structure):
     ]
 
 
+class VtcRotary(C.Structure):
+    _fields_ = [("head_dim", C.c_int32), ("rotary_dim", C.c_int32), ("layout", C.c_int32), ("reserved", C.c_int32),
+                ("amplitude", C.c_double), ("frequency", C.POINTER(C.c_double))]
+
+
+class VtcHeads(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("x_batch", "x_row", "x_head", "y_batch", "y_row", "y_head")] + [
+        ("heads", C.c_int32), ("reserved", C.c_int32)]
+
+
+class VtcRows3(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("batch", C.c_int64), ("row", C.c_int64)]
+
+
 # every symbol include/vtc_amd.h declares: name -> (restype, argtypes)
 _i64p, _i32p, _f64p = C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.POINTER(C.c_double)
 SYMBOLS = {
@@ -86,6 +101,15 @@ SYMBOLS = {
     "vtc_profile_enable": (C.c_int, [C.c_void_p, C.c_int32]),
     "vtc_profile_read": (C.c_int, [C.c_void_p, _f64p, _i64p, _f64p, _f64p]),
     "vtc_profile_class_name": (C.c_char_p, [C.c_int32]),
+    "vtc_rotary_heads": (C.c_int, [C.c_int, C.c_int, C.POINTER(VtcRotary), C.c_int64, C.c_int64, C.POINTER(VtcHeads), C.c_int32,
+                                   C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_void_p]),
+    "vtc_group_norm_act_workspace": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    "vtc_group_norm_act": (C.c_int, [C.c_int, C.c_int, C.POINTER(VtcRows3), C.POINTER(VtcRows3), C.c_int64, C.c_int64, C.c_int32, C.c_int32,
+                                     C.c_void_p, C.c_void_p, C.c_int32, C.c_double, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                     C.c_void_p, C.c_int64, C.c_void_p]),
+    "vtc_group_norm_act_backward": (C.c_int, [C.c_int, C.c_int, C.POINTER(VtcRows3), C.POINTER(VtcRows3), C.POINTER(VtcRows3), C.c_int64,
+                                              C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
+                                              C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
 }
 
 LIB_PATH = Path(os.environ.get("VTC_AMD_LIB", Path(__file__).resolve().parent / "libvtc_amd.so"))
