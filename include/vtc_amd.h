@@ -296,6 +296,35 @@ int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows3* dy, cons
                                 int32_t act, const int32_t* lengths, const float* mean, const float* rstd, void* dweight /*[dev] or NULL*/,
                                 void* dbias /*[dev] or NULL*/, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Gated feed-forward block on rows of f16 / bf16 (sums in fp32): g = x W_gate^T + b_gate, u = x W_up^T + b_up,
+ * h = act(g) * u (NONE, GELU, SILU, SIGMOID), y = h W_down^T + b_down.  x [rows][width], W_gate and W_up [inner][width], W_down
+ * [out_width][inner] (as torch.nn.Linear keeps them), y [rows][out_width]; any sizes and row pitches (elements; operands whose
+ * rows are not made of aligned 16-byte pieces are copied into the workspace first).  Biases may be NULL; of the operands' type, or
+ * fp32 with bias_f32 = 1.  h, and with `saved` g, u and h for the backward call (vtc_gated_ffn_saved bytes, 256-byte aligned), are
+ * rounded to the operands' type.
+ * Backward: dy [rows][out_width] -> any of dx (row pitch dx_row), the weights' gradients (all three or none; dense, in the weights'
+ * layout and type) and the biases' (of the biases' type); NULL leaves one out.  dx may not overlap x or dy. */
+typedef struct {
+  const void* p; /* [dev] */
+  int64_t row;   /* elements between rows */
+} vtc_mat;
+typedef struct {
+  void* dx;
+  int64_t dx_row;
+  void *dw_gate, *dw_up, *dw_down;
+  void *db_gate, *db_up, *db_down;
+} vtc_ffn_grads;
+int64_t vtc_gated_ffn_workspace(int64_t rows, int32_t width, int32_t inner, int32_t out_width, int32_t backward);
+int64_t vtc_gated_ffn_saved(int64_t rows, int32_t inner);
+int vtc_gated_ffn(int device, int dtype, int64_t rows, int32_t width, int32_t inner, int32_t out_width, const vtc_mat* x,
+                  const vtc_mat* w_gate, const vtc_mat* w_up, const vtc_mat* w_down, const void* b_gate, const void* b_up, const void* b_down,
+                  int32_t bias_f32, int32_t act, const vtc_mat* y, void* saved, int64_t saved_bytes, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+int vtc_gated_ffn_backward(int device, int dtype, int64_t rows, int32_t width, int32_t inner, int32_t out_width, const vtc_mat* dy,
+                           const vtc_mat* x, const vtc_mat* w_gate, const vtc_mat* w_up, const vtc_mat* w_down, const void* saved,
+                           int64_t saved_bytes, int32_t bias_f32, int32_t act, const vtc_ffn_grads* grads, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -491,3 +491,270 @@ def test_group_norm_refusals_with_tensors():
             bad()
     with pytest.raises(L.VtcError, match="eps"):
         ops.group_norm_act(x, 2, eps=-1.0)
+
+
+# --------------------------------------------------------------------------------------------- gated feed-forward
+def ffn_64(x, wg, wu, wd, bg, bu, bd, act, dy=None):
+    x, wg, wu, wd = (t.double() for t in (x, wg, wu, wd))
+    z = lambda t: 0.0 if t is None else t.double()  # noqa: E731
+    g, u = x @ wg.t() + z(bg), x @ wu.t() + z(bu)
+    a, d = act_64(act, g)
+    h = a * u
+    out = {"y": h @ wd.t() + z(bd)}
+    if dy is not None:
+        dy = dy.double()
+        dh = dy @ wd
+        dg, du = dh * u * d, dh * a
+        out |= {"dx": dg @ wg + du @ wu, "dw_gate": dg.t() @ x, "dw_up": du.t() @ x, "dw_down": dy.t() @ h, "db_gate": dg.sum(0),
+                "db_up": du.sum(0), "db_down": dy.sum(0)}
+    return out
+
+
+def ffn_tolerances(x, wg, wu, wd, bg, bu, bd, act, dy, kind):
+    """Worst case of every rounding, carried through the formulas with absolute values.  e = half a step of the type for what is
+    stored between the products (h; g, u, dg, du in the backward pass), s = fp32 sums: at most n 2^-24 of the sum of magnitudes."""
+    e = torch.finfo(kind).eps / 2
+    tiny = torch.finfo(kind).smallest_normal * torch.finfo(kind).eps
+    x, wg, wu, wd = (t.double() for t in (x, wg, wu, wd))
+    z = lambda t: 0.0 if t is None else t.double()  # noqa: E731
+    m, k = x.shape
+    f, n = wd.shape[1], wd.shape[0]
+    s = lambda c: (c + 16) * 2.0 ** -24  # noqa: E731
+    at = act_tol(act, "bf16")
+    g, u = x @ wg.t() + z(bg), x @ wu.t() + z(bu)
+    ag, au = x.abs() @ wg.abs().t() + abs(z(bg)), x.abs() @ wu.abs().t() + abs(z(bu))
+    a, d = act_64(act, g)
+    eg, eu = ag * s(k), au * s(k)                        # g and u in fp32
+    ea = 1.13 * eg + at                                  # slopes of the activations are below 1.13
+    h = a * u
+    eh = ea * u.abs() + a.abs() * eu + ea * eu + e * h.abs() + tiny
+    tol = {"y": eh @ wd.abs().t() + (h.abs() + eh) @ wd.abs().t() * s(f) + abs(z(bd)) * 2.0 ** -24}
+    if dy is not None:
+        dy = dy.double()
+        egr, eur = eg + e * g.abs() + tiny, eu + e * u.abs() + tiny          # g and u as stored
+        dh, adh = dy @ wd, dy.abs() @ wd.abs()
+        edh = adh * s(n)
+        ed, ear = 1.2 * egr + at, 1.13 * egr + at                            # |act''| is below 1.2
+        dg, du = dh * u * d, dh * a
+        edg = edh * (u.abs() + eur) * (d.abs() + ed) + dh.abs() * (eur * (d.abs() + ed) + u.abs() * ed) + e * dg.abs() + tiny
+        edu = edh * (a.abs() + ear) + dh.abs() * ear + e * du.abs() + tiny
+        prod = lambda err, val, w: err @ w.abs() + (val.abs() + err) @ w.abs() * s(w.shape[0])  # noqa: E731
+        tol["dx"] = prod(edg, dg, wg) + prod(edu, du, wu)
+        tol["dw_gate"], tol["dw_up"] = prod(edg.t(), dg.t(), x), prod(edu.t(), du.t(), x)
+        tol["dw_down"] = prod(torch.zeros_like(dy.t()), dy.t(), h) + dy.abs().t() @ eh
+        tol["db_gate"], tol["db_up"] = edg.sum(0) + dg.abs().sum(0) * s(256), edu.sum(0) + du.abs().sum(0) * s(256)
+        tol["db_down"] = dy.abs().sum(0) * s(256)
+    return tol
+
+
+def make_ffn(kind, m, k, f, n, bias, seed=0, bias_kind=None):
+    g = torch.Generator(device="cuda").manual_seed(seed + m + 7 * k + 13 * f)
+    r = lambda *shape, std=1.0: (torch.randn(shape, generator=g, device="cuda") * std)  # noqa: E731
+    x, dy = r(m, k).to(kind), r(m, n).to(kind)
+    w = (r(f, k, std=k ** -0.5).to(kind), r(f, k, std=k ** -0.5).to(kind), r(n, f, std=f ** -0.5).to(kind))
+    b = tuple((r(c, std=0.3).to(bias_kind or kind) if bias else None) for c in (f, f, n))
+    return x, w, b, dy
+
+
+NAMES = ("dx", "dw_gate", "dw_up", "dw_down", "db_gate", "db_up", "db_down")
+
+
+def check_ffn(kind, x, w, b, act, dy, y, grads):
+    want = ffn_64(x, *w, *b, act, dy)
+    tol = ffn_tolerances(x, *w, *b, act, dy, kind)
+    for name, got in (("y", y),) + tuple(zip(NAMES, grads or ())):
+        if got is not None:
+            ref = want[name].cpu()
+            close(got, ref, half_step(got.dtype, ref) + tol[name].cpu() * 1.001, name)
+
+
+FFN_SIZES = [(1, 64, 64, 64), (1, 8, 8, 8), (3, 1, 1, 1), (16, 768, 2048, 768), (17, 40, 72, 24), (33, 389, 131, 77), (64, 256, 512, 256),
+             (65, 256, 512, 256), (200, 64, 128, 192), (257, 129, 250, 311), (511, 768, 512, 768), (1030, 100, 300, 50), (2048, 192, 384, 192)]
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("m,k,f,n", FFN_SIZES)
+def test_gated_ffn_forward_and_backward(kind, m, k, f, n):
+    act = ("silu", "gelu", "sigmoid", "none")[(m + f) % 4]
+    bias = (m + k) % 3 != 0
+    x, w, b, dy = make_ffn(TYPES[kind], m, k, f, n, bias)
+    y, saved = ops.gated_ffn_forward(x, *w, *b, act=act, save=True)
+    y2, none = ops.gated_ffn_forward(x, *w, *b, act=act)
+    assert none is None and torch.equal(y, y2)
+    grads = ops.gated_ffn_backward(dy, x, *w, saved, act=act, biases=bias)
+    check_ffn(TYPES[kind], x, w, b, act, dy, y, grads)
+
+
+@gpu
+@pytest.mark.parametrize("act", ["none", "gelu", "silu", "sigmoid"])
+@pytest.mark.parametrize("m", [5, 300])
+def test_gated_ffn_activations_and_fp32_biases(act, m):
+    x, w, b, dy = make_ffn(torch.float16, m, 96, 160, 96, True, bias_kind=torch.float32)
+    y, saved = ops.gated_ffn_forward(x, *w, *b, act=act, save=True)
+    grads = ops.gated_ffn_backward(dy, x, *w, saved, act=act, bias_dtype=torch.float32)
+    check_ffn(torch.float16, x, w, b, act, dy, y, grads)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 40, 700])
+def test_gated_ffn_strides_shapes_and_partial_gradients(m):
+    kind = torch.bfloat16
+    x, w, b, dy = make_ffn(kind, m, 96, 160, 64, True)
+    want, saved = ops.gated_ffn_forward(x, *w, *b, save=True)
+    grads = ops.gated_ffn_backward(dy, x, *w, saved)
+    wide = torch.zeros((m, 3 * 96), dtype=kind, device="cuda")
+    wide[:, 96:192] = x
+    for view in (wide[:, 96:192], torch.cat([x, x], 1)[:, :96]):               # rows that are further apart
+        assert torch.equal(ops.gated_ffn_forward(view, *w, *b)[0], want)
+    off = torch.zeros(m * 96 + 1, dtype=kind, device="cuda")[1:].view(m, 96)    # rows that are not aligned to 16 bytes
+    off.copy_(x)
+    wide_w = torch.zeros((160, 2, 96), dtype=kind, device="cuda")               # gate and up interleaved row by row
+    wide_w[:, 0], wide_w[:, 1] = w[0], w[1]
+    odd_w = torch.zeros(64 * 163 + 1, dtype=kind, device="cuda")[1:].view(64, 163)[:, :160]
+    odd_w.copy_(w[2])
+    y, s2 = ops.gated_ffn_forward(off, wide_w[:, 0], wide_w[:, 1], odd_w, *b, save=True)
+    assert torch.equal(y, want)
+    for a, c in zip(ops.gated_ffn_backward(dy, off, wide_w[:, 0], w[1].clone(), odd_w, s2), grads):
+        assert torch.equal(a, c)
+    y3 = ops.gated_ffn(x.view(1, m, 1, 96), *w, *b)
+    assert y3.shape == (1, m, 1, 64) and torch.equal(y3.view(m, 64), want)
+    for kw in (dict(need_dx=False), dict(need_dw=False), dict(biases=False)):
+        got = ops.gated_ffn_backward(dy, x, *w, saved, **kw)
+        for i, (a, c) in enumerate(zip(got, grads)):
+            gone = (i == 0 and "need_dx" in kw) or (1 <= i <= 3 and "need_dw" in kw) or (i >= 4 and "biases" in kw)
+            assert a is None if gone else torch.equal(a, c)
+    y, s = ops.gated_ffn_forward(x[:0], *w, *b, save=True)
+    assert y.shape == (0, 64)
+    assert not any(t.any() for t in ops.gated_ffn_backward(dy[:0], x[:0], *w, s)[1:])
+
+
+@gpu
+def test_gated_ffn_rows_do_not_reach_each_other():
+    """An infinite row stays alone, in every kernel the rows can take; so do rows next to the end of a tile."""
+    for m in (40, 300):
+        x, w, b, _ = make_ffn(torch.float16, m, 100, 132, 60, True)
+        want = ops.gated_ffn(x, *w, *b)
+        x[7] = float("nan")
+        got = ops.gated_ffn(x, *w, *b)
+        assert got[7].isnan().all() and torch.equal(got[:7], want[:7]) and torch.equal(got[8:], want[8:])
+
+
+@gpu
+def test_gated_ffn_differentiable_call_formula_and_differences():
+    x, w, b, dy = make_ffn(torch.float16, 70, 48, 64, 40, True)
+    leaves = [t.detach().clone().requires_grad_() for t in (x,) + w + b]
+    y = ops.gated_ffn(*leaves, act="gelu")
+    grads = torch.autograd.grad(y, leaves, dy)
+    check_ffn(torch.float16, x, w, b, "gelu", dy, y.detach(), grads)
+    only = ops.gated_ffn(x, w[0], w[1], w[2], leaves[4], None, None, act="gelu")
+    (db,) = torch.autograd.grad(only, (leaves[4],), dy)
+    assert db.shape == (64,)
+    # central differences of the 64-bit definition along a direction, against the returned gradients
+    g = torch.Generator(device="cuda").manual_seed(11)
+    tol = ffn_tolerances(x, *w, *b, "gelu", dy, torch.float16)
+    base = [t.double() for t in (x,) + w + b]
+    for i, name in enumerate(NAMES):
+        v = torch.randn(base[i].shape, generator=g, device="cuda", dtype=torch.float64)
+        f = [float((ffn_64(*(t + (s * v if j == i else 0) for j, t in enumerate(base)), "gelu")["y"] * dy.double()).sum()) for s in (1e-4, -1e-4)]
+        num, ana = (f[0] - f[1]) / 2e-4, float((grads[i].double() * v).sum())
+        room = float(((tol[name] + half_step(torch.float16, grads[i].double())) * v.abs()).sum())
+        assert abs(num - ana) <= room + 1e-5 * abs(num) + 1e-4, (name, num, ana, room)   # 64-bit differences: 1e-16 / 1e-4 and 1e-8 of f'''
+
+
+@gpu
+def test_gated_ffn_long_contraction_offsets_beyond_32_bits():
+    """rows x inner beyond 2^31 elements: the last rows and the sums over all of them are right."""
+    m, k, f, n = 1_100_000, 8, 2048, 8
+    g = torch.Generator(device="cuda").manual_seed(12)
+    kind = torch.bfloat16
+    x = torch.zeros((m, k), dtype=kind, device="cuda")
+    dy = torch.zeros((m, n), dtype=kind, device="cuda")
+    x[-300:], dy[-300:] = torch.randn((300, k), generator=g, device="cuda").to(kind), torch.randn((300, n), generator=g, device="cuda").to(kind)
+    w = tuple((torch.randn(s, generator=g, device="cuda") * s[1] ** -0.5).to(kind) for s in ((f, k), (f, k), (n, f)))
+    y, saved = ops.gated_ffn_forward(x, *w, save=True)
+    grads = ops.gated_ffn_backward(dy, x, *w, saved, biases=False)
+    assert not y[:-300].any() and not grads[0][:-300].any()
+    check_ffn(kind, x[-300:], w, (None,) * 3, "silu", dy[-300:], y[-300:], (grads[0][-300:],) + grads[1:4])
+
+
+@gpu
+def test_gated_ffn_in_a_graph():
+    x, w, b, dy = make_ffn(torch.bfloat16, 600, 136, 200, 136, True)
+
+    def step():
+        y, saved = ops.gated_ffn_forward(x, *w, *b, act="gelu", save=True)
+        small = ops.gated_ffn_forward(x[:9], *w, *b, act="gelu")[0]
+        return (y, small) + ops.gated_ffn_backward(dy, x, *w, saved, act="gelu")
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        x.mul_(-0.9)
+        want = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        assert all(torch.equal(a, c) for a, c in zip(out, want))
+        (out[0].float() * 2).sum().item()
+
+
+def _ffn_c(backward=False, **over):
+    a = dict(dtype=1, m=100, k=64, f=128, n=64, f32=0, act=2, x=L.VtcMat(1 << 20, 64), wg=L.VtcMat(2 << 20, 64), wu=L.VtcMat(3 << 20, 64),
+             wd=L.VtcMat(4 << 20, 128), y=L.VtcMat(5 << 20, 64), saved=6 << 20, saved_size=1 << 20, ws=8 << 20, size=1 << 30, dx=7 << 20, dx_row=64, dw=1 << 28,
+             dw2=1 << 28)
+    a.update(over)
+    ref = lambda s: None if s is None else C.byref(s)  # noqa: E731
+    so = L.load()
+    mats = [ref(a[n]) for n in ("x", "wg", "wu", "wd")]
+    if backward:
+        grads = L.VtcFfnGrads(a["dx"], a["dx_row"], a["dw"], a["dw2"], a["dw"])
+        rc = so.vtc_gated_ffn_backward(0, a["dtype"], a["m"], a["k"], a["f"], a["n"], ref(a["y"]), *mats, a["saved"], a["saved_size"], a["f32"], a["act"],
+                                       C.byref(grads), a["ws"], a["size"], None)
+    else:
+        rc = so.vtc_gated_ffn(0, a["dtype"], a["m"], a["k"], a["f"], a["n"], *mats, None, None, None, a["f32"], a["act"], ref(a["y"]), a["saved"],
+                              a["saved_size"], a["ws"], a["size"], None)
+    return rc, L.last_error(None)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("over,text,code", [
+    (dict(dtype=0), "f16 or bf16", L.ERR_ARG), (dict(act=4), "activation", L.ERR_ARG), (dict(f32=2), "bias_f32", L.ERR_ARG),
+    (dict(m=-1), "rows", L.ERR_ARG), (dict(m=1 << 31), "rows", L.ERR_ARG), (dict(k=0), "width", L.ERR_ARG), (dict(f=(1 << 18) + 1), "width", L.ERR_ARG),
+    (dict(x=None), "x is null", L.ERR_ARG), (dict(wg=L.VtcMat(None, 64)), "w_gate is null", L.ERR_ARG), (dict(wd=L.VtcMat(4 << 20, 127)), "pitch", L.ERR_ARG),
+    (dict(x=L.VtcMat(1 << 20, (1 << 20) + 1)), "pitch", L.ERR_ARG), (dict(x=L.VtcMat((1 << 20) + 1, 64)), "aligned", L.ERR_ARG),
+    (dict(y=L.VtcMat(5 << 20, 63)), "pitch", L.ERR_ARG), (dict(size=10, x=L.VtcMat((1 << 20) + 2, 64)), "workspace", L.ERR_CAPACITY),
+    (dict(saved_size=10), "saved", L.ERR_CAPACITY), (dict(ws=(8 << 20) + 16), "256", L.ERR_ARG), (dict(saved=(6 << 20) + 16), "256", L.ERR_ARG)])
+def test_gated_ffn_refusals_of_the_library(backward, over, text, code):
+    rc, msg = _ffn_c(backward, **over)
+    assert rc == code and text in msg, (rc, msg)
+
+
+def test_gated_ffn_refusals_of_one_direction():
+    for backward, over, text in ((False, dict(y=L.VtcMat((1 << 20) + 64, 64)), "overlaps x"), (True, dict(dx=1 << 20), "overlaps"),
+                                 (True, dict(dx=5 << 20), "overlaps"), (True, dict(dx_row=63), "pitch"), (True, dict(dw=None), "go together"),
+                                 (True, dict(m=0), "no rows"), (True, dict(dx=(7 << 20) + 1), "aligned")):
+        rc, msg = _ffn_c(backward, **over)
+        assert rc == L.ERR_ARG and text in msg, (rc, msg)
+    so = L.load()
+    assert so.vtc_gated_ffn_workspace(10, 0, 8, 8, 0) == L.ERR_ARG and so.vtc_gated_ffn_workspace(0, 8, 8, 8, 1) == 0
+    assert so.vtc_gated_ffn_saved(-1, 8) == L.ERR_ARG
+
+
+@gpu
+def test_gated_ffn_refusals_with_tensors():
+    x, w, b, dy = make_ffn(torch.float16, 6, 16, 24, 8, True)
+    y, saved = ops.gated_ffn_forward(x, *w, *b, save=True)
+    for bad in (lambda: ops.gated_ffn(x.float(), *w), lambda: ops.gated_ffn(x, w[0].bfloat16(), w[1], w[2]), lambda: ops.gated_ffn(x[:, :8], *w),
+                lambda: ops.gated_ffn(x, w[0], w[1][:8], w[2]), lambda: ops.gated_ffn(x, w[0], w[1], w[2].t()), lambda: ops.gated_ffn(x, *w, act="relu"),
+                lambda: ops.gated_ffn(x, w[0].t().contiguous().t(), w[1], w[2]), lambda: ops.gated_ffn(x, *w, b[0][:4]),
+                lambda: ops.gated_ffn(x, *w, b[0], b[1].float()), lambda: ops.gated_ffn(x.cpu(), *w), lambda: ops.gated_ffn_backward(dy, x, *w, None),
+                lambda: ops.gated_ffn_backward(dy[:3], x, *w, saved), lambda: ops.gated_ffn_backward(dy, x, *w, saved[:100]),
+                lambda: ops.gated_ffn_backward(dy, x, *w, saved, bias_dtype=torch.bfloat16)):
+        with pytest.raises(ValueError):
+            bad()

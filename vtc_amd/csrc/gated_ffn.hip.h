@@ -1,0 +1,184 @@
+// Gated feed-forward block: g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) u, y = h Wd^T + bd, and its gradients
+//   dh = dy Wd, dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h.
+//
+// Both projections, the activation and the product are one kernel: a tile holds the same columns of W_gate (first half) and W_up
+// (second half), so a lane's two accumulators are g and u of the same elements and only h leaves the chip (g and u as well when a
+// backward pass will want them).  Backward: dh never exists in memory (its tile turns into dg and du in the epilogue).
+// Rounding: h, and for the backward pass g, u, dg, du, are stored in the operands' 16-bit type, since they are operands of the
+// next matrix product; every sum is fp32 (fp64 where K-split partials and column sums are joined).
+//
+// Few rows (at most 64: single frames, live streams) are bound by reading the weights once, and by latency: skinny_kernel
+// below.  Everything else runs on op_gemm_kernel.
+#pragma once
+#include "common.hip.h"
+#include "op_act.hip.h"
+#include "op_gemm.hip.h"
+
+namespace vtc {
+
+// rows x cols of src, zero-filled to dcols columns (a multiple of 8): operands whose rows are not made of aligned 16-byte pieces
+__global__ __launch_bounds__(256) void pad_copy_kernel(const h16* src, long long lds_, h16* dst, long long rows, int cols, int dcols) {
+  const int pieces = dcols / 8;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * pieces; i += (long long)gridDim.x * 256) {
+    const long long r = i / pieces;
+    const int c = (int)(i - r * pieces) * 8;
+    u16x8 v;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? src[r * lds_ + c + k] : (h16)0;
+    *(u16x8*)(dst + r * dcols + c) = v;
+  }
+}
+
+// column sums of 256 rows (dy -> partial sums of d b_down); part [blocks of rows][pitch]
+template <bool F16>
+__global__ __launch_bounds__(256) void colsum_kernel(const h16* x, long long ld, float* part, int pitch, long long rows, int cols) {
+  __shared__ float red[4][64 * 8];
+  const int v = blockIdx.y * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const long long r0 = (long long)blockIdx.x * 256, r1 = min(rows, r0 + 256);
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (v * 8 < cols)
+#pragma unroll 4
+    for (long long r = r0 + w; r < r1; r += 4) {
+      const u16x8 f = *(const u16x8*)(x + r * ld + v * 8);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[k] += from_h16<F16>(f[k]);
+    }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) red[w][(threadIdx.x & 63) * 8 + k] = s[k];
+  __syncthreads();
+  if (w == 0 && v * 8 < pitch)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = threadIdx.x * 8 + k;
+      part[(long long)blockIdx.x * pitch + v * 8 + k] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+    }
+}
+
+struct ColReduce { const float* part; void* out; long long n; int pitch, cols; };
+// bias gradients: out[c] = sum over n partial rows, in order, fp64; up to three of them in one launch (blockIdx.y)
+struct ColReduceParams { ColReduce r[3]; int f16, out_f32; };
+__global__ __launch_bounds__(256) void col_reduce_kernel(const ColReduceParams p) {
+  __shared__ double red[4][64];
+  const ColReduce& q = p.r[blockIdx.y];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  double s = 0.0;
+  if (c < q.cols)
+    for (long long i = w; i < q.n; i += 4) s += (double)q.part[i * q.pitch + c];
+  red[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w || c >= q.cols) return;
+  const float v = (float)((red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]));
+  if (p.out_f32) ((float*)q.out)[c] = v;
+  else ((h16*)q.out)[c] = p.f16 ? to_h16<true>(v) : to_h16<false>(v);
+}
+
+// K-split partials -> 16-bit result; up to three matrices in one launch
+struct SplitReduce { const float* part; h16* out; long long ldo, pitch, rows; int cols, vec; };
+struct SplitReduceParams { SplitReduce r[3]; int n, splits; long long stride; };
+template <bool F16>
+__global__ __launch_bounds__(256) void split_reduce_kernel(const SplitReduceParams p) {
+  const SplitReduce& q = p.r[blockIdx.y];
+  const long long pieces = q.pitch / 4;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < q.rows * pieces; i += (long long)gridDim.x * 256) {
+    const long long r = i / pieces;
+    const int c = (int)(i - r * pieces) * 4;
+    if (c >= q.cols) continue;
+    const float* src = q.part + r * q.pitch + c;
+    float4 s = *(const float4*)src;
+    for (int k = 1; k < p.splits; ++k) {
+      const float4 t = *(const float4*)(src + k * p.stride);
+      s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+    }
+    h16* o = q.out + r * q.ldo + c;
+    if (q.vec) {
+      typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+      *(u32x2*)o = u32x2{pack2<F16>(s.x, s.y), pack2<F16>(s.z, s.w)};
+    } else {
+      const float v[4] = {s.x, s.y, s.z, s.w};
+      for (int k = 0; k < 4 && c + k < q.cols; ++k) o[k] = to_h16<F16>(v[k]);
+    }
+  }
+}
+
+// ---- few rows: C[M <= 16 MT][N] = A W^T.  A block owns 16 columns, its 8 waves take every 8th K step of 32 straight from global
+// memory (the weights are read once, by nobody else), their partial tiles meet in LDS.  MFMA computes C^T: lane (fr, fq) holds
+// row fr of A and columns 4 fq .. + 4.
+struct SkinnyParams {
+  const h16 *x, *w0, *w1;     // w1: W_up (GATE)
+  long long ldx, ldw;
+  int M, K, N, Nb;            // N: columns written (padding included), Nb: rows of w
+  const void *b0, *b1;
+  int bias_f32, act, cvec;
+  h16 *out, *g, *u;
+  long long ldo;
+};
+template <bool F16, int MT, bool GATE>
+__global__ __launch_bounds__(512) void skinny_kernel(const SkinnyParams p) {
+  constexpr int NW = GATE ? 2 : 1;
+  __shared__ float part[8][NW * MT * 256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int fr = lane & 15, fq = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int rows_w = min(16, p.Nb - n0);
+  constexpr unsigned OOB = 0x80000000u;
+  auto rsrc = [&](const h16* b, long long ld, int rows) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, rows > 0 ? (int)(((rows - 1) * ld + ((p.K + 7) & ~7)) * 2) : 0, 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t r0 = rsrc(p.w0 + n0 * p.ldw, p.ldw, rows_w), r1 = GATE ? rsrc(p.w1 + n0 * p.ldw, p.ldw, rows_w) : r0;
+  const __amdgpu_buffer_rsrc_t rx = rsrc(p.x, p.ldx, p.M);
+  const unsigned vw = (unsigned)(fr * (int)p.ldw * 2), vx = (unsigned)(fr * (int)p.ldx * 2), stepx = (unsigned)(16 * (int)p.ldx * 2);
+  f32x4 acc[NW][MT];
+#pragma unroll
+  for (int w = 0; w < NW; ++w)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[w][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int steps = (p.K + 31) / 32;
+  constexpr int D = MT == 4 ? 2 : 4;            // K steps in flight; steps behind the end read as zero
+  for (int s0 = wave; s0 < steps; s0 += 8 * D) {
+    u16x8 a[D][NW], b[D][MT];
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      const int k = (s0 + 8 * j) * 32 + fq * 8;
+      const unsigned ko = k < p.K ? (unsigned)k * 2u : OOB;   // OOB + any row offset stays out of range (below 2^30 each)
+      a[j][0] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(r0, vw + ko, 0, 0));
+      if constexpr (GATE) a[j][1] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(r1, vw + ko, 0, 0));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) b[j][m] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(rx, vx + m * stepx + ko, 0, 0));
+    }
+#pragma unroll
+    for (int j = 0; j < D; ++j)
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[w][m] = mfma16<F16>(a[j][w], b[j][m], acc[w][m]);
+  }
+#pragma unroll
+  for (int w = 0; w < NW; ++w)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) *(f32x4*)&part[wave][(w * MT + m) * 256 + fr * 16 + fq * 4] = acc[w][m];   // [row][column]
+  __syncthreads();
+  for (int i = threadIdx.x; i < MT * 256; i += 512) {
+    const int r = i >> 4, c = i & 15, col = n0 + c;
+    float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      v0 += part[w][i];
+      if constexpr (GATE) v1 += part[w][MT * 256 + i];
+    }
+    if (r >= p.M || col >= p.N) continue;
+    if (col < p.Nb) v0 += op_bias(p.b0, col, p.bias_f32, F16);
+    if constexpr (GATE) {
+      if (col < p.Nb) v1 += op_bias(p.b1, col, p.bias_f32, F16);
+      if (p.g) { p.g[r * p.ldo + col] = to_h16<F16>(v0); p.u[r * p.ldo + col] = to_h16<F16>(v1); }
+      float a;
+      if (p.act == ACT_GELU) a = op_act<ACT_GELU, false>(v0);
+      else if (p.act == ACT_SILU) a = op_act<ACT_SILU, false>(v0);
+      else if (p.act == ACT_SIGMOID) a = op_act<ACT_SIGMOID, false>(v0);
+      else a = v0;
+      v0 = a * v1;
+    }
+    p.out[r * p.ldo + col] = to_h16<F16>(v0);
+  }
+}
+
+}  // namespace vtc

@@ -7,6 +7,7 @@
 #include <cstring>
 
 #include "../../include/vtc_amd.h"
+#include "gated_ffn.hip.h"
 #include "groupnorm.hip.h"
 #include "ops.h"
 #include "rotary.hip.h"
@@ -371,4 +372,345 @@ extern "C" int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows
     });
   });
   return launched("group norm backward");
+}
+
+// ===================================================================================== gated feed-forward
+namespace {
+
+constexpr int64_t kFfnMaxDim = 1 << 18;   // width, inner width: tile offsets stay far below 2^31 bytes
+constexpr int kSkinnyRows = 64;
+constexpr long long kMaxPitch = 1 << 20;  // elements between rows of a matrix
+
+// Carves a workspace; with base == null it only measures.
+struct Arena {
+  char* base;
+  size_t used = 0;
+  template <typename T> T* take(size_t n) {
+    T* p = base ? (T*)(base + used) : nullptr;
+    used += align256(n * sizeof(T));
+    return p;
+  }
+};
+int up8(int64_t n) { return (int)((n + 7) & ~(int64_t)7); }
+
+struct FfnArgs {
+  int dtype, act, bias_f32;
+  int64_t M;
+  int K, F, N;
+  const vtc_mat *x, *wg, *wu, *wd;
+  const void *bg, *bu, *bd;
+};
+
+int ffn_check_mat(const char* what, const char* name, const vtc_mat* m, int64_t rows, int cols) {
+  if (!m || !m->p) return fail_handleless(VTC_ERR_ARG, "%s: %s is null", what, name);
+  if (m->row < cols || m->row > kMaxPitch) return fail_handleless(VTC_ERR_ARG, "%s: %s has a row pitch of %lld for %d columns (at most %lld)", what, name, (long long)m->row, cols, kMaxPitch);
+  if ((uintptr_t)m->p % 2) return fail_handleless(VTC_ERR_ARG, "%s: %s is not aligned to its type", what, name);
+  (void)rows;
+  return VTC_OK;
+}
+int ffn_check(const char* what, const FfnArgs& a) {
+  if (a.dtype != OP_F16 && a.dtype != OP_BF16) return fail_handleless(VTC_ERR_ARG, "%s: operands are f16 or bf16 (matrix instructions with fp32 sums), got type %d", what, a.dtype);
+  if (a.act < ACT_NONE || a.act > ACT_SIGMOID) return fail_handleless(VTC_ERR_ARG, "%s: unknown activation %d", what, a.act);
+  if (a.bias_f32 != 0 && a.bias_f32 != 1) return fail_handleless(VTC_ERR_ARG, "%s: bias_f32 must be 0 or 1", what);
+  if (a.M < 0 || a.M > (1ll << 31) - 256) return fail_handleless(VTC_ERR_ARG, "%s: %lld rows not in 0..2^31 - 256", what, (long long)a.M);
+  for (int64_t d : {(int64_t)a.K, (int64_t)a.F, (int64_t)a.N})
+    if (d < 1 || d > kFfnMaxDim) return fail_handleless(VTC_ERR_ARG, "%s: width %lld not in 1..%lld", what, (long long)d, (long long)kFfnMaxDim);
+  if (int rc = ffn_check_mat(what, "x", a.x, a.M, a.K)) return rc;
+  if (int rc = ffn_check_mat(what, "w_gate", a.wg, a.F, a.K)) return rc;
+  if (int rc = ffn_check_mat(what, "w_up", a.wu, a.F, a.K)) return rc;
+  if (int rc = ffn_check_mat(what, "w_down", a.wd, a.N, a.F)) return rc;
+  return VTC_OK;
+}
+bool pieces_ok(const vtc_mat* m, int cols) { return cols % 8 == 0 && m->row % 8 == 0 && (uintptr_t)m->p % 16 == 0; }
+
+// An operand made of aligned 16-byte pieces: the caller's memory where it is, a padded copy in the workspace where it is not.
+OpMat operand(Arena& ar, const vtc_mat* m, int64_t rows, int cols, bool force, hipStream_t s, bool launch) {
+  if (!force && pieces_ok(m, cols)) return OpMat{(const h16*)m->p, m->row};
+  const int d = up8(cols);
+  h16* c = ar.take<h16>((size_t)rows * d);
+  if (launch && rows > 0) {
+    const long long n = rows * (d / 8);
+    hipLaunchKernelGGL(pad_copy_kernel, dim3((unsigned)std::min<long long>((n + 255) / 256, 65536)), dim3(256), 0, s, (const h16*)m->p, (long long)m->row, c,
+                       (long long)rows, cols, d);
+  }
+  return OpMat{c, d};
+}
+
+// Column-group width of a product's tile order: see launch_gemm256
+int group_of(int tiles_m, int tiles_n, double a_bytes, double w_bytes, double w_group_bytes) {
+  const double rounds = (double)tiles_m * tiles_n / 256.0;
+  double best = 1e300;
+  int r = tiles_n;
+  for (int g = 1; g <= tiles_n; ++g) {
+    if (tiles_n % g) continue;
+    const bool fits = g * w_group_bytes <= 2.5e6;
+    const double est = a_bytes * (tiles_n / g) + w_bytes * 8.0 * (fits ? 1.0 : (rounds > 1.0 ? rounds : 1.0));
+    if (est < best) { best = est; r = g; }
+  }
+  return r;
+}
+
+void finish_prob(OpProb& q, int bn, int K, int tile0) {
+  q.tiles_m = (q.M + 255) / 256;
+  q.tiles_n = (q.N + bn - 1) / bn;
+  q.group_n = group_of(q.tiles_m, q.tiles_n, 2.0 * q.M * K, 2.0 * q.N * K, 2.0 * bn * K);
+  q.tile0 = tile0;
+}
+void set_k(OpGemmParams& p, int k0, int k1 = 0) {
+  p.K[0] = k0; p.K[1] = k1;
+  p.nk0 = (k0 + 63) / 64;
+  p.nk = (p.nk0 + (k1 + 63) / 64 + 1) & ~1;   // the kernel takes K-tiles in pairs; one behind the end reads as zero
+  if (!k1) p.nk0 = p.nk;
+  p.splits = 1; p.kps = p.nk;
+}
+template <bool F16, bool AKS, bool BKS, int EPI, int BN> void launch_op_gemm(OpGemmParams& p, hipStream_t s) {
+  const int units = p.ntiles * p.splits;
+  hipLaunchKernelGGL((op_gemm_kernel<F16, AKS, BKS, EPI, BN>), dim3((unsigned)std::min(units, 256)), dim3(512), 0, s, p);
+}
+template <typename F> void by_f16(int dtype, F&& f) {
+  if (dtype == OP_F16) f(std::true_type{});
+  else f(std::false_type{});
+}
+
+size_t ffn_forward(const FfnArgs& a, const vtc_mat* y, h16* save_g, h16* save_u, h16* save_h, char* ws, bool launch, hipStream_t s) {
+  Arena ar{ws};
+  const int F8 = up8(a.F);
+  const OpMat x = operand(ar, a.x, a.M, a.K, false, s, launch);
+  // gate and up share one pitch in the kernel
+  const bool copy_w = a.wg->row != a.wu->row || !pieces_ok(a.wg, a.K) || !pieces_ok(a.wu, a.K);
+  const OpMat wg = operand(ar, a.wg, a.F, a.K, copy_w, s, launch), wu = operand(ar, a.wu, a.F, a.K, copy_w, s, launch);
+  const OpMat wd = operand(ar, a.wd, a.N, a.F, false, s, launch);
+  h16* h = save_h ? save_h : ar.take<h16>((size_t)a.M * F8);
+  if (!launch) return ar.used;
+  const int cvec = a.N % 8 == 0 && y->row % 8 == 0 && (uintptr_t)y->p % 16 == 0;
+  by_f16(a.dtype, [&](auto f) {
+    constexpr bool F16 = decltype(f)::value;
+    if (a.M <= kSkinnyRows) {
+      SkinnyParams p{};
+      p.x = x.p; p.ldx = x.ld; p.w0 = wg.p; p.w1 = wu.p; p.ldw = wg.ld;
+      p.M = (int)a.M; p.K = a.K; p.N = F8; p.Nb = a.F; p.b0 = a.bg; p.b1 = a.bu; p.bias_f32 = a.bias_f32; p.act = a.act;
+      p.out = h; p.g = save_g; p.u = save_u; p.ldo = F8;
+      SkinnyParams d{};
+      d.x = h; d.ldx = F8; d.w0 = d.w1 = wd.p; d.ldw = wd.ld;
+      d.M = (int)a.M; d.K = a.F; d.N = d.Nb = a.N; d.b0 = a.bd; d.bias_f32 = a.bias_f32; d.out = (h16*)y->p; d.ldo = y->row;
+      auto go = [&](auto mt) {
+        constexpr int MT = decltype(mt)::value;
+        hipLaunchKernelGGL((skinny_kernel<F16, MT, true>), dim3((unsigned)((F8 + 15) / 16)), dim3(512), 0, s, p);
+        hipLaunchKernelGGL((skinny_kernel<F16, MT, false>), dim3((unsigned)((a.N + 15) / 16)), dim3(512), 0, s, d);
+      };
+      if (a.M <= 16) go(std::integral_constant<int, 1>{});
+      else if (a.M <= 32) go(std::integral_constant<int, 2>{});
+      else go(std::integral_constant<int, 4>{});
+      return;
+    }
+    OpGemmParams p{};
+    p.nprob = 1;
+    OpProb& q = p.prob[0];
+    q.a[0] = x; q.b[0] = wg; q.b[1] = wu; q.c = h; q.ldc = F8; q.M = (int)a.M; q.N = F8; q.Nb = a.F; q.cvec = 1;
+    finish_prob(q, 128, a.K, 0);
+    p.ntiles = q.tiles_m * q.tiles_n;
+    set_k(p, a.K);
+    p.bias = a.bg; p.bias2 = a.bu; p.bias_f32 = a.bias_f32; p.act = a.act; p.g = save_g; p.u = save_u; p.ldg = F8;
+    launch_op_gemm<F16, false, false, OG_GATE, 256>(p, s);
+    OpGemmParams d{};
+    d.nprob = 1;
+    OpProb& e = d.prob[0];
+    e.a[0] = OpMat{h, F8}; e.b[0] = wd; e.c = (void*)y->p; e.ldc = y->row; e.M = (int)a.M; e.N = e.Nb = a.N; e.cvec = cvec;
+    finish_prob(e, 192, a.F, 0);
+    d.ntiles = e.tiles_m * e.tiles_n;
+    set_k(d, a.F);
+    d.bias = a.bd; d.bias_f32 = a.bias_f32;
+    launch_op_gemm<F16, false, false, OG_PLAIN, 192>(d, s);
+  });
+  return ar.used;
+}
+
+// K splits of the weights' gradients: few output tiles, a long contraction over the rows.  Enough units for every CU, no split
+// shorter than 8 K-tiles (512 rows: below that the fp32 partials cost more than they save).
+void ffn_splits(int tiles, int nk, int* splits, int* kps) {
+  int best = 1;
+  double cost = 1e300;
+  for (int sp = 1; sp <= 64; ++sp) {
+    const int k = (((nk + sp - 1) / sp) + 1) & ~1;
+    const int real = (nk + k - 1) / k;
+    if (real != sp || (sp > 1 && k < 8)) continue;
+    const double rounds = std::ceil((double)tiles * sp / 256.0);
+    const double c = rounds * (k + 4.0) + 0.35 * sp * tiles / 256.0 * 4.0;   // K-tile times; a tile's partial costs ~1.4 of them to write and read
+    if (c < cost) { cost = c; best = sp; }
+  }
+  *kps = (((nk + best - 1) / best) + 1) & ~1;
+  *splits = best;
+}
+
+size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const h16* g, const h16* u, const h16* h, const vtc_ffn_grads* o, char* ws, bool launch, hipStream_t s) {
+  Arena ar{ws};
+  const int K8 = up8(a.K), F8 = up8(a.F), N8 = up8(a.N);
+  const int M = (int)a.M;
+  const OpMat x = operand(ar, a.x, a.M, a.K, false, s, launch), y = operand(ar, dy, a.M, a.N, false, s, launch);
+  const bool copy_w = a.wg->row != a.wu->row || !pieces_ok(a.wg, a.K) || !pieces_ok(a.wu, a.K);
+  const OpMat wg = operand(ar, a.wg, a.F, a.K, copy_w, s, launch), wu = operand(ar, a.wu, a.F, a.K, copy_w, s, launch);
+  const OpMat wd = operand(ar, a.wd, a.N, a.F, false, s, launch);
+  h16 *dg = ar.take<h16>((size_t)a.M * F8), *du = ar.take<h16>((size_t)a.M * F8);
+  const int tiles_m = (M + 255) / 256, row_blocks = (M + 255) / 256;
+  float* cs_f = (o->db_gate || o->db_up) || !launch ? ar.take<float>((size_t)2 * 2 * tiles_m * F8) : nullptr;
+  float* cs_n = o->db_down || !launch ? ar.take<float>((size_t)row_blocks * N8) : nullptr;
+  // weights' gradients
+  OpGemmParams w{};
+  w.nprob = 3;
+  const h16* as[3] = {dg, du, y.p};
+  const long long lda[3] = {F8, F8, y.ld};
+  const h16* bs[3] = {x.p, x.p, h};
+  const long long ldb[3] = {x.ld, x.ld, F8};
+  const int rows[3] = {a.F, a.F, a.N}, cols[3] = {a.K, a.K, a.F}, pitch[3] = {K8, K8, F8};
+  int tiles = 0;
+  for (int i = 0; i < 3; ++i) {
+    OpProb& q = w.prob[i];
+    q.a[0] = OpMat{as[i], lda[i]}; q.b[0] = OpMat{bs[i], ldb[i]};
+    q.M = rows[i]; q.N = pitch[i]; q.Nb = cols[i]; q.ldc = pitch[i];
+    finish_prob(q, 256, M, tiles);
+    tiles += q.tiles_m * q.tiles_n;
+  }
+  w.ntiles = tiles;
+  set_k(w, M);
+  ffn_splits(tiles, w.nk, &w.splits, &w.kps);
+  const long long one = (long long)a.F * K8;
+  w.split_stride = 2 * one + (long long)a.N * F8;
+  float* part = ar.take<float>((size_t)w.splits * w.split_stride);
+  if (!launch) return ar.used;
+  for (int i = 0; i < 3; ++i) w.prob[i].c = part + i * one;
+
+  by_f16(a.dtype, [&](auto f) {
+    constexpr bool F16 = decltype(f)::value;
+    OpGemmParams d{};
+    d.nprob = 1;
+    OpProb& e = d.prob[0];
+    e.a[0] = y; e.b[0] = wd; e.M = M; e.N = F8; e.Nb = a.F; e.ldc = F8;
+    finish_prob(e, 256, a.N, 0);
+    d.ntiles = e.tiles_m * e.tiles_n;
+    set_k(d, a.N);
+    d.act = a.act; d.g = (h16*)g; d.u = (h16*)u; d.dg = dg; d.du = du; d.ldg = F8; d.colsum = cs_f;
+    launch_op_gemm<F16, false, true, OG_DGATE, 256>(d, s);
+    if (o->dx) {
+      OpGemmParams c{};
+      c.nprob = 1;
+      OpProb& q = c.prob[0];
+      q.a[0] = OpMat{dg, F8}; q.a[1] = OpMat{du, F8}; q.b[0] = wg; q.b[1] = wu;
+      q.c = o->dx; q.ldc = o->dx_row; q.M = M; q.N = q.Nb = a.K;
+      q.cvec = a.K % 8 == 0 && o->dx_row % 8 == 0 && (uintptr_t)o->dx % 16 == 0;
+      finish_prob(q, 256, 2 * a.F, 0);
+      c.ntiles = q.tiles_m * q.tiles_n;
+      set_k(c, a.F, a.F);
+      launch_op_gemm<F16, false, true, OG_PLAIN, 256>(c, s);
+    }
+    if (o->dw_gate) {
+      launch_op_gemm<F16, true, true, OG_PART, 256>(w, s);
+      SplitReduceParams r{};
+      void* outs[3] = {o->dw_gate, o->dw_up, o->dw_down};
+      long long most = 0;
+      for (int i = 0; i < 3; ++i) {
+        r.r[i] = SplitReduce{part + i * one, (h16*)outs[i], cols[i], pitch[i], rows[i], cols[i], cols[i] % 8 == 0 && (uintptr_t)outs[i] % 16 == 0};
+        most = std::max(most, (long long)rows[i] * (pitch[i] / 4));
+      }
+      r.n = 3; r.splits = w.splits; r.stride = w.split_stride;
+      hipLaunchKernelGGL((split_reduce_kernel<F16>), dim3((unsigned)std::min<long long>((most + 255) / 256, 16384), 3), dim3(256), 0, s, r);
+    }
+    if (cs_n) hipLaunchKernelGGL((colsum_kernel<F16>), dim3((unsigned)row_blocks, (unsigned)((N8 / 8 + 63) / 64)), dim3(256), 0, s, y.p, y.ld, cs_n, N8,
+                                 (long long)M, a.N);
+    if (cs_f || cs_n) {
+      ColReduceParams r{};
+      int n = 0, widest = 1;
+      auto add = [&](float* src, void* out, long long parts, int pitch_, int c) {
+        if (!out) return;
+        r.r[n++] = ColReduce{src, out, parts, pitch_, c};
+        widest = std::max(widest, c);
+      };
+      add(cs_f, o->db_gate, 2ll * tiles_m, F8, a.F);
+      add(cs_f ? cs_f + (size_t)2 * tiles_m * F8 : nullptr, o->db_up, 2ll * tiles_m, F8, a.F);
+      add(cs_n, o->db_down, row_blocks, N8, a.N);
+      r.f16 = F16; r.out_f32 = a.bias_f32;
+      hipLaunchKernelGGL(col_reduce_kernel, dim3((unsigned)((widest + 63) / 64), (unsigned)n), dim3(256), 0, s, r);
+    }
+  });
+  return ar.used;
+}
+
+}  // namespace
+
+extern "C" int64_t vtc_gated_ffn_workspace(int64_t rows, int32_t width, int32_t inner, int32_t out_width, int32_t backward) {
+  if (rows < 0 || rows > (1ll << 31) - 256 || width < 1 || inner < 1 || out_width < 1 || width > kFfnMaxDim || inner > kFfnMaxDim || out_width > kFfnMaxDim) {
+    fail_handleless(VTC_ERR_ARG, "gated ffn: bad sizes");
+    return VTC_ERR_ARG;
+  }
+  if (rows == 0) return 0;
+  const vtc_mat m{nullptr, 0};   // a null matrix counts as one that has to be copied: enough for every alignment
+  FfnArgs a{OP_F16, 0, 0, rows, width, inner, out_width, &m, &m, &m, &m, nullptr, nullptr, nullptr};
+  vtc_mat odd{(const void*)2, 1};
+  a.x = a.wg = a.wu = a.wd = &odd;
+  vtc_ffn_grads o{};
+  return (int64_t)(backward ? ffn_backward(a, &odd, nullptr, nullptr, nullptr, &o, nullptr, false, nullptr)
+                            : ffn_forward(a, nullptr, nullptr, nullptr, nullptr, nullptr, false, nullptr));
+}
+
+extern "C" int64_t vtc_gated_ffn_saved(int64_t rows, int32_t inner) {
+  if (rows < 0 || inner < 1 || inner > kFfnMaxDim || rows > (1ll << 31) - 256) { fail_handleless(VTC_ERR_ARG, "gated ffn: bad sizes"); return VTC_ERR_ARG; }
+  return 3 * (int64_t)align256((size_t)rows * up8(inner) * 2);
+}
+
+extern "C" int vtc_gated_ffn(int device, int dtype, int64_t rows, int32_t width, int32_t inner, int32_t out_width, const vtc_mat* x,
+                             const vtc_mat* w_gate, const vtc_mat* w_up, const vtc_mat* w_down, const void* b_gate, const void* b_up,
+                             const void* b_down, int32_t bias_f32, int32_t act, const vtc_mat* y, void* saved, int64_t saved_bytes,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "gated ffn";
+  FfnArgs a{dtype, act, bias_f32, rows, width, inner, out_width, x, w_gate, w_up, w_down, b_gate, b_up, b_down};
+  if (int rc = ffn_check(what, a)) return rc;
+  if (int rc = ffn_check_mat(what, "y", y, rows, out_width)) return rc;
+  if (rows == 0) return VTC_OK;
+  const char* y_end = end_of(y->p, {{rows, y->row}}, out_width, 2);
+  if (overlap(x->p, end_of(x->p, {{rows, x->row}}, width, 2), y->p, y_end)) return fail_handleless(VTC_ERR_ARG, "%s: y overlaps x", what);
+  const int64_t need_s = vtc_gated_ffn_saved(rows, inner);
+  if (saved && saved_bytes < need_s) return fail_handleless(VTC_ERR_CAPACITY, "%s: the saved buffer holds %lld bytes, %lld needed", what, (long long)saved_bytes, (long long)need_s);
+  const size_t need = ffn_forward(a, nullptr, nullptr, nullptr, (h16*)saved, nullptr, false, nullptr);
+  if (need && (!workspace || workspace_bytes < (int64_t)need)) return fail_handleless(VTC_ERR_CAPACITY, "%s: the workspace holds %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
+  if ((uintptr_t)workspace % 256 || (uintptr_t)saved % 256) return fail_handleless(VTC_ERR_ARG, "%s: workspace and saved buffer must be aligned to 256 bytes", what);
+  DeviceGuard guard(device);
+  if (guard.rc) return guard.rc;
+  const size_t part = align256((size_t)rows * up8(inner) * 2);
+  h16* sg = (h16*)saved;
+  h16* su = saved ? (h16*)((char*)saved + part) : nullptr;
+  h16* sh = saved ? (h16*)((char*)saved + 2 * part) : nullptr;
+  ffn_forward(a, y, sg, su, sh, (char*)workspace, true, (hipStream_t)stream);
+  return launched(what);
+}
+
+extern "C" int vtc_gated_ffn_backward(int device, int dtype, int64_t rows, int32_t width, int32_t inner, int32_t out_width, const vtc_mat* dy,
+                                      const vtc_mat* x, const vtc_mat* w_gate, const vtc_mat* w_up, const vtc_mat* w_down, const void* saved,
+                                      int64_t saved_bytes, int32_t bias_f32, int32_t act, const vtc_ffn_grads* grads, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+  const char* what = "gated ffn backward";
+  FfnArgs a{dtype, act, bias_f32, rows, width, inner, out_width, x, w_gate, w_up, w_down, nullptr, nullptr, nullptr};
+  if (int rc = ffn_check(what, a)) return rc;
+  if (int rc = ffn_check_mat(what, "dy", dy, rows, out_width)) return rc;
+  if (!grads) return fail_handleless(VTC_ERR_ARG, "%s: null argument", what);
+  if (rows == 0) return fail_handleless(VTC_ERR_ARG, "%s: no rows (the gradients of nothing are zeros, which the caller has)", what);
+  if ((grads->dw_gate || grads->dw_up || grads->dw_down) && !(grads->dw_gate && grads->dw_up && grads->dw_down))
+    return fail_handleless(VTC_ERR_ARG, "%s: the three weight gradients go together", what);
+  for (const void* p : {grads->dx, grads->dw_gate, grads->dw_up, grads->dw_down})
+    if ((uintptr_t)p % 2) return fail_handleless(VTC_ERR_ARG, "%s: a gradient is not aligned to its type", what);
+  if (grads->dx) {
+    if (grads->dx_row < width || grads->dx_row > kMaxPitch) return fail_handleless(VTC_ERR_ARG, "%s: dx has a row pitch of %lld for %d columns", what, (long long)grads->dx_row, width);
+    const char* e = end_of(grads->dx, {{rows, grads->dx_row}}, width, 2);
+    if (overlap(x->p, end_of(x->p, {{rows, x->row}}, width, 2), grads->dx, e) || overlap(dy->p, end_of(dy->p, {{rows, dy->row}}, out_width, 2), grads->dx, e))
+      return fail_handleless(VTC_ERR_ARG, "%s: dx overlaps x or dy", what);
+  }
+  const int64_t need_s = vtc_gated_ffn_saved(rows, inner);
+  if (!saved || saved_bytes < need_s) return fail_handleless(VTC_ERR_CAPACITY, "%s: the saved buffer of the forward call holds %lld bytes, %lld needed", what, (long long)saved_bytes, (long long)need_s);
+  const size_t need = ffn_backward(a, dy, nullptr, nullptr, nullptr, grads, nullptr, false, nullptr);
+  if (!workspace || workspace_bytes < (int64_t)need) return fail_handleless(VTC_ERR_CAPACITY, "%s: the workspace holds %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
+  if ((uintptr_t)workspace % 256 || (uintptr_t)saved % 256) return fail_handleless(VTC_ERR_ARG, "%s: workspace and saved buffer must be aligned to 256 bytes", what);
+  DeviceGuard guard(device);
+  if (guard.rc) return guard.rc;
+  const size_t part = align256((size_t)rows * up8(inner) * 2);
+  ffn_backward(a, dy, (const h16*)saved, (const h16*)((const char*)saved + part), (const h16*)((const char*)saved + 2 * part), grads, (char*)workspace, true,
+               (hipStream_t)stream);
+  return launched(what);
 }

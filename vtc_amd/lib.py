@@ -68,8 +68,18 @@ class VtcRows3(C.Structure):
     _fields_ = [("p", C.c_void_p), ("batch", C.c_int64), ("row", C.c_int64)]
 
 
+class VtcMat(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("row", C.c_int64)]
+
+
+class VtcFfnGrads(C.Structure):
+    _fields_ = [("dx", C.c_void_p), ("dx_row", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("dw_gate", "dw_up", "dw_down", "db_gate", "db_up", "db_down")]
+
+
 # every symbol include/vtc_amd.h declares: name -> (restype, argtypes)
 _i64p, _i32p, _f64p = C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.POINTER(C.c_double)
+_matp = C.POINTER(VtcMat)
 SYMBOLS = {
     "vtc_create": (C.c_int, [C.POINTER(VtcSpec), C.POINTER(VtcWeights), C.c_int, C.POINTER(C.c_void_p)]),
     "vtc_destroy": (None, [C.c_void_p]),
@@ -110,6 +120,14 @@ SYMBOLS = {
     "vtc_group_norm_act_backward": (C.c_int, [C.c_int, C.c_int, C.POINTER(VtcRows3), C.POINTER(VtcRows3), C.POINTER(VtcRows3), C.c_int64,
                                               C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
                                               C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "vtc_gated_ffn_workspace": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "vtc_gated_ffn_saved": (C.c_int64, [C.c_int64, C.c_int32]),
+    "vtc_gated_ffn": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int32, C.c_int32, C.c_int32, _matp, _matp, _matp, _matp, C.c_void_p,
+                                C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, _matp, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                C.c_void_p]),
+    "vtc_gated_ffn_backward": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int32, C.c_int32, C.c_int32, _matp, _matp, _matp, _matp, _matp,
+                                         C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.POINTER(VtcFfnGrads), C.c_void_p, C.c_int64,
+                                         C.c_void_p]),
 }
 
 LIB_PATH = Path(os.environ.get("VTC_AMD_LIB", Path(__file__).resolve().parent / "libvtc_amd.so"))

@@ -326,3 +326,131 @@ def group_norm_act(x: torch.Tensor, groups: int, weight=None, bias=None, eps: fl
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _GroupNormActFunction.apply(x, groups, weight, bias, eps, act, lengths)
     return group_norm_act_forward(x, groups, weight, bias, eps, act, lengths)[0]
+
+
+# ------------------------------------------------------------------------------------------------ gated feed-forward
+def _mat(t):
+    return L.VtcMat(p=t.data_ptr(), row=max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0))
+
+
+def _ffn_args(what, x, w_gate, w_up, w_down, biases, act):
+    index = _need_gpu(x, what)
+    dt = _dtype(x, what, (torch.float16, torch.bfloat16))
+    _same(what, x, w_gate=w_gate, w_up=w_up, w_down=w_down)
+    if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.dim() != 2 or w_down.shape[1] != w_gate.shape[0] or x.dim() < 1 or x.shape[-1] != w_gate.shape[1]:
+        raise ValueError(f"{what}: x (.., width), w_gate and w_up (inner, width), w_down (out, inner) do not go together: {tuple(x.shape)}, "
+                         f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
+    for name, t in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
+        if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise ValueError(f"{what}: {name} must be stored row by row")
+    if act not in ACTS:
+        raise ValueError(f"{what}: act must be one of {list(ACTS)}, got {act!r}")
+    f32, kinds = 0, set()
+    for name, b, n in zip(("b_gate", "b_up", "b_down"), biases, (w_gate.shape[0], w_gate.shape[0], w_down.shape[0])):
+        if b is None:
+            continue
+        if b.device != x.device or b.shape != (n,) or not b.is_contiguous() or b.dtype not in (x.dtype, torch.float32):
+            raise ValueError(f"{what}: {name} must be contiguous, of shape ({n},) and type {x.dtype} or float32 on {x.device}")
+        kinds.add(b.dtype)
+        f32 = int(b.dtype == torch.float32)
+    if len(kinds) > 1:
+        raise ValueError(f"{what}: the biases must have one type")
+    return index, dt, f32
+
+
+def _rows2(t, what):
+    """t (.., n) as rows (m, n) whose elements are contiguous; a view where the strides allow it."""
+    r = t.reshape(-1, t.shape[-1])
+    if r.numel() and (r.stride(1) != 1 or (r.shape[0] > 1 and r.stride(0) < r.shape[1])):
+        r = r.contiguous()
+    return r
+
+
+def gated_ffn_forward(x: torch.Tensor, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu", save: bool = False):
+    """(y, saved): y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down on rows x (.., width) in float16 or bfloat16,
+    sums in fp32; w_gate, w_up (inner, width), w_down (out, inner); biases of x's type or float32.  With save, `saved` is what
+    gated_ffn_backward needs (three times rows x inner in x's type), else None."""
+    what = "gated_ffn"
+    index, dt, f32 = _ffn_args(what, x, w_gate, w_up, w_down, (b_gate, b_up, b_down), act)
+    rows = _rows2(x, what)
+    m, k = rows.shape
+    f, n = w_gate.shape[0], w_down.shape[0]
+    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    so = L.load()
+    size = so.vtc_gated_ffn_workspace(m, k, f, n, 0)
+    if size < 0:
+        L.check(int(size))
+    saved = _workspace(so.vtc_gated_ffn_saved(m, f), x.device) if save else None
+    if m == 0:
+        return y, saved
+    ws = _workspace(size, x.device)
+    L.check(so.vtc_gated_ffn(index, dt, m, k, f, n, C.byref(_mat(rows)), C.byref(_mat(w_gate)), C.byref(_mat(w_up)), C.byref(_mat(w_down)),
+                             _ptr(b_gate), _ptr(b_up), _ptr(b_down), f32, ACTS[act], C.byref(L.VtcMat(y.data_ptr(), n)), _ptr(saved),
+                             0 if saved is None else saved.numel(), _ptr(ws), ws.numel(), _stream(x.device)))
+    return y, saved
+
+
+def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate, w_up, w_down, saved, act: str = "silu", biases: bool = True,
+                       bias_dtype=None, need_dx: bool = True, need_dw: bool = True):
+    """(dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down) for dy = dLoss / dy and the forward call's `saved`; what is not asked for
+    (biases, need_dx, need_dw) is None.  Gradients have the type of what they belong to (biases: bias_dtype, default x's)."""
+    what = "gated_ffn_backward"
+    index, dt, _ = _ffn_args(what, x, w_gate, w_up, w_down, (None, None, None), act)
+    _same(what, x, dy=dy)
+    f, n = w_gate.shape[0], w_down.shape[0]
+    if dy.shape != x.shape[:-1] + (n,):
+        raise ValueError(f"{what}: dy must have shape {tuple(x.shape[:-1] + (n,))}, got {tuple(dy.shape)}")
+    bias_dtype = bias_dtype or x.dtype
+    if bias_dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{what}: bias_dtype must be {x.dtype} or float32")
+    rows, drows = _rows2(x, what), _rows2(dy, what)
+    m, k = rows.shape
+    new = lambda shape, kind: torch.empty(shape, dtype=kind, device=x.device)  # noqa: E731
+    dx = new(x.shape, x.dtype) if need_dx else None
+    dw = tuple(new(w.shape, x.dtype) if need_dw else None for w in (w_gate, w_up, w_down))
+    db = tuple(new((c,), bias_dtype) if biases else None for c in (f, f, n))
+    if m == 0:
+        for t in dw + db:
+            if t is not None:
+                t.zero_()
+        return (dx,) + dw + db
+    so = L.load()
+    size = so.vtc_gated_ffn_workspace(m, k, f, n, 1)
+    if size < 0:
+        L.check(int(size))
+    if saved is None or saved.device != x.device or saved.dtype != torch.uint8 or saved.numel() < so.vtc_gated_ffn_saved(m, f):
+        raise ValueError(f"{what}: saved is the forward call's (with save=True)")
+    ws = _workspace(size, x.device)
+    adr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    grads = L.VtcFfnGrads(adr(dx), k, *(adr(t) for t in dw + db))
+    L.check(so.vtc_gated_ffn_backward(index, dt, m, k, f, n, C.byref(_mat(drows)), C.byref(_mat(rows)), C.byref(_mat(w_gate)),
+                                      C.byref(_mat(w_up)), C.byref(_mat(w_down)), _ptr(saved), saved.numel(),
+                                      int(bias_dtype == torch.float32), ACTS[act], C.byref(grads), _ptr(ws), ws.numel(), _stream(x.device)))
+    return (dx,) + dw + db
+
+
+class _GatedFfnFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
+        y, saved = gated_ffn_forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, save=True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
+        ctx.act, ctx.kinds = act, tuple(None if b is None else b.dtype for b in (b_gate, b_up, b_down))
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w_gate, w_up, w_down, saved = ctx.saved_tensors
+        kinds = [k for k in ctx.kinds if k is not None]
+        need = ctx.needs_input_grad
+        got = gated_ffn_backward(dy, x, w_gate, w_up, w_down, saved, ctx.act, biases=bool(kinds) and any(need[4:7]),
+                                 bias_dtype=kinds[0] if kinds else None, need_dx=need[0], need_dw=any(need[1:4]))
+        return tuple(t if i < 4 or ctx.kinds[i - 4] is not None else None for i, t in enumerate(got)) + (None,)
+
+
+def gated_ffn(x: torch.Tensor, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu") -> torch.Tensor:
+    """The block with a gradient for x, the weights and the biases; see gated_ffn_forward."""
+    _need_gpu(x, "gated_ffn")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_gate, w_up, w_down, b_gate, b_up, b_down)):
+        return _GatedFfnFunction.apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
+    return gated_ffn_forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)[0]
