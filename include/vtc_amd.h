@@ -325,6 +325,27 @@ int vtc_gated_ffn_backward(int device, int dtype, int64_t rows, int32_t width, i
                            int64_t saved_bytes, int32_t bias_f32, int32_t act, const vtc_ffn_grads* grads, void* workspace,
                            int64_t workspace_bytes, void* stream);
 
+/* A model whose encoder differs from HuBERT-base in one or more of these pieces (everything else, and every call on the model, is
+ * that of vtc_create).  Zeroed fields keep the HuBERT-base piece.
+ *   conv_norm_groups != 0: conv layers 1..6 are followed by a group norm with that many groups (a divisor of 512) in front of their
+ *     GELU, conv_gn_w / conv_gn_b[1..6] its affine [512] (conv layer 0 keeps its own, one group per channel).
+ *   rotary.rotary_dim != 0: rotary positions on the queries and keys of every layer (head_dim is 64; position = frame of the
+ *     window), no positional conv: w->pos_w and pos_b are not read.
+ *   ffn_act != 0: gated feed-forward with this activation; layer[l].ff1_w / ff1_b are the up projection [ffn_inner,768], ff2_w is
+ *     [768,ffn_inner], gate_w / gate_b[l] the gate [ffn_inner,768], [ffn_inner].  ffn_inner: a multiple of 128, 256..8192. */
+typedef struct {
+  int32_t conv_norm_groups;
+  int32_t ffn_act;
+  int32_t ffn_inner;
+  int32_t reserved;
+  vtc_rotary rotary;
+  const float* conv_gn_w[7];
+  const float* conv_gn_b[7];
+  const float* gate_w[VTC_N_LAYERS];
+  const float* gate_b[VTC_N_LAYERS];
+} vtc_variant;
+int vtc_create_variant(const vtc_spec* spec, const vtc_weights* w, const vtc_variant* variant, int device, vtc_model** out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -139,11 +139,25 @@ def _q(x: torch.Tensor, emulate_bf16: bool) -> torch.Tensor:
     return x.to(torch.bfloat16).to(torch.float32) if emulate_bf16 else x
 
 
-def encoder_stages(w: dict, wav: torch.Tensor, emulate_bf16: bool = False, ranges: dict | None = None) -> dict:
+def rotate_heads(x: torch.Tensor, rotary) -> torch.Tensor:
+    """Rotary positions 0, 1, .. on (batch, heads, frames, 64) from a rotation's frequencies (64 bits), layout and amplitude."""
+    r = rotary.rotary_dim
+    a = torch.arange(x.shape[2], dtype=torch.float64)[:, None] * torch.from_numpy(np.asarray(rotary.frequency))
+    c, s = (torch.cos(a) * rotary.amplitude).float(), (torch.sin(a) * rotary.amplitude).float()
+    first = slice(0, r // 2) if rotary.layout == "half" else slice(0, r, 2)
+    second = slice(r // 2, r) if rotary.layout == "half" else slice(1, r, 2)
+    y = x.clone()
+    y[..., first], y[..., second] = x[..., first] * c - x[..., second] * s, x[..., first] * s + x[..., second] * c
+    return y
+
+
+def encoder_stages(w: dict, wav: torch.Tensor, emulate_bf16: bool = False, ranges: dict | None = None, variant=None) -> dict:
     """Forward (B, W) fp32 waveforms; returns every stage output (fp32).
 
     emulate_bf16=True rounds every GEMM operand (activations and weights) to bf16 with fp32
     accumulation, which is what the MFMA path does; used to size the error budget on CPU.
+    variant: an engine.EncoderVariant, for encoders that differ from HuBERT-base (group norm behind conv layers 1..6, rotary
+    positions in place of the positional conv, a gated feed-forward block).
     ranges: if a dict, receives max |value| of every tensor class the HIP path keeps in 16-bit storage between kernels
     (conv activations, pre-LayerNorm residual rows, q/k/v, attention context, FFN hidden): how close a weight set comes
     to the fp16 limit of 65,504.
@@ -164,6 +178,9 @@ def encoder_stages(w: dict, wav: torch.Tensor, emulate_bf16: bool = False, range
     out["conv0"] = x
     for i in range(1, 7):  # modeling_hubert.py:106-124
         x = F.conv1d(q(x), q(w[f"feature_extractor.conv_layers.{i}.conv.weight"]), stride=CONV_STRIDES[i])
+        if variant is not None and variant.conv_norm_groups:
+            p = f"feature_extractor.conv_layers.{i}.layer_norm."
+            x = F.group_norm(q(x), variant.conv_norm_groups, w[p + "weight"], w[p + "bias"], eps=1e-5)
         x = see("conv_activations", F.gelu(x))
         out[f"conv{i}"] = x
     x = x.transpose(1, 2)  # (B, T, 512)
@@ -173,9 +190,10 @@ def encoder_stages(w: dict, wav: torch.Tensor, emulate_bf16: bool = False, range
     x = F.linear(q(x), q(w["feature_projection.projection.weight"]), w["feature_projection.projection.bias"])
     out["proj"] = x
     # positional conv + residual + LN (modeling_hubert.py:83-92, 439-441)
-    pc = F.conv1d(q(x.transpose(1, 2)), q(pos_conv_weight(w)), w["encoder.pos_conv_embed.conv.bias"],
-                  padding=64, groups=16)[:, :, :-1]
-    x = see("pre_layernorm_rows", x + F.gelu(pc).transpose(1, 2))
+    if variant is None or variant.rotary is None:
+        pc = F.conv1d(q(x.transpose(1, 2)), q(pos_conv_weight(w)), w["encoder.pos_conv_embed.conv.bias"],
+                      padding=64, groups=16)[:, :, :-1]
+        x = see("pre_layernorm_rows", x + F.gelu(pc).transpose(1, 2))
     x = F.layer_norm(x, (768,), w["encoder.layer_norm.weight"], w["encoder.layer_norm.bias"], eps=1e-5)
     out["enc_in"] = x
     b, t, _ = x.shape
@@ -186,12 +204,19 @@ def encoder_stages(w: dict, wav: torch.Tensor, emulate_bf16: bool = False, range
         kh = F.linear(xq, q(w[p + "attention.k_proj.weight"]), w[p + "attention.k_proj.bias"])
         vh = F.linear(xq, q(w[p + "attention.v_proj.weight"]), w[p + "attention.v_proj.bias"])
         qh, kh, vh = (q(see("qkv", z)).view(b, t, 12, 64).transpose(1, 2) for z in (qh, kh, vh))
+        if variant is not None and variant.rotary is not None:
+            qh, kh = q(rotate_heads(qh, variant.rotary)), q(rotate_heads(kh, variant.rotary))
         att = torch.softmax(qh @ kh.transpose(2, 3), dim=-1)   # modeling_hubert.py:248-253
         ctx = see("attention_context", (q(att) @ vh).transpose(1, 2).reshape(b, t, 768))
         x = see("pre_layernorm_rows", x + F.linear(q(ctx), q(w[p + "attention.out_proj.weight"]), w[p + "attention.out_proj.bias"]))
         x = F.layer_norm(x, (768,), w[p + "layer_norm.weight"], w[p + "layer_norm.bias"], eps=1e-5)
-        h = see("ffn_hidden", F.gelu(F.linear(q(x), q(w[p + "feed_forward.intermediate_dense.weight"]),
-                                              w[p + "feed_forward.intermediate_dense.bias"])))
+        up = F.linear(q(x), q(w[p + "feed_forward.intermediate_dense.weight"]), w[p + "feed_forward.intermediate_dense.bias"])
+        if variant is not None and variant.ffn != "gelu":
+            gate = F.linear(q(x), q(w[p + "feed_forward.gate_dense.weight"]), w[p + "feed_forward.gate_dense.bias"])
+            h = {"gated_gelu": F.gelu, "gated_silu": F.silu, "gated_sigmoid": torch.sigmoid}[variant.ffn](gate) * up
+        else:
+            h = F.gelu(up)
+        h = see("ffn_hidden", h)
         x = see("pre_layernorm_rows", x + F.linear(q(h), q(w[p + "feed_forward.output_dense.weight"]),
                                                    w[p + "feed_forward.output_dense.bias"]))
         x = F.layer_norm(x, (768,), w[p + "final_layer_norm.weight"], w[p + "final_layer_norm.bias"], eps=1e-5)

@@ -74,6 +74,8 @@ bool g_static_pending[kMaxDevices] = {false};
 struct LayerDev {
   h16 *qkv_w, *o_w, *ff1_w, *ff2_w;
   float *qkv_b, *qkv_s, *o_bb, *ff1_b, *ff1_s, *ff2_bb;
+  h16* gate_w;                                   // gated feed-forward (encoder variant): ff1_w is the up projection, not folded
+  float* gate_b;
   float *g_in, *ln1_w, *ln1_b, *ln2_w, *ln2_b;   // g_in: gamma of the LayerNorm that feeds the layer (previous ln2 / encoder LN)
 };
 
@@ -140,6 +142,14 @@ struct vtc_model {
   bool dec_active = false, dec_want_summary = false;
   long long dec_n = 0, dec_rcap = 0;
   std::vector<int64_t> dec_rows;
+
+  // encoder variant (vtc_create_variant); zero: HuBERT-base
+  int conv_norm_groups = 0, ffn_act = 0, ffn_inner = 3072;
+  vtc_rotary rotary{};                             // rotary_dim 0: positional conv
+  std::vector<double> rotary_freq;
+  float *conv_gn_w[7] = {nullptr}, *conv_gn_b[7] = {nullptr}, *conv_gn_stat = nullptr;   // stat: mean, then rstd
+  char* conv_gn_ws = nullptr;
+  int64_t conv_gn_ws_bytes = 0;
 
   int debug_stop = -1;
   bool big_tiles = true;   // 256x256 8-phase GEMM (VTC_GEMM_TILE=128 selects the 128x128 kernel, for A/B runs)
@@ -420,7 +430,18 @@ int forward_impl(vtc_model* m, const float* wav, int nw, float* logits, hipStrea
     p.rows_per_batch = L[i];
     p.a_row_stride = (long long)kStrides[i] * 512;
     p.a_batch_stride = (long long)L[i - 1] * 512;
-    gemm_go<F16, 128, EPI_GELU>(m, p, 1, s);
+    if (m->conv_norm_groups) {   // encoder variant: the conv's rows, then group norm + GELU in place
+      gemm_go<F16, 128, 0>(m, p, 1, s);
+      const vtc_rows3 rows{dst, (int64_t)L[i] * 512, 512};
+      int rc = 0;
+      LAUNCH(m, PC_LAYERNORM, 0.0, (double)p.M * 512 * 6, s,
+             rc = vtc_group_norm_act(m->device, F16 ? VTC_F16 : VTC_BF16, &rows, &rows, nw, L[i], 512, m->conv_norm_groups, m->conv_gn_w[i],
+                                     m->conv_gn_b[i], 1, 1e-5, VTC_ACT_GELU, nullptr, m->conv_gn_stat,
+                                     m->conv_gn_stat + (size_t)nw * m->conv_norm_groups, m->conv_gn_ws, m->conv_gn_ws_bytes, s));
+      if (rc) return fail(m, rc, "%s", g_create_error.c_str());
+    } else {
+      gemm_go<F16, 128, EPI_GELU>(m, p, 1, s);
+    }
     std::swap(src, dst);
     if (m->debug_stop == i) return 0;
   }
@@ -431,18 +452,22 @@ int forward_impl(vtc_model* m, const float* wav, int nw, float* logits, hipStrea
   gemm_go<F16, 128, EPI_BIAS | EPI_F32>(m, plain(dst, m->fp_w, m->h0, m->fp_b, nullptr, M, 768, 512), 1, s);
   if (m->debug_stop == 7) return 0;
 
-  // ---- positional conv (16 groups x [T x 6144] x [6144 x 48]) + GELU + residual, then LayerNorm
+  // ---- positional conv (16 groups x [T x 6144] x [6144 x 48]) + GELU + residual, then LayerNorm; rotary positions need none
+  if (!m->rotary.rotary_dim) {
   LAUNCH(m, PC_PACK, 0.0, (double)M * 768 * 6, s,
          hipLaunchKernelGGL((posconv_pack_kernel<F16>), dim3((T + 128 + 3) / 4, nw), dim3(192), 0, s, m->h0, m->posin, T));
   LAUNCH(m, PC_GEMM, 2.0 * M * 768.0 * 48 * 128, 0.0, s,
          hipLaunchKernelGGL((posconv_kernel<F16>), dim3((T + kPcRows - 1) / kPcRows, 16, nw), dim3(256), 0, s, m->posin,
                             m->pos_w, m->pos_b, m->h0, m->tmp32, T));
+  }
+  const float* pre_ln = m->rotary.rotary_dim ? m->h0 : m->tmp32;
   // ---- entry of the LayerNorm-free layers: the fp32 pre-LN rows rounded to 16 bit + the statistics of the encoder LayerNorm
   HeadParams nohead{};
   const dim3 ln_grid((M + 4 * kLnRows - 1) / (4 * kLnRows)), ln_blk(256);
   LAUNCH(m, PC_LAYERNORM, 0.0, (double)M * 768 * 6, s,
-         hipLaunchKernelGGL((ln_round_stats_kernel<F16>), dim3((M + 3) / 4), dim3(256), 0, s, m->tmp32, m->x16, m->ln_stats, M));
-  // test hook: materialise LayerNorm(u) (what the oracle calls the stage output) in ctx16, which is free between layers
+         hipLaunchKernelGGL((ln_round_stats_kernel<F16>), dim3((M + 3) / 4), dim3(256), 0, s, pre_ln, m->x16, m->ln_stats, M));
+  // materialise LayerNorm(u) in ctx16, which is free between attention blocks: for the test hook (what the oracle calls the stage
+  // output) and in front of a gated feed-forward block
   auto debug_ln = [&](const float* g, const float* b) {
     hipLaunchKernelGGL((layernorm768_kernel<F16, false, 1>), ln_grid, ln_blk, 0, s, (const void*)m->x16, g, b,
                        (float*)nullptr, m->ctx16, M, nohead);
@@ -468,11 +493,26 @@ int forward_impl(vtc_model* m, const float* wav, int nw, float* logits, hipStrea
   for (int l = 0; l < VTC_N_LAYERS; ++l) {
     const LayerDev& w = m->layer[l];
     ln_in_gemm(std::integral_constant<int, EPI_BIAS | EPI_LNIN>{}, w.qkv_w, m->qkv16, w.qkv_b, w.qkv_s, 2304);
+    if (m->rotary.rotary_dim) {   // q and k of the fused rows, in place; the query scale commutes with the rotation
+      vtc_heads qk[2] = {};
+      for (int i = 0; i < 2; ++i)
+        qk[i] = vtc_heads{m->qkv16 + 768 * i, m->qkv16 + 768 * i, (int64_t)T * 2304, 2304, 64, (int64_t)T * 2304, 2304, 64, 12, 0};
+      int rc = 0;
+      LAUNCH(m, PC_PACK, 0.0, (double)M * 1536 * 4, s,
+             rc = vtc_rotary_heads(m->device, F16 ? VTC_F16 : VTC_BF16, &m->rotary, nw, T, qk, 2, nullptr, 0, 0, 0, 0, 0, s));
+      if (rc) return fail(m, rc, "%s", g_create_error.c_str());
+    }
     LAUNCH(m, PC_ATTN, attn_flops, 0.0, s,
            hipLaunchKernelGGL((attention_kernel<F16>), dim3(nqb, nw * 12), dim3(512), 0, s, m->qkv16, m->ctx16, T, nkt));
     ln_res_gemm(m->ctx16, w.o_w, w.o_bb, w.g_in, 768);          // u1 = LN_in(u) + ctx W_o^T + b_o, statistics of ln1
-    ln_in_gemm(std::integral_constant<int, EPI_BIAS | EPI_GELU | EPI_LNIN>{}, w.ff1_w, m->ffn16, w.ff1_b, w.ff1_s, 3072);
-    ln_res_gemm(m->ffn16, w.ff2_w, w.ff2_bb, w.ln1_w, 3072);    // u2 = LN_1(u1) + h W_2^T + b_2, statistics of ln2
+    if (m->ffn_act) {   // gated: the LayerNorm's rows (ctx16 is free here), then gate, up, activation and product in one kernel
+      LAUNCH(m, PC_LAYERNORM, 0.0, (double)M * 768 * 4, s, debug_ln(w.ln1_w, w.ln1_b));
+      LAUNCH(m, PC_GEMM, 4.0 * M * 768.0 * m->ffn_inner, 0.0, s,
+             launch_gated_up(F16 ? OP_F16 : OP_BF16, M, 768, m->ffn_inner, m->ctx16, w.gate_w, w.ff1_w, w.gate_b, w.ff1_b, m->ffn_act, m->ffn16, s));
+    } else {
+      ln_in_gemm(std::integral_constant<int, EPI_BIAS | EPI_GELU | EPI_LNIN>{}, w.ff1_w, m->ffn16, w.ff1_b, w.ff1_s, 3072);
+    }
+    ln_res_gemm(m->ffn16, w.ff2_w, w.ff2_bb, w.ln1_w, m->ffn_inner);    // u2 = LN_1(u1) + h W_2^T + b_2, statistics of ln2
     if (m->debug_stop == 9 + l) { debug_ln(w.ln2_w, w.ln2_b); return 0; }
   }
   // ---- final LayerNorm with the per-frame multi-label head fused; writes stitched logits
@@ -547,7 +587,12 @@ void vtc_destroy(vtc_model* m) {
 }
 
 int vtc_create(const vtc_spec* spec, const vtc_weights* w, int device, vtc_model** out) {
-  if (!spec || !w || !out) return fail(nullptr, VTC_ERR_ARG, "null argument");
+  const vtc_variant base{};
+  return vtc_create_variant(spec, w, &base, device, out);
+}
+
+int vtc_create_variant(const vtc_spec* spec, const vtc_weights* w, const vtc_variant* variant, int device, vtc_model** out) {
+  if (!spec || !w || !variant || !out) return fail(nullptr, VTC_ERR_ARG, "null argument");
   *out = nullptr;
   if (spec->abi_version != VTC_ABI_VERSION) return fail(nullptr, VTC_ERR_ARG, "ABI version %d != %d", spec->abi_version, VTC_ABI_VERSION);
   if (spec->n_labels < 1 || spec->n_labels > VTC_MAX_LABELS) return fail(nullptr, VTC_ERR_ARG, "n_labels %d out of range", spec->n_labels);
@@ -557,6 +602,25 @@ int vtc_create(const vtc_spec* spec, const vtc_weights* w, int device, vtc_model
   if (T < 1 || T > 2048)   // attention streams K/V, nothing is sized by T but the scratch buffers; 2048 frames = 41 s
     return fail(nullptr, VTC_ERR_ARG, "window of %d samples gives %lld frames; supported 1..2048",
                 spec->window_samples, T);
+  const vtc_variant& var = *variant;
+  if (var.conv_norm_groups < 0 || (var.conv_norm_groups && 512 % var.conv_norm_groups))
+    return fail(nullptr, VTC_ERR_ARG, "conv_norm_groups %d does not divide 512", var.conv_norm_groups);
+  if (var.ffn_act < 0 || var.ffn_act > VTC_ACT_SIGMOID) return fail(nullptr, VTC_ERR_ARG, "unknown ffn_act %d", var.ffn_act);
+  if (var.ffn_act && (var.ffn_inner % 128 || var.ffn_inner < 256 || var.ffn_inner > 8192))
+    return fail(nullptr, VTC_ERR_ARG, "ffn_inner %d is not a multiple of 128 in 256..8192", var.ffn_inner);
+  const bool gated = var.ffn_act != 0, rot = var.rotary.rotary_dim != 0;
+  if (rot) {
+    const vtc_rotary& r = var.rotary;
+    if (r.head_dim != 64 || r.rotary_dim < 2 || r.rotary_dim > 64 || r.rotary_dim % 2 || !r.frequency || !std::isfinite(r.amplitude) ||
+        (r.layout != VTC_ROTARY_HALF && r.layout != VTC_ROTARY_INTERLEAVED))
+      return fail(nullptr, VTC_ERR_ARG, "rotary: head_dim must be 64, rotary_dim even and in 2..64, with frequencies, a finite amplitude and a layout");
+    for (int j = 0; j < r.rotary_dim / 2; ++j)
+      if (!std::isfinite(r.frequency[j])) return fail(nullptr, VTC_ERR_ARG, "rotary: frequency %d is not finite", j);
+  }
+  for (int i = 1; i < 7 && var.conv_norm_groups; ++i)
+    if (!var.conv_gn_w[i] || !var.conv_gn_b[i]) return fail(nullptr, VTC_ERR_ARG, "missing group norm tensor of conv layer %d", i);
+  for (int l = 0; l < VTC_N_LAYERS && gated; ++l)
+    if (!var.gate_w[l] || !var.gate_b[l]) return fail(nullptr, VTC_ERR_ARG, "missing gate tensor in layer %d", l);
   int ndev = 0;
   if (hipGetDeviceCount(&ndev) != hipSuccess || ndev < 1) return fail(nullptr, VTC_ERR_NO_GPU, "no HIP device visible");
   if (device < 0 || device >= ndev) return fail(nullptr, VTC_ERR_ARG, "device %d out of range (%d visible)", device, ndev);
@@ -573,6 +637,15 @@ int vtc_create(const vtc_spec* spec, const vtc_weights* w, int device, vtc_model
   if (const char* e = getenv("VTC_GEMM_TILE")) m->big_tiles = atoi(e) != 128;
   if (const char* e = getenv("VTC_CONV0_MFMA")) m->conv0_mfma = atoi(e) != 0;
   m->T = (int)T;
+  m->conv_norm_groups = var.conv_norm_groups;
+  m->ffn_act = var.ffn_act;
+  if (gated) m->ffn_inner = var.ffn_inner;
+  const int inner = m->ffn_inner;
+  if (rot) {
+    m->rotary_freq.assign(var.rotary.frequency, var.rotary.frequency + var.rotary.rotary_dim / 2);
+    m->rotary = var.rotary;
+    m->rotary.frequency = m->rotary_freq.data();
+  }
   {
     int n = spec->window_samples;
     for (int i = 0; i < 7; ++i) { n = (n - kKernels[i]) / kStrides[i] + 1; m->L[i] = n; }
@@ -603,11 +676,17 @@ int vtc_create(const vtc_spec* spec, const vtc_weights* w, int device, vtc_model
   }
   TRY(upload_f32(m, &m->fp_ln_w, w->fp_ln_w, 512));
   TRY(upload_f32(m, &m->fp_ln_b, w->fp_ln_b, 512));
-  if (!w->fp_w || !w->pos_w) return bail(fail(m, VTC_ERR_ARG, "missing projection / positional weight"));
+  for (int i = 1; i < 7 && m->conv_norm_groups; ++i) {
+    TRY(upload_f32(m, &m->conv_gn_w[i], var.conv_gn_w[i], 512));
+    TRY(upload_f32(m, &m->conv_gn_b[i], var.conv_gn_b[i], 512));
+  }
+  if (!w->fp_w || (!rot && !w->pos_w)) return bail(fail(m, VTC_ERR_ARG, "missing projection / positional weight"));
   TRY(upload_h16(m, &m->fp_w, pack_linear(w->fp_w, 768, 512, f16)));
   TRY(upload_f32(m, &m->fp_b, w->fp_b, 768));
-  TRY(upload_h16(m, &m->pos_w, pack_posconv(w->pos_w, f16)));
-  TRY(upload_f32(m, &m->pos_b, w->pos_b, 768));
+  if (!rot) {
+    TRY(upload_h16(m, &m->pos_w, pack_posconv(w->pos_w, f16)));
+    TRY(upload_f32(m, &m->pos_b, w->pos_b, 768));
+  }
   TRY(upload_f32(m, &m->enc_ln_w, w->enc_ln_w, 768));
   TRY(upload_f32(m, &m->enc_ln_b, w->enc_ln_b, 768));
   // Host-side packing of the 12 layers (LayerNorm folding with fp64 column sums, 16-bit rounding: 7 M weights per layer) runs
@@ -624,7 +703,7 @@ int vtc_create(const vtc_spec* spec, const vtc_weights* w, int device, vtc_model
     const float* b_in = l == 0 ? w->enc_ln_b : w->layer[l - 1].ln2_b;
     if (!g_in || !b_in) return bail(fail(m, VTC_ERR_ARG, "missing LayerNorm in front of layer %d", l));
   }
-  struct LayerHost { FoldedLinear fq, f1; std::vector<unsigned short> ow, f2w; std::vector<float> obb, f2bb; };
+  struct LayerHost { FoldedLinear fq, f1; std::vector<unsigned short> ow, f2w, gate; std::vector<float> obb, f2bb; };
   std::vector<LayerHost> host(VTC_N_LAYERS);
   {
     std::vector<std::thread> pack;
@@ -649,8 +728,13 @@ int vtc_create(const vtc_spec* spec, const vtc_weights* w, int device, vtc_model
         // out-proj adds the residual LN_in(u): its beta joins the bias
         h.obb.resize(768); h.f2bb.resize(768);
         for (int i = 0; i < 768; ++i) { h.obb[i] = s.o_b[i] + b_in[i]; h.f2bb[i] = s.ff2_b[i] + s.ln1_b[i]; }
-        h.f1 = fold_layernorm(s.ff1_w, s.ff1_b, 3072, 768, s.ln1_w, s.ln1_b, f16);
-        h.f2w = pack_linear(s.ff2_w, 768, 3072, f16);
+        if (gated) {
+          h.f1.w = pack_linear(s.ff1_w, inner, 768, f16);
+          h.gate = pack_linear(var.gate_w[l], inner, 768, f16);
+        } else {
+          h.f1 = fold_layernorm(s.ff1_w, s.ff1_b, 3072, 768, s.ln1_w, s.ln1_b, f16);
+        }
+        h.f2w = pack_linear(s.ff2_w, 768, inner, f16);
       });
     for (auto& t : pack) t.join();
   }
@@ -667,8 +751,14 @@ int vtc_create(const vtc_spec* spec, const vtc_weights* w, int device, vtc_model
     TRY(upload_f32(m, &d.ln1_w, s.ln1_w, 768));
     TRY(upload_f32(m, &d.ln1_b, s.ln1_b, 768));
     TRY(upload_h16(m, &d.ff1_w, h.f1.w));
-    TRY(upload_f32(m, &d.ff1_b, h.f1.bias.data(), 3072));
-    TRY(upload_f32(m, &d.ff1_s, h.f1.colsum.data(), 3072));
+    if (gated) {
+      TRY(upload_h16(m, &d.gate_w, h.gate));
+      TRY(upload_f32(m, &d.gate_b, var.gate_b[l], inner));
+      TRY(upload_f32(m, &d.ff1_b, s.ff1_b, inner));
+    } else {
+      TRY(upload_f32(m, &d.ff1_b, h.f1.bias.data(), 3072));
+      TRY(upload_f32(m, &d.ff1_s, h.f1.colsum.data(), 3072));
+    }
     TRY(upload_h16(m, &d.ff2_w, h.f2w));
     TRY(upload_f32(m, &d.ff2_bb, h.f2bb.data(), 768));
     TRY(upload_f32(m, &d.ln2_w, s.ln2_w, 768));
@@ -689,8 +779,15 @@ int vtc_create(const vtc_spec* spec, const vtc_weights* w, int device, vtc_model
   TRY(dev_alloc(m, &m->ln_part, (MT + 16) * 32));
   TRY(dev_alloc(m, &m->qkv16, MT * 2304));
   TRY(dev_alloc(m, &m->ctx16, MT * 768));
-  TRY(dev_alloc(m, &m->ffn16, MT * 3072));
-  TRY(dev_alloc(m, &m->posin, B * 16 * (size_t)(m->T + 128) * 48));
+  TRY(dev_alloc(m, &m->ffn16, MT * inner));
+  if (!rot) TRY(dev_alloc(m, &m->posin, B * 16 * (size_t)(m->T + 128) * 48));
+  if (m->conv_norm_groups) {
+    for (size_t b = 1; b <= B; ++b)   // any number of windows up to max_batch: row blocks per window shrink as there are more
+      for (int i = 1; i < 7; ++i)
+        m->conv_gn_ws_bytes = std::max(m->conv_gn_ws_bytes, vtc_group_norm_act_workspace((int64_t)b, m->L[i], 512, m->conv_norm_groups, 0));
+    TRY(dev_alloc(m, &m->conv_gn_ws, (size_t)m->conv_gn_ws_bytes));
+    TRY(dev_alloc(m, &m->conv_gn_stat, B * 2 * m->conv_norm_groups));
+  }
   TRY(dev_alloc(m, &m->gn_scale, B * 512));
   TRY(dev_alloc(m, &m->gn_shift, B * 512));
   m->nchunk = (m->L[0] + kStatChunk - 1) / kStatChunk;

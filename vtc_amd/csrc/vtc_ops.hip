@@ -467,9 +467,56 @@ template <bool F16, bool AKS, bool BKS, int EPI, int BN> void launch_op_gemm(OpG
   const int units = p.ntiles * p.splits;
   hipLaunchKernelGGL((op_gemm_kernel<F16, AKS, BKS, EPI, BN>), dim3((unsigned)std::min(units, 256)), dim3(512), 0, s, p);
 }
+template <bool F16, bool GATE> void launch_skinny(const SkinnyParams& p, hipStream_t s) {
+  const dim3 grid((unsigned)((p.N + 15) / 16)), block(512);
+  if (p.M <= 16) hipLaunchKernelGGL((skinny_kernel<F16, 1, GATE>), grid, block, 0, s, p);
+  else if (p.M <= 32) hipLaunchKernelGGL((skinny_kernel<F16, 2, GATE>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((skinny_kernel<F16, 4, GATE>), grid, block, 0, s, p);
+}
 template <typename F> void by_f16(int dtype, F&& f) {
   if (dtype == OP_F16) f(std::true_type{});
   else f(std::false_type{});
+}
+
+struct GateOut { h16 *h, *g, *u; };   // g, u: null where no backward pass follows
+template <bool F16> void gate_up(int64_t M, int K, int F, OpMat x, OpMat wg, OpMat wu, const void* bg, const void* bu, int bias_f32, int act, GateOut o, hipStream_t s) {
+  const int F8 = up8(F);
+  if (M <= kSkinnyRows) {
+    SkinnyParams p{};
+    p.x = x.p; p.ldx = x.ld; p.w0 = wg.p; p.w1 = wu.p; p.ldw = wg.ld;
+    p.M = (int)M; p.K = K; p.N = F8; p.Nb = F; p.b0 = bg; p.b1 = bu; p.bias_f32 = bias_f32; p.act = act;
+    p.out = o.h; p.g = o.g; p.u = o.u; p.ldo = F8;
+    launch_skinny<F16, true>(p, s);
+    return;
+  }
+  OpGemmParams p{};
+  p.nprob = 1;
+  OpProb& q = p.prob[0];
+  q.a[0] = x; q.b[0] = wg; q.b[1] = wu; q.c = o.h; q.ldc = F8; q.M = (int)M; q.N = F8; q.Nb = F; q.cvec = 1;
+  finish_prob(q, 128, K, 0);
+  p.ntiles = q.tiles_m * q.tiles_n;
+  set_k(p, K);
+  p.bias = bg; p.bias2 = bu; p.bias_f32 = bias_f32; p.act = act; p.g = o.g; p.u = o.u; p.ldg = F8;
+  launch_op_gemm<F16, false, false, OG_GATE, 256>(p, s);
+}
+template <bool F16> void down(int64_t M, int F, int N, OpMat h, OpMat wd, const void* bd, int bias_f32, void* y, long long ldy, hipStream_t s) {
+  const int cvec = N % 8 == 0 && ldy % 8 == 0 && (uintptr_t)y % 16 == 0;
+  if (M <= kSkinnyRows) {
+    SkinnyParams p{};
+    p.x = h.p; p.ldx = h.ld; p.w0 = p.w1 = wd.p; p.ldw = wd.ld;
+    p.M = (int)M; p.K = F; p.N = p.Nb = N; p.b0 = bd; p.bias_f32 = bias_f32; p.out = (h16*)y; p.ldo = ldy;
+    launch_skinny<F16, false>(p, s);
+    return;
+  }
+  OpGemmParams p{};
+  p.nprob = 1;
+  OpProb& q = p.prob[0];
+  q.a[0] = h; q.b[0] = wd; q.c = y; q.ldc = ldy; q.M = (int)M; q.N = q.Nb = N; q.cvec = cvec;
+  finish_prob(q, 192, F, 0);
+  p.ntiles = q.tiles_m * q.tiles_n;
+  set_k(p, F);
+  p.bias = bd; p.bias_f32 = bias_f32;
+  launch_op_gemm<F16, false, false, OG_PLAIN, 192>(p, s);
 }
 
 size_t ffn_forward(const FfnArgs& a, const vtc_mat* y, h16* save_g, h16* save_u, h16* save_h, char* ws, bool launch, hipStream_t s) {
@@ -482,45 +529,10 @@ size_t ffn_forward(const FfnArgs& a, const vtc_mat* y, h16* save_g, h16* save_u,
   const OpMat wd = operand(ar, a.wd, a.N, a.F, false, s, launch);
   h16* h = save_h ? save_h : ar.take<h16>((size_t)a.M * F8);
   if (!launch) return ar.used;
-  const int cvec = a.N % 8 == 0 && y->row % 8 == 0 && (uintptr_t)y->p % 16 == 0;
   by_f16(a.dtype, [&](auto f) {
     constexpr bool F16 = decltype(f)::value;
-    if (a.M <= kSkinnyRows) {
-      SkinnyParams p{};
-      p.x = x.p; p.ldx = x.ld; p.w0 = wg.p; p.w1 = wu.p; p.ldw = wg.ld;
-      p.M = (int)a.M; p.K = a.K; p.N = F8; p.Nb = a.F; p.b0 = a.bg; p.b1 = a.bu; p.bias_f32 = a.bias_f32; p.act = a.act;
-      p.out = h; p.g = save_g; p.u = save_u; p.ldo = F8;
-      SkinnyParams d{};
-      d.x = h; d.ldx = F8; d.w0 = d.w1 = wd.p; d.ldw = wd.ld;
-      d.M = (int)a.M; d.K = a.F; d.N = d.Nb = a.N; d.b0 = a.bd; d.bias_f32 = a.bias_f32; d.out = (h16*)y->p; d.ldo = y->row;
-      auto go = [&](auto mt) {
-        constexpr int MT = decltype(mt)::value;
-        hipLaunchKernelGGL((skinny_kernel<F16, MT, true>), dim3((unsigned)((F8 + 15) / 16)), dim3(512), 0, s, p);
-        hipLaunchKernelGGL((skinny_kernel<F16, MT, false>), dim3((unsigned)((a.N + 15) / 16)), dim3(512), 0, s, d);
-      };
-      if (a.M <= 16) go(std::integral_constant<int, 1>{});
-      else if (a.M <= 32) go(std::integral_constant<int, 2>{});
-      else go(std::integral_constant<int, 4>{});
-      return;
-    }
-    OpGemmParams p{};
-    p.nprob = 1;
-    OpProb& q = p.prob[0];
-    q.a[0] = x; q.b[0] = wg; q.b[1] = wu; q.c = h; q.ldc = F8; q.M = (int)a.M; q.N = F8; q.Nb = a.F; q.cvec = 1;
-    finish_prob(q, 128, a.K, 0);
-    p.ntiles = q.tiles_m * q.tiles_n;
-    set_k(p, a.K);
-    p.bias = a.bg; p.bias2 = a.bu; p.bias_f32 = a.bias_f32; p.act = a.act; p.g = save_g; p.u = save_u; p.ldg = F8;
-    launch_op_gemm<F16, false, false, OG_GATE, 256>(p, s);
-    OpGemmParams d{};
-    d.nprob = 1;
-    OpProb& e = d.prob[0];
-    e.a[0] = OpMat{h, F8}; e.b[0] = wd; e.c = (void*)y->p; e.ldc = y->row; e.M = (int)a.M; e.N = e.Nb = a.N; e.cvec = cvec;
-    finish_prob(e, 192, a.F, 0);
-    d.ntiles = e.tiles_m * e.tiles_n;
-    set_k(d, a.F);
-    d.bias = a.bd; d.bias_f32 = a.bias_f32;
-    launch_op_gemm<F16, false, false, OG_PLAIN, 192>(d, s);
+    gate_up<F16>(a.M, a.K, a.F, x, wg, wu, a.bg, a.bu, a.bias_f32, a.act, GateOut{h, save_g, save_u}, s);
+    down<F16>(a.M, a.F, a.N, OpMat{h, F8}, wd, a.bd, a.bias_f32, (void*)y->p, y->row, s);
   });
   return ar.used;
 }
@@ -635,6 +647,13 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const h16* g, const h16
 }
 
 }  // namespace
+
+void vtc::launch_gated_up(int dtype, int64_t M, int K, int F, const unsigned short* x, const unsigned short* wg, const unsigned short* wu, const float* bg,
+                          const float* bu, int act, unsigned short* h, hipStream_t s) {
+  by_f16(dtype, [&](auto f) {
+    gate_up<decltype(f)::value>(M, K, F, OpMat{x, K}, OpMat{wg, K}, OpMat{wu, K}, bg, bu, 1, act, GateOut{h, nullptr, nullptr}, s);
+  });
+}
 
 extern "C" int64_t vtc_gated_ffn_workspace(int64_t rows, int32_t width, int32_t inner, int32_t out_width, int32_t backward) {
   if (rows < 0 || rows > (1ll << 31) - 256 || width < 1 || inner < 1 || out_width < 1 || width > kFfnMaxDim || inner > kFfnMaxDim || out_width > kFfnMaxDim) {

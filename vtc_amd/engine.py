@@ -7,16 +7,19 @@ All arithmetic of the hot path runs in libvtc_amd.so (hand-written gfx950 kernel
 from __future__ import annotations
 
 import ctypes as C
+from dataclasses import dataclass
 
 import numpy as np
 import torch
 
 from . import lib as L
+from .ops import ACTS, Rotary
 
 SAMPLE_RATE = 16_000
 RF_STEP = 320   # reference: src/analysis/chunk_artifact.py:51
 RF_SIZE = 400   # reference: src/analysis/chunk_artifact.py:11-13
 DTYPES = {"bf16": 0, "f16": 1}
+FFN_ACTS = {"gelu": 0, "gated_gelu": ACTS["gelu"], "gated_silu": ACTS["silu"], "gated_sigmoid": ACTS["sigmoid"]}
 
 import weakref
 
@@ -59,9 +62,28 @@ def fold_weight_norm(sd: dict) -> np.ndarray:
     return np.ascontiguousarray(g * v / norm)
 
 
+@dataclass
+class EncoderVariant:
+    """Pieces of the encoder that differ from HuBERT-base (include/vtc_amd.h: vtc_variant).  The state dict then also holds
+    feature_extractor.conv_layers.{1..6}.layer_norm.{weight,bias} (conv_norm_groups) and
+    encoder.layers.{l}.feed_forward.gate_dense.{weight,bias} (a gated block; intermediate_dense is its up projection, and the inner
+    width is the weights'); with rotary positions it needs no encoder.pos_conv_embed."""
+    rotary: Rotary | None = None     # rotary positions on q and k in place of the positional conv
+    ffn: str = "gelu"                # "gelu" (dense) | "gated_gelu" | "gated_silu" | "gated_sigmoid"
+    conv_norm_groups: int = 0        # group norm in front of the GELU of conv layers 1..6
+
+    def __post_init__(self):
+        if self.ffn not in FFN_ACTS:
+            raise ValueError(f"ffn must be one of {list(FFN_ACTS)}, got {self.ffn!r}")
+        if self.conv_norm_groups < 0 or (self.conv_norm_groups and 512 % self.conv_norm_groups):
+            raise ValueError(f"conv_norm_groups {self.conv_norm_groups} does not divide 512")
+        if self.rotary is not None and self.rotary.rotary_dim > 64:
+            raise ValueError(f"rotary_dim {self.rotary.rotary_dim} is more than the head's 64")
+
+
 class VtcEngine:
     def __init__(self, state_dict: dict, n_labels: int, chunk_duration_s: float, max_batch: int = 64,
-                 mfma_dtype: str = "f16", device: int | str | torch.device = 0):
+                 mfma_dtype: str = "f16", device: int | str | torch.device = 0, variant: EncoderVariant | None = None):
         if not torch.cuda.is_available():
             raise RuntimeError("vtc_amd needs a ROCm GPU (gfx950); there is no CPU fallback")
         if mfma_dtype not in DTYPES:
@@ -91,7 +113,9 @@ class VtcEngine:
         w.gn_w, w.gn_b = ptr("feature_extractor.conv_layers.0.layer_norm.weight"), ptr("feature_extractor.conv_layers.0.layer_norm.bias")
         w.fp_ln_w, w.fp_ln_b = ptr("feature_projection.layer_norm.weight"), ptr("feature_projection.layer_norm.bias")
         w.fp_w, w.fp_b = ptr("feature_projection.projection.weight"), ptr("feature_projection.projection.bias")
-        w.pos_w, w.pos_b = ptr(fold_weight_norm(state_dict)), ptr("encoder.pos_conv_embed.conv.bias")
+        self.variant = variant or EncoderVariant()
+        if self.variant.rotary is None:
+            w.pos_w, w.pos_b = ptr(fold_weight_norm(state_dict)), ptr("encoder.pos_conv_embed.conv.bias")
         w.enc_ln_w, w.enc_ln_b = ptr("encoder.layer_norm.weight"), ptr("encoder.layer_norm.bias")
         for l in range(L.N_LAYERS):
             p = f"encoder.layers.{l}."
@@ -108,12 +132,47 @@ class VtcEngine:
 
         spec = L.VtcSpec(abi_version=L.ABI_VERSION, n_labels=self.n_labels, window_samples=self.window_samples,
                          max_batch=self.max_batch, mfma_dtype=DTYPES[mfma_dtype])
-        L.check(self._lib.vtc_create(C.byref(spec), C.byref(w), dev_index, C.byref(self._handle)), None)
+        L.check(self._lib.vtc_create_variant(C.byref(spec), C.byref(w), C.byref(self._variant(state_dict, ptr, keep)), dev_index,
+                                             C.byref(self._handle)), None)
         self.frames_per_window = int(self._lib.vtc_frames_per_window(self._handle))
         self.step = self.frames_per_window * RF_STEP   # reference: chunk_artifact.py:71-73
         _SERIAL[0] += 1
         self._serial = _SERIAL[0]
         _LIVE.add(self)
+
+    def _variant(self, state_dict, ptr, keep) -> L.VtcVariant:
+        """The C description of self.variant; tensor shapes are checked here, the library only sees pointers."""
+        v, out = self.variant, L.VtcVariant()
+
+        def check(name, shape):
+            if tuple(np.shape(state_dict[name])) != shape:
+                raise ValueError(f"{name} has shape {tuple(np.shape(state_dict[name]))}, expected {shape}")
+
+        def take(name, shape):
+            check(name, shape)
+            return ptr(name)
+
+        if v.conv_norm_groups:
+            out.conv_norm_groups = v.conv_norm_groups
+            for i in range(1, 7):
+                p = f"feature_extractor.conv_layers.{i}.layer_norm."
+                out.conv_gn_w[i], out.conv_gn_b[i] = take(p + "weight", (512,)), take(p + "bias", (512,))
+        if v.rotary is not None:
+            out.rotary, freq = v.rotary._struct(64)
+            keep.append(freq)
+        inner = 3072
+        if FFN_ACTS[v.ffn]:
+            out.ffn_act = FFN_ACTS[v.ffn]
+            inner = out.ffn_inner = int(np.shape(state_dict["encoder.layers.0.feed_forward.gate_dense.weight"])[0])
+            for l in range(L.N_LAYERS):
+                p = f"encoder.layers.{l}.feed_forward.gate_dense."
+                out.gate_w[l], out.gate_b[l] = take(p + "weight", (inner, 768)), take(p + "bias", (inner,))
+        for l in range(L.N_LAYERS):
+            p = f"encoder.layers.{l}.feed_forward."
+            check(p + "intermediate_dense.weight", (inner, 768))
+            check(p + "intermediate_dense.bias", (inner,))
+            check(p + "output_dense.weight", (768, inner))
+        return out
 
     # ------------------------------------------------------------------ lifecycle
     def close(self):

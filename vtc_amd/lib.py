@@ -68,6 +68,12 @@ class VtcRows3(C.Structure):
     _fields_ = [("p", C.c_void_p), ("batch", C.c_int64), ("row", C.c_int64)]
 
 
+class VtcVariant(C.Structure):
+    _fields_ = [("conv_norm_groups", C.c_int32), ("ffn_act", C.c_int32), ("ffn_inner", C.c_int32), ("reserved", C.c_int32),
+                ("rotary", VtcRotary), ("conv_gn_w", _f32p * 7), ("conv_gn_b", _f32p * 7), ("gate_w", _f32p * N_LAYERS),
+                ("gate_b", _f32p * N_LAYERS)]
+
+
 class VtcMat(C.Structure):
     _fields_ = [("p", C.c_void_p), ("row", C.c_int64)]
 
@@ -82,6 +88,7 @@ _i64p, _i32p, _f64p = C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.POINTER(C.c_
 _matp = C.POINTER(VtcMat)
 SYMBOLS = {
     "vtc_create": (C.c_int, [C.POINTER(VtcSpec), C.POINTER(VtcWeights), C.c_int, C.POINTER(C.c_void_p)]),
+    "vtc_create_variant": (C.c_int, [C.POINTER(VtcSpec), C.POINTER(VtcWeights), C.POINTER(VtcVariant), C.c_int, C.POINTER(C.c_void_p)]),
     "vtc_destroy": (None, [C.c_void_p]),
     "vtc_last_error": (C.c_char_p, [C.c_void_p]),
     "vtc_frames_per_window": (C.c_int, [C.c_void_p]),

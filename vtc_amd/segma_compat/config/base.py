@@ -33,8 +33,23 @@ class EngineConfig:
 
 
 @dataclass
+class EncoderConfig:
+    """Pieces of the encoder that differ from HuBERT-base (engine.EncoderVariant); the defaults are HuBERT-base's."""
+    position: str = "conv"             # "conv" (positional conv) | "rotary"
+    rotary_dim: int = 64
+    rotary_layout: str = "half"        # "half" | "interleaved"
+    rotary_base: float = 10000.0
+    rotary_scaling: str = "none"       # "none" | "linear" | "ntk" | "by_parts"
+    rotary_factor: float = 1.0
+    rotary_original_length: int = 0    # by_parts: frames per window the model was trained on
+    ffn: str = "gelu"                  # "gelu" | "gated_gelu" | "gated_silu" | "gated_sigmoid"
+    conv_norm_groups: int = 0          # group norm behind conv layers 1..6
+
+
+@dataclass
 class Config:
     data: DataConfig = field(default_factory=DataConfig)
     model: ModelConfig = field(default_factory=ModelConfig)
     audio: AudioConfig = field(default_factory=AudioConfig)
     engine: EngineConfig = field(default_factory=EngineConfig)
+    encoder: EncoderConfig = field(default_factory=EncoderConfig)

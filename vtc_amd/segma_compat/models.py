@@ -13,7 +13,8 @@ from pathlib import Path
 import numpy as np
 import torch
 
-from ..engine import VtcEngine
+from ..engine import EncoderVariant, VtcEngine
+from ..ops import Rotary
 from .. import synth
 
 _ANCHOR = "feature_extractor.conv_layers.0.conv.weight"
@@ -109,6 +110,17 @@ def normalise_state_dict(sd: dict, n_labels: int) -> dict:
     return out
 
 
+def encoder_variant(cfg) -> EncoderVariant:
+    """The `encoder` block of a config as what the engine takes."""
+    if cfg.position not in ("conv", "rotary"):
+        raise ValueError(f"encoder.position must be 'conv' or 'rotary', got {cfg.position!r}")
+    rotary = None
+    if cfg.position == "rotary":
+        rotary = Rotary(cfg.rotary_dim, layout=cfg.rotary_layout, base=cfg.rotary_base, scaling=cfg.rotary_scaling,
+                        factor=cfg.rotary_factor, original_length=cfg.rotary_original_length)
+    return EncoderVariant(rotary=rotary, ffn=cfg.ffn, conv_norm_groups=cfg.conv_norm_groups)
+
+
 class VtcModel:
     conv_settings = ConvSettings()
 
@@ -116,6 +128,7 @@ class VtcModel:
         self.state_dict_host = state_dict
         self.label_encoder = label_encoder
         self.config = config
+        self.variant = encoder_variant(config.encoder) if hasattr(config, "encoder") else EncoderVariant()
         self.device = torch.device("cpu")
         self._engines = {}
         self._rescue = {}
@@ -128,6 +141,8 @@ class VtcModel:
         if cp.startswith("synthetic"):
             seed = int(cp.split(":", 1)[1]) if ":" in cp else int(getattr(config.engine, "synthetic_seed", 0))
             sd = synth.make_weights(seed=seed, n_labels=label_encoder.n_labels)
+            if hasattr(config, "encoder"):
+                sd = synth.variant_weights(sd, seed, ffn=config.encoder.ffn, conv_norm_groups=config.encoder.conv_norm_groups)
         else:
             sd = normalise_state_dict(_load_state_dict(Path(cp)), label_encoder.n_labels)
         return cls(sd, label_encoder, config)
@@ -151,7 +166,8 @@ class VtcModel:
                 e.close()
             self._engines.clear()
             self._engines[key] = VtcEngine(self.state_dict_host, self.label_encoder.n_labels, chunk_duration_s,
-                                           max_batch=key[1], mfma_dtype=self.config.engine.mfma_dtype, device=index)
+                                           max_batch=key[1], mfma_dtype=self.config.engine.mfma_dtype, device=index,
+                                           variant=self.variant)
         return self._engines[key]
 
     def rescue_engine(self, chunk_duration_s: float, batch_size: int, device=None) -> VtcEngine:
@@ -166,7 +182,8 @@ class VtcModel:
                 e.close()
             self._rescue.clear()
             self._rescue[key] = VtcEngine(self.state_dict_host, self.label_encoder.n_labels, chunk_duration_s,
-                                          max_batch=int(batch_size), mfma_dtype="bf16", device=index)
+                                          max_batch=int(batch_size), mfma_dtype="bf16", device=index,
+                                          variant=self.variant)
         return self._rescue[key]
 
     def close_rescue(self):

@@ -137,6 +137,31 @@ def make_weights(seed: int = 0, n_labels: int = 4, logit_std: float = 2.0, famil
     return w
 
 
+def variant_weights(w: dict, seed: int, ffn: str = "gelu", conv_norm_groups: int = 0, inner: int = 2048, hub: bool = False) -> dict:
+    """The tensors of an encoder variant (engine.EncoderVariant) beside make_weights' (its own PCG64 stream, so the base tensors are
+    unchanged): a gated block of `inner` columns (2/3 of the dense block's width: as many parameters) in place of the dense
+    one, and the affine of the conv layers' group norms.  hub: initialisation scales of family "hubert"."""
+    if ffn == "gelu" and not conv_norm_groups:
+        return w
+    w = dict(w)
+    rng = np.random.default_rng([seed, 0x6A7E])
+
+    def randn(*shape, std):
+        return rng.standard_normal(shape, dtype=np.float32) * np.float32(std)
+
+    if conv_norm_groups:
+        for i in range(1, 7):
+            p = f"feature_extractor.conv_layers.{i}.layer_norm."
+            w[p + "weight"], w[p + "bias"] = 1.0 + randn(512, std=0.0 if hub else 0.1), randn(512, std=0.0 if hub else 0.1)
+    if ffn != "gelu":
+        for l in range(12):
+            p = f"encoder.layers.{l}.feed_forward."
+            for nm, n, k in (("gate_dense", inner, 768), ("intermediate_dense", inner, 768), ("output_dense", 768, inner)):
+                w[p + nm + ".weight"] = randn(n, k, std=0.02 if hub else k ** -0.5)
+                w[p + nm + ".bias"] = randn(n, std=0.0 if hub else 0.02)
+    return w
+
+
 N_OUTLIER_CHANNELS = 6
 
 
