@@ -317,6 +317,27 @@ def test_group_norm_forward_and_backward(kind, n, t, c, groups):
 
 @gpu
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,t,c,groups", [(2, 8000, 32, 2), (2, 8192, 16, 16), (2, 8193, 16, 16), (3, 700, 128, 4), (2, 500, 128, 2), (2, 2049, 64, 8),
+                                          (9, 1, 64, 4), (2, 515, 128, 1)])
+def test_group_norm_samples_that_fit_on_chip_and_just_do_not(kind, n, t, c, groups):
+    test_group_norm_forward_and_backward(kind, n, t, c, groups)
+
+
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_group_norm_sample_does_not_depend_on_its_batch(kind):
+    g = torch.Generator(device="cuda").manual_seed(21)
+    for t, c, groups in ((300, 64, 4), (9000, 32, 2), (130, 45, 5)):
+        x, dy = (torch.randn((5, t, c), generator=g, device="cuda").to(TYPES[kind]) for _ in range(2))
+        y, m, r = ops.group_norm_act_forward(x, groups, act="gelu")
+        dx, _, _ = ops.group_norm_act_backward(dy, x, groups, m, r, act="gelu")
+        y1, m1, r1 = ops.group_norm_act_forward(x[3:4], groups, act="gelu")
+        assert torch.equal(y[3:4], y1) and torch.equal(m[3:4], m1)
+        assert torch.equal(dx[3:4], ops.group_norm_act_backward(dy[3:4], x[3:4], groups, m1, r1, act="gelu")[0])
+
+
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("act", ["none", "gelu", "silu"])
 @pytest.mark.parametrize("c,groups", [(64, 4), (64, 64), (45, 5), (512, 32)])
 def test_group_norm_padded_batches(kind, act, c, groups):

@@ -31,6 +31,7 @@ struct GnParams {
   void *dw, *db;                // gradients of the affine, may be null
   long long N, L;
   int C, G, cpg, cv, rows, chunks;   // cv = C / VEC; rows per row block (chunk)
+  int cvb;                      // whole-sample kernels: 16-byte channel vectors of a block
   int affine_f32;               // w, b, dw, db are fp32 (else the tensors' type)
   float eps;
 };
@@ -72,6 +73,7 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const GnParams p) {
     if (on) {
       const T* src = x + (long long)v * VEC;
       OpVec<DT, VEC>::load(src, first);
+#pragma unroll 8
       for (int r = tr; r < rows; r += rp) {
         float f[VEC];
         OpVec<DT, VEC>::load(src + r * p.xl, f);
@@ -122,26 +124,36 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const GnParams p) {
   }
 }
 
-// ---- merge the row blocks of a sample: one thread per group walks them in order
-template <int DT>
-__global__ __launch_bounds__(64) void gn_finalize_kernel(const GnParams p) {
-  const unsigned per = (unsigned)(p.G + 63) / 64;
+// ---- merge the row blocks of a sample: 16 groups x 16 threads, thread i takes row blocks i, i + 16, .., their results merge in order
+struct GnMoment { double mean, m2, cnt; };
+__device__ __forceinline__ void gn_merge(GnMoment& a, double mean, double m2, double cnt) {   // Chan's formula
+  if (cnt == 0.0) return;
+  const double d = mean - a.mean, tot = a.cnt + cnt;
+  a.mean += d * (cnt / tot);
+  a.m2 += m2 + d * d * (a.cnt * cnt / tot);
+  a.cnt = tot;
+}
+__global__ __launch_bounds__(256) void gn_finalize_kernel(const GnParams p) {
+  __shared__ GnMoment sh[16][16];
+  const unsigned per = (unsigned)(p.G + 15) / 16;
   const long long n = blockIdx.x / per;
-  const int g = (int)(blockIdx.x % per) * 64 + threadIdx.x;
-  if (g >= p.G) return;
+  const int g = (int)(blockIdx.x % per) * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
   const long long len = gn_length(p, n);
-  double mean = 0.0, m2 = 0.0, cnt = 0.0;
-  const float2* part = (const float2*)p.part + n * p.chunks * p.G + g;
-  for (int k = 0; k < p.chunks && (long long)k * p.rows < len; ++k) {
-    const float2 t = part[(long long)k * p.G];
-    const double c = (double)min((long long)p.rows, len - (long long)k * p.rows) * p.cpg;
-    const double d = (double)t.x - mean, tot = cnt + c;
-    mean += d * (c / tot);
-    m2 += (double)t.y + d * d * (cnt * c / tot);
-    cnt = tot;
+  GnMoment a{0.0, 0.0, 0.0};
+  if (g < p.G) {
+    const float2* part = (const float2*)p.part + n * p.chunks * p.G + g;
+    const int live = (int)min((long long)p.chunks, (len + p.rows - 1) / p.rows);
+    for (int k = slice; k < live; k += 16) {
+      const float2 t = part[(long long)k * p.G];
+      gn_merge(a, t.x, t.y, (double)min((long long)p.rows, len - (long long)k * p.rows) * p.cpg);
+    }
   }
-  p.mean[n * p.G + g] = (float)mean;
-  p.rstd[n * p.G + g] = cnt > 0.0 ? (float)(1.0 / sqrt(m2 / cnt + (double)p.eps)) : 0.f;
+  sh[slice][threadIdx.x & 15] = a;
+  __syncthreads();
+  if (slice || g >= p.G) return;
+  for (int i = 1; i < 16; ++i) { const GnMoment& o = sh[i][threadIdx.x]; gn_merge(a, o.mean, o.m2, o.cnt); }
+  p.mean[n * p.G + g] = (float)a.mean;
+  p.rstd[n * p.G + g] = a.cnt > 0.0 ? (float)(1.0 / sqrt(a.m2 / a.cnt + (double)p.eps)) : 0.f;
 }
 
 // ---- y = act((x - mean) rstd w + b), row blocks again; rows behind the length become zero
@@ -165,6 +177,8 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
       mu[k] = p.mean[n * p.G + g];
       a[k] = p.rstd[n * p.G + g] * gn_param<DT>(p.w, c, p.affine_f32, 1.f);
       b[k] = gn_param<DT>(p.b, c, p.affine_f32, 0.f);
+      // 16-bit inputs: the mean folded into the offset costs |mean| rstd |w| 2^-24, their own rounding is 2^11 times that
+      if constexpr (DT != 0) b[k] = fmaf(-mu[k], a[k], b[k]);
     }
     const T* xs = x + (long long)v * VEC;
     T* ys = y + (long long)v * VEC;
@@ -174,7 +188,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
       float f[VEC];
       OpVec<DT, VEC>::load(xs + r * p.xl, f);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) f[k] = op_act<ACT, DT == 0>(fmaf(f[k] - mu[k], a[k], b[k]));
+      for (int k = 0; k < VEC; ++k) f[k] = op_act<ACT, DT == 0>(DT == 0 ? fmaf(f[k] - mu[k], a[k], b[k]) : fmaf(f[k], a[k], b[k]));
       OpVec<DT, VEC>::store(ys + r * p.ol, f);
     }
     for (; r < rows; r += rp) {
@@ -252,20 +266,28 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(const GnParams p) {
   }
 }
 
-// ---- pass 2a: sums over the row blocks of a sample, fp64, a thread per channel
-__global__ __launch_bounds__(64) void gn_bwd_merge_kernel(const GnParams p) {
+// ---- pass 2a: sums over the row blocks of a sample, fp64, 4 threads per channel
+__global__ __launch_bounds__(256) void gn_bwd_merge_kernel(const GnParams p) {
+  __shared__ double2 sh[4][64];
   const unsigned per = (unsigned)(p.C + 63) / 64;
   const long long n = blockIdx.x / per;
-  const int c = (int)(blockIdx.x % per) * 64 + threadIdx.x;
-  if (c >= p.C) return;
+  const int c = (int)(blockIdx.x % per) * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
   const long long len = gn_length(p, n);
-  const float2* part = (const float2*)p.part + n * p.chunks * p.C + c;
   double s = 0.0, q = 0.0;
-  for (int k = 0; k < p.chunks && (long long)k * p.rows < len; ++k) {
-    const float2 t = part[(long long)k * p.C];
-    s += t.x;
-    q += t.y;
+  if (c < p.C) {
+    const float2* part = (const float2*)p.part + n * p.chunks * p.C + c;
+    const int live = (int)min((long long)p.chunks, (len + p.rows - 1) / p.rows);
+#pragma unroll 4
+    for (int k = slice; k < live; k += 4) {
+      const float2 t = part[(long long)k * p.C];
+      s += t.x;
+      q += t.y;
+    }
   }
+  sh[slice][threadIdx.x & 63] = make_double2(s, q);
+  __syncthreads();
+  if (slice || c >= p.C) return;
+  for (int i = 1; i < 4; ++i) { s += sh[i][threadIdx.x].x; q += sh[i][threadIdx.x].y; }
   p.sums[(n * p.C + c) * 2] = s;
   p.sums[(n * p.C + c) * 2 + 1] = q;
 }
@@ -356,6 +378,259 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnParams p) {
       for (int k = 0; k < VEC; ++k) f[k] = 0.f;
       OpVec<DT, VEC>::store(dx + r * p.ol + (long long)v * VEC, f);
     }
+  }
+}
+
+// ---- whole samples on chip: one block owns `bc` channels (whole groups, at least 32 B of a row) of one sample and keeps its rows in
+// registers, so x (and dy) are read once.  512 threads, NV 16-byte vectors each: vector i of thread t is piece (t + 512 i), piece
+// = row * cvb + channel vector.  Bound: HBM and the activation's VALU work, about equal.  Neighbouring
+// blocks share 128-byte lines and run on one XCD (xcd_remap), so the L2 serves the other parts of a line.
+template <int DT> struct GnVec {
+  static constexpr int VEC = 16 / (int)sizeof(typename OpType<DT>::T);
+  static __device__ __forceinline__ void unpack(const u16x8& r, float (&f)[VEC]) {
+    if constexpr (DT == 0) {
+      const f32x4 v = __builtin_bit_cast(f32x4, r);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = v[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = from_h16<DT == 1>(r[k]);
+    }
+  }
+  static __device__ __forceinline__ u16x8 pack(const float (&f)[VEC]) {
+    if constexpr (DT == 0) return __builtin_bit_cast(u16x8, f32x4{f[0], f[1], f[2], f[3]});
+    else {
+      u16x8 r;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) r[k] = to_h16<DT == 1>(f[k]);
+      return r;
+    }
+  }
+};
+
+// sum over the lanes of a row of 16 that hold the same channel vector (lane % cvb), on the VALU (DPP rotations)
+template <int CTRL> __device__ __forceinline__ float gn_ror_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float gn_row_sum(float v, int cvb) {
+  if (cvb <= 1) v = gn_ror_add<0x121>(v);
+  if (cvb <= 2) v = gn_ror_add<0x122>(v);
+  if (cvb <= 4) v = gn_ror_add<0x124>(v);
+  if (cvb <= 8) v = gn_ror_add<0x128>(v);
+  return v;
+}
+constexpr int kGnMaxCvb = 8;
+constexpr int kGnSlabThreads = 512;
+
+// Block sums of NQ values per channel vector: v in every thread on entry, tot[vector * NQ + k] on exit.  Fixed order.
+template <int NQ> __device__ __forceinline__ void gn_block_sums(const float (&v)[NQ], int cvb, float* red, float* tot) {
+  const int row = threadIdx.x >> 4, in = threadIdx.x & 15, outs = cvb * NQ;
+#pragma unroll
+  for (int k = 0; k < NQ; ++k) {
+    const float s = gn_row_sum(v[k], cvb);
+    if (in < cvb) red[row * outs + in * NQ + k] = s;   // 32 rows of 16 lanes
+  }
+  __syncthreads();
+  const int o = threadIdx.x >> 2, part = threadIdx.x & 3;   // at most 128 sums, 4 threads each
+  float s = 0.f;
+  if (o < outs)
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s += red[(part * 8 + r) * outs + o];
+  s += __shfl_xor(s, 1);
+  s += __shfl_xor(s, 2);
+  if (o < outs && part == 0) tot[o] = s;
+  __syncthreads();
+}
+
+template <int DT, int NV, int ACT>
+__global__ __launch_bounds__(kGnSlabThreads, 4) void gn_slab_kernel(const GnParams p) {
+  typedef typename OpType<DT>::T T;
+  constexpr int VEC = GnVec<DT>::VEC;
+  __shared__ float red[kGnSlabThreads / 16 * kGnMaxCvb * VEC], tot[kGnMaxCvb * VEC], gmean[kGnMaxCvb * VEC], grstd[kGnMaxCvb * VEC];
+  const int cvb = p.cvb, bc = cvb * VEC, bundles = p.C / bc, ngb = bc / p.cpg;
+  const unsigned blk = xcd_remap(blockIdx.x, gridDim.x);
+  const long long n = blk / (unsigned)bundles;
+  const int c_base = (int)(blk % (unsigned)bundles) * bc;
+  const int v = threadIdx.x & (cvb - 1), r0 = threadIdx.x / cvb, dr = kGnSlabThreads / cvb;
+  const long long len = gn_length(p, n);
+  const int real = (int)len;
+  const T* x = (const T*)p.x + n * p.xn + c_base + v * VEC;
+  T* y = (T*)p.out + n * p.on + c_base + v * VEC;
+  u16x8 data[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int r = r0 + i * dr;
+    if (r < real) data[i] = *(const u16x8*)(x + r * p.xl);
+  }
+  // One pass as the rows arrive: sums of x - f and (x - f)^2, f = the thread's own first value.  A set that holds its own shift
+  // cancels at most a factor of its size (NV rows), whatever the data; the threads' means and M2 then merge by Chan's formula.
+  float s[VEC], q[VEC], first[VEC], base[VEC];
+  const int cnt = r0 < real ? (real - r0 + dr - 1) / dr : 0;   // rows of this thread
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) s[k] = q[k] = first[k] = base[k] = 0.f;
+  if (cnt > 0) {
+    GnVec<DT>::unpack(*(const u16x8*)x, base);                 // the channels' values in row 0: the reference of every sum below
+    GnVec<DT>::unpack(data[0], first);
+  }
+#pragma unroll
+  for (int i = 1; i < NV; ++i)
+    if (r0 + i * dr < real) {
+      float f[VEC];
+      GnVec<DT>::unpack(data[i], f);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) { const float d = f[k] - first[k]; s[k] += d; q[k] = fmaf(d, d, q[k]); }
+    }
+  const float fc = (float)cnt, ic = cnt > 0 ? 1.f / fc : 0.f;
+  float v0[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) v0[k] = fmaf(fc, first[k] - base[k], s[k]);
+  gn_block_sums<VEC>(v0, cvb, red, tot);
+  const float inv = real > 0 ? 1.f / ((float)real * (float)p.cpg) : 0.f;
+  if ((int)threadIdx.x < ngb) {
+    double t = 0.0;
+    if (real > 0)
+      for (int c = 0; c < p.cpg; ++c) {
+        const int ch = threadIdx.x * p.cpg + c;
+        t += (double)op_load<DT>(((const T*)p.x)[n * p.xn + c_base + ch]) + (double)tot[ch] / (double)real;
+      }
+    gmean[threadIdx.x] = (float)(t / (double)p.cpg);
+  }
+  __syncthreads();
+  float mu[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    mu[k] = gmean[(v * VEC + k) / p.cpg];
+    const float d = fmaf(s[k], ic, first[k] - mu[k]);          // the thread's mean, from the group's
+    v0[k] = cnt > 0 ? fmaf(fc * d, d, fmaf(-s[k], s[k] * ic, q[k])) : 0.f;
+  }
+  gn_block_sums<VEC>(v0, cvb, red, tot);
+  if ((int)threadIdx.x < ngb) {
+    float t = 0.f;
+    for (int c = 0; c < p.cpg; ++c) t += tot[threadIdx.x * p.cpg + c];
+    const float rs = real > 0 ? (float)(1.0 / sqrt((double)t * (double)inv + (double)p.eps)) : 0.f;
+    grstd[threadIdx.x] = rs;
+    const long long g = n * p.G + c_base / p.cpg + threadIdx.x;
+    p.mean[g] = gmean[threadIdx.x];
+    p.rstd[g] = rs;
+  }
+  __syncthreads();
+  float a[VEC], b[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    const int c = c_base + v * VEC + k;
+    a[k] = grstd[(v * VEC + k) / p.cpg] * gn_param<DT>(p.w, c, p.affine_f32, 1.f);
+    b[k] = gn_param<DT>(p.b, c, p.affine_f32, 0.f);
+    if constexpr (DT != 0) b[k] = fmaf(-mu[k], a[k], b[k]);   // see gn_apply_kernel
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int r = r0 + i * dr;
+    if (r >= p.L) break;
+    float f[VEC];
+    if (r < real) {
+      GnVec<DT>::unpack(data[i], f);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = op_act<ACT, DT == 0>(DT == 0 ? fmaf(f[k] - mu[k], a[k], b[k]) : fmaf(f[k], a[k], b[k]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = 0.f;
+    }
+    *(u16x8*)(y + r * p.ol) = GnVec<DT>::pack(f);
+  }
+}
+
+// backward of the same: x stays in registers, and dz in fp32, so the slope is computed once
+template <int DT, int NV, int ACT>
+__global__ __launch_bounds__(kGnSlabThreads, NV <= 4 ? 4 : 2) void gn_bwd_slab_kernel(const GnParams p) {
+  typedef typename OpType<DT>::T T;
+  constexpr int VEC = GnVec<DT>::VEC;
+  __shared__ float red[kGnSlabThreads / 16 * kGnMaxCvb * 2 * VEC], tot[kGnMaxCvb * 2 * VEC], gA[kGnMaxCvb * VEC], gB[kGnMaxCvb * VEC];
+  const int cvb = p.cvb, bc = cvb * VEC, bundles = p.C / bc, ngb = bc / p.cpg;
+  const unsigned blk = xcd_remap(blockIdx.x, gridDim.x);
+  const long long n = blk / (unsigned)bundles;
+  const int c_base = (int)(blk % (unsigned)bundles) * bc;
+  const int v = threadIdx.x & (cvb - 1), r0 = threadIdx.x / cvb, dr = kGnSlabThreads / cvb;
+  const int real = (int)gn_length(p, n);
+  const T* x = (const T*)p.x + n * p.xn + c_base + v * VEC;
+  const T* dy = (const T*)p.dy + n * p.dn + c_base + v * VEC;
+  T* dx = (T*)p.out + n * p.on + c_base + v * VEC;
+  u16x8 xd[NV], yd[NV];
+  float dzk[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int r = r0 + i * dr;
+    if (r < real) {
+      xd[i] = *(const u16x8*)(x + r * p.xl);
+      yd[i] = *(const u16x8*)(dy + r * p.dl);
+    }
+  }
+  float mu[VEC], rs[VEC], w[VEC], b[VEC], s[2 * VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    const int c = c_base + v * VEC + k, g = c / p.cpg;
+    mu[k] = p.mean[n * p.G + g];
+    rs[k] = p.rstd[n * p.G + g];
+    w[k] = gn_param<DT>(p.w, c, p.affine_f32, 1.f);
+    b[k] = gn_param<DT>(p.b, c, p.affine_f32, 0.f);
+    s[k] = s[VEC + k] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (r0 + i * dr < real) {
+      float f[VEC], d[VEC];
+      GnVec<DT>::unpack(xd[i], f);
+      GnVec<DT>::unpack(yd[i], d);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float h = (f[k] - mu[k]) * rs[k];
+        float a, g;
+        op_act_grad<ACT, DT == 0>(fmaf(h, w[k], b[k]), a, g);
+        const float dz = d[k] * g;
+        dzk[i][k] = dz;
+        s[k] += dz;
+        s[VEC + k] = fmaf(dz, h, s[VEC + k]);
+      }
+    }
+  gn_block_sums<2 * VEC>(s, cvb, red, tot);
+  if ((int)threadIdx.x < bc) {   // a channel's sums: for the affine's gradients, and into its group
+    const int vv = threadIdx.x / VEC, k = threadIdx.x % VEC;
+    double* o = p.sums + (n * p.C + c_base + threadIdx.x) * 2;
+    o[0] = tot[vv * 2 * VEC + k];
+    o[1] = tot[vv * 2 * VEC + VEC + k];
+  }
+  if ((int)threadIdx.x < ngb) {
+    const float inv = real > 0 ? 1.f / ((float)real * (float)p.cpg) : 0.f;
+    float A = 0.f, B = 0.f;
+    for (int i = 0; i < p.cpg; ++i) {
+      const int c = threadIdx.x * p.cpg + i, vv = c / VEC, k = c % VEC;
+      const float wc = gn_param<DT>(p.w, c_base + c, p.affine_f32, 1.f);
+      A = fmaf(wc, tot[vv * 2 * VEC + k], A);
+      B = fmaf(wc, tot[vv * 2 * VEC + VEC + k], B);
+    }
+    gA[threadIdx.x] = A * inv;
+    gB[threadIdx.x] = B * inv;
+  }
+  __syncthreads();
+  float A[VEC], B[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) { A[k] = gA[(v * VEC + k) / p.cpg]; B[k] = gB[(v * VEC + k) / p.cpg]; }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int r = r0 + i * dr;
+    if (r >= p.L) break;
+    float f[VEC];
+    if (r < real) {
+      GnVec<DT>::unpack(xd[i], f);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float h = (f[k] - mu[k]) * rs[k];
+        f[k] = rs[k] * fmaf(dzk[i][k], w[k], -fmaf(h, B[k], A[k]));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = 0.f;
+    }
+    *(u16x8*)(dx + r * p.ol) = GnVec<DT>::pack(f);
   }
 }
 

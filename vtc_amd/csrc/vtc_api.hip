@@ -782,9 +782,8 @@ int vtc_create_variant(const vtc_spec* spec, const vtc_weights* w, const vtc_var
   TRY(dev_alloc(m, &m->ffn16, MT * inner));
   if (!rot) TRY(dev_alloc(m, &m->posin, B * 16 * (size_t)(m->T + 128) * 48));
   if (m->conv_norm_groups) {
-    for (size_t b = 1; b <= B; ++b)   // any number of windows up to max_batch: row blocks per window shrink as there are more
-      for (int i = 1; i < 7; ++i)
-        m->conv_gn_ws_bytes = std::max(m->conv_gn_ws_bytes, vtc_group_norm_act_workspace((int64_t)b, m->L[i], 512, m->conv_norm_groups, 0));
+    for (int i = 1; i < 7; ++i)
+      m->conv_gn_ws_bytes = std::max(m->conv_gn_ws_bytes, vtc_group_norm_act_workspace((int64_t)B, m->L[i], 512, m->conv_norm_groups, 0));
     TRY(dev_alloc(m, &m->conv_gn_ws, (size_t)m->conv_gn_ws_bytes));
     TRY(dev_alloc(m, &m->conv_gn_stat, B * 2 * m->conv_norm_groups));
   }

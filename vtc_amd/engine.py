@@ -132,7 +132,7 @@ class VtcEngine:
 
         spec = L.VtcSpec(abi_version=L.ABI_VERSION, n_labels=self.n_labels, window_samples=self.window_samples,
                          max_batch=self.max_batch, mfma_dtype=DTYPES[mfma_dtype])
-        L.check(self._lib.vtc_create_variant(C.byref(spec), C.byref(w), C.byref(self._variant(state_dict, ptr, keep)), dev_index,
+        L.check(self._lib.vtc_create_variant(C.byref(spec), C.byref(w), C.byref(self._variant(state_dict, ptr)), dev_index,
                                              C.byref(self._handle)), None)
         self.frames_per_window = int(self._lib.vtc_frames_per_window(self._handle))
         self.step = self.frames_per_window * RF_STEP   # reference: chunk_artifact.py:71-73
@@ -140,7 +140,7 @@ class VtcEngine:
         self._serial = _SERIAL[0]
         _LIVE.add(self)
 
-    def _variant(self, state_dict, ptr, keep) -> L.VtcVariant:
+    def _variant(self, state_dict, ptr) -> L.VtcVariant:
         """The C description of self.variant; tensor shapes are checked here, the library only sees pointers."""
         v, out = self.variant, L.VtcVariant()
 
@@ -158,8 +158,7 @@ class VtcEngine:
                 p = f"feature_extractor.conv_layers.{i}.layer_norm."
                 out.conv_gn_w[i], out.conv_gn_b[i] = take(p + "weight", (512,)), take(p + "bias", (512,))
         if v.rotary is not None:
-            out.rotary, freq = v.rotary._struct(64)
-            keep.append(freq)
+            out.rotary = v.rotary._struct(64)
         inner = 3072
         if FFN_ACTS[v.ffn]:
             out.ffn_act = FFN_ACTS[v.ffn]

@@ -25,37 +25,49 @@ LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = ("none", "linear", "ntk", "by_parts")
 
 
+_so = None
+
+
+def _library():
+    global _so
+    if _so is None:
+        _so = L.load()
+    return _so
+
+
 def _need_gpu(x: torch.Tensor, what: str) -> int:
+    """The index of x's GPU."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what}: expected a tensor, got {type(x).__name__}")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError(f"{what}: tensors must be on a ROCm GPU (there is no CPU path), got {x.device}")
-    return x.device.index
+    return x.get_device()
 
 
-def _same(what: str, x: torch.Tensor, **others) -> None:
-    for name, t in others.items():
-        if t is not None and (t.device != x.device or t.dtype != x.dtype):
-            raise ValueError(f"{what}: {name} is {t.dtype} on {t.device}, expected {x.dtype} on {x.device}")
+def _same(what: str, x: torch.Tensor, name: str, t) -> None:
+    if t.dtype is not x.dtype or not t.is_cuda or t.get_device() != x.get_device():
+        raise ValueError(f"{what}: {name} is {t.dtype} on {t.device}, expected {x.dtype} on {x.device}")
 
 
-def _dtype(x: torch.Tensor, what: str, allowed=(torch.float32, torch.float16, torch.bfloat16)) -> int:
-    if x.dtype not in allowed:
+def _dtype(x: torch.Tensor, what: str, allowed=_DTYPES) -> int:
+    dt = allowed.get(x.dtype)
+    if dt is None:
         raise ValueError(f"{what}: type {x.dtype} is not one of {', '.join(str(a) for a in allowed)}")
-    return _DTYPES[x.dtype]
+    return dt
 
 
-def _stream(device) -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+# the raw handle without a Stream object around it, which costs several microseconds per call
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _ptr(t) -> C.c_void_p:
-    return C.c_void_p(0 if t is None else t.data_ptr())
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
-def _workspace(n: int, device) -> torch.Tensor:
+def _workspace(n: int, x: torch.Tensor) -> torch.Tensor:
     # the allocator's blocks start at multiples of 512 bytes; inside a graph capture they come from the graph's own pool
-    return torch.empty(max(int(n), 1), dtype=torch.uint8, device=device)
+    return torch.empty(n if n > 0 else 1, dtype=torch.uint8, device=x.device)
 
 
 # ------------------------------------------------------------------------------------------------ rotary positions
@@ -70,10 +82,10 @@ class Rotary:
                 than once are divided by `factor`, between them a ramp linear in the pair's index; the result is multiplied by
                 1 + 0.1 ln(factor)
 
-    Frequencies are 64-bit; `frequency` and `amplitude` may be replaced by the caller's own."""
+    Frequencies are 64-bit; frequency= and amplitude= give the caller's own instead.  The object does not change once it is made."""
 
     def __init__(self, rotary_dim: int, layout: str = "half", base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
-                 original_length: int = 0):
+                 original_length: int = 0, frequency=None, amplitude: float | None = None):
         r, s = int(rotary_dim), float(factor)
         if r < 2 or r % 2 or r > 512:
             raise ValueError(f"rotary_dim must be even and in 2..512, got {rotary_dim}")
@@ -100,15 +112,23 @@ class Rotary:
             ramp = np.clip((j - low) / max(high - low, 1e-3), 0.0, 1.0)
             f = f / s * ramp + f * (1.0 - ramp)
             self.amplitude = 0.1 * math.log(s) + 1.0 if s > 1.0 else 1.0
-        self.frequency = np.ascontiguousarray(f)
+        if frequency is not None:
+            f = np.array(frequency, dtype=np.float64)
+        if amplitude is not None:
+            self.amplitude = float(amplitude)
+        if f.shape != (r // 2,):
+            raise ValueError(f"frequency must have {r // 2} entries, got shape {f.shape}")
+        f.setflags(write=False)
+        self.frequency = f
+        self._structs = {}
 
-    def _struct(self, head_dim: int):
-        f = np.ascontiguousarray(self.frequency, dtype=np.float64)
-        if f.shape != (self.rotary_dim // 2,):
-            raise ValueError(f"frequency must have {self.rotary_dim // 2} entries, got shape {f.shape}")
-        s = L.VtcRotary(head_dim=head_dim, rotary_dim=self.rotary_dim, layout=LAYOUTS[self.layout], amplitude=float(self.amplitude),
-                        frequency=f.ctypes.data_as(L._f64p))
-        return s, f   # f has to live until the call returns
+    def _struct(self, head_dim: int) -> L.VtcRotary:
+        """The C description for heads of this size (it points into self.frequency)."""
+        s = self._structs.get(head_dim)
+        if s is None:
+            s = self._structs[head_dim] = L.VtcRotary(head_dim, self.rotary_dim, LAYOUTS[self.layout], 0, self.amplitude,
+                                                      self.frequency.ctypes.data_as(L._f64p))
+        return s
 
 
 def _rotary_call(tensors, spec: Rotary, positions, offset: int, inverse: bool, outs):
@@ -117,50 +137,58 @@ def _rotary_call(tensors, spec: Rotary, positions, offset: int, inverse: bool, o
     dt = _dtype(x0, "rotary")
     if not isinstance(spec, Rotary):
         raise TypeError("rotary: expected a Rotary")
-    if x0.dim() not in (3, 4):
-        raise ValueError(f"rotary: tensors are (batch, length, heads, head_dim) or (length, heads, head_dim), got {tuple(x0.shape)}")
-    batch, length = (x0.shape[0], x0.shape[1]) if x0.dim() == 4 else (1, x0.shape[0])
-    head_dim = x0.shape[-1]
+    shape0 = x0.shape
+    nd = len(shape0)
+    if nd == 4:
+        batch, length, _, head_dim = shape0
+    elif nd == 3:
+        (length, _, head_dim), batch = shape0, 1
+    else:
+        raise ValueError(f"rotary: tensors are (batch, length, heads, head_dim) or (length, heads, head_dim), got {tuple(shape0)}")
     if spec.rotary_dim > head_dim:
         raise ValueError(f"rotary: rotary_dim {spec.rotary_dim} is more than head_dim {head_dim}")
-    arr = (L.VtcHeads * len(tensors))()
-    given = outs
-    outs = []
+    heads, results, empty = [], [], batch == 0 or length == 0
     for i, x in enumerate(tensors):
-        _same("rotary", x0, tensor=x)
-        if x.dim() != x0.dim() or x.shape[:-2] != x0.shape[:-2] or x.shape[-1] != head_dim:
-            raise ValueError(f"rotary: shapes {tuple(x0.shape)} and {tuple(x.shape)} do not go together")
-        if x.numel() and x.stride(-1) != 1:
+        shape = shape0
+        if x is not x0:
+            _same("rotary", x0, "a tensor", x)
+            shape = x.shape
+            if len(shape) != nd or shape[:-2] != shape0[:-2] or shape[-1] != head_dim:
+                raise ValueError(f"rotary: shapes {tuple(shape0)} and {tuple(shape)} do not go together")
+        sx = x.stride()
+        empty = empty or shape[-2] == 0
+        if sx[-1] != 1 and not empty:
             raise ValueError("rotary: the elements of a head must be contiguous")
-        y = given[i] if given is not None else None
-        if y is None:
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if outs is None:
+            y = torch.empty(shape, dtype=x.dtype, device=x.device)
         else:
-            _same("rotary", x0, out=y)
-            if y.shape != x.shape or (y.numel() and y.stride(-1) != 1):
-                raise ValueError(f"rotary: out must have shape {tuple(x.shape)} with contiguous heads, got {tuple(y.shape)}")
-        outs.append(y)
-        sx = ((0,) if x.dim() == 3 else ()) + x.stride()
-        sy = ((0,) if y.dim() == 3 else ()) + y.stride()
-        arr[i] = L.VtcHeads(x=x.data_ptr(), y=y.data_ptr(), x_batch=sx[0], x_row=sx[1], x_head=sx[2], y_batch=sy[0], y_row=sy[1],
-                            y_head=sy[2], heads=x.shape[-2])
+            y = outs[i]
+            _same("rotary", x0, "out", y)
+            if y.shape != shape or (y.stride(-1) != 1 and not empty):
+                raise ValueError(f"rotary: out must have shape {tuple(shape)} with contiguous heads, got {tuple(y.shape)}")
+        results.append(y)
+        sy = y.stride()
+        if nd == 3:
+            sx, sy = (0,) + sx, (0,) + sy
+        heads.append((x.data_ptr(), y.data_ptr(), sx[0], sx[1], sx[2], sy[0], sy[1], sy[2], shape[-2]))
     pos, pos64, pb, pt = None, 0, 0, 0
     if positions is not None:
-        if positions.device != x0.device or positions.dtype not in (torch.int32, torch.int64):
+        if not positions.is_cuda or positions.get_device() != index or positions.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"rotary: positions must be int32 or int64 on {x0.device}")
-        if positions.shape not in ((length,), (batch, length)):
-            raise ValueError(f"rotary: positions must have shape ({length},) or ({batch}, {length}), got {tuple(positions.shape)}")
-        pos, pos64 = positions, int(positions.dtype == torch.int64)
-        pb, pt = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
-    if batch == 0 or length == 0 or any(x.shape[-2] == 0 for x in tensors):
-        if all(y.numel() == 0 for y in outs):
-            return outs
+        shape = positions.shape
+        if shape != (batch, length) and shape != (length,):
+            raise ValueError(f"rotary: positions must have shape ({length},) or ({batch}, {length}), got {tuple(shape)}")
+        pos, pos64 = positions.data_ptr(), int(positions.dtype is torch.int64)
+        pb, pt = positions.stride() if len(shape) == 2 else (0, positions.stride(0))
+    if empty:
+        if all(y.numel() == 0 for y in results):
+            return results
         raise ValueError("rotary: a tensor without heads beside one with heads")
-    s, keep = spec._struct(head_dim)
-    L.check(L.load().vtc_rotary_heads(index, dt, C.byref(s), batch, length, arr, len(tensors), _ptr(pos), pos64, pb, pt, int(offset),
-                                      int(bool(inverse)), _stream(x0.device)))
-    del keep
-    return outs
+    rc = _library().vtc_rotary_heads(index, dt, spec._struct(head_dim), batch, length, (L.VtcHeads * len(heads))(*heads), len(heads), pos, pos64,
+                                     pb, pt, offset, 1 if inverse else 0, _stream(index))
+    if rc:
+        L.check(rc)
+    return results
 
 
 class _RotaryFunction(torch.autograd.Function):
@@ -209,36 +237,52 @@ def rotary(x: torch.Tensor, spec: Rotary, positions: torch.Tensor | None = None,
 
 
 # ------------------------------------------------------------------------------------------------ group norm + activation
+_GN_ACTS = ("none", "gelu", "silu")
+
+
 def _gn_args(what, x, groups, weight, bias, lengths, act):
     index = _need_gpu(x, what)
     dt = _dtype(x, what)
-    if x.dim() != 3:
-        raise ValueError(f"{what}: rows are (batch, length, channels), got {tuple(x.shape)}")
-    if x.numel() and x.stride(2) != 1:
+    shape = x.shape
+    if len(shape) != 3:
+        raise ValueError(f"{what}: rows are (batch, length, channels), got {tuple(shape)}")
+    n, t, c = shape
+    if x.stride(2) != 1 and n * t * c:
         raise ValueError(f"{what}: the channels of a row must be contiguous")
-    n, t, c = x.shape
     if groups < 1 or c < 1 or c % groups:
         raise ValueError(f"{what}: {c} channels do not divide into {groups} groups")
-    if act not in ("none", "gelu", "silu"):
+    if act not in _GN_ACTS:
         raise ValueError(f"{what}: act must be 'none', 'gelu' or 'silu', got {act!r}")
     f32 = 0
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
-        if p.device != x.device or p.shape != (c,) or not p.is_contiguous():
+        if not p.is_cuda or p.get_device() != index or p.shape != (c,) or not p.is_contiguous():
             raise ValueError(f"{what}: {name} must be contiguous with shape ({c},) on {x.device}")
-        if p.dtype not in (x.dtype, torch.float32):
-            raise ValueError(f"{what}: {name} must be {x.dtype} or float32, got {p.dtype}")
-        f32 = int(p.dtype == torch.float32)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        kind = p.dtype
+        if kind is not x.dtype and kind is not torch.float32:
+            raise ValueError(f"{what}: {name} must be {x.dtype} or float32, got {kind}")
+        f32 = 1 if kind is torch.float32 else 0
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise ValueError(f"{what}: weight and bias must have one type")
-    if lengths is not None and (lengths.device != x.device or lengths.dtype != torch.int32 or lengths.shape != (n,) or not lengths.is_contiguous()):
+    if lengths is not None and (not lengths.is_cuda or lengths.get_device() != index or lengths.dtype is not torch.int32 or lengths.shape != (n,) or
+                                not lengths.is_contiguous()):
         raise ValueError(f"{what}: lengths must be a contiguous int32 tensor of shape ({n},) on {x.device}")
-    return index, dt, f32
+    return index, dt, f32, n, t, c
 
 
 def _rows3(t):
-    return L.VtcRows3(p=t.data_ptr(), batch=t.stride(0), row=t.stride(1))
+    s = t.stride()
+    return L.VtcRows3(t.data_ptr(), s[0], s[1])
+
+
+def _gn_out(what, x, out):
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _same(what, x, "out", out)
+    if out.shape != x.shape or (out.numel() and out.stride(2) != 1):
+        raise ValueError(f"{what}: out must have shape {tuple(x.shape)} with contiguous channels")
+    return out
 
 
 def group_norm_act_forward(x: torch.Tensor, groups: int, weight=None, bias=None, eps: float = 1e-5, act: str = "none", lengths=None,
@@ -246,29 +290,24 @@ def group_norm_act_forward(x: torch.Tensor, groups: int, weight=None, bias=None,
     """(y, mean, rstd): y = act(group_norm(x)) on channel-last rows (batch, length, channels), statistics per sample and group of
     neighbouring channels over the first lengths[n] rows (int32 tensor, default all).  Rows behind a sample's length are not read
     and come out as zero.  weight / bias: of x's type or float32.  out: where y goes (x itself for in place).  mean and rstd
-    (batch, groups, float32) are what the backward call needs."""
+    (batch, groups, float32) are what the backward call needs.  A sample's result does not depend on the rest of its batch."""
     what = "group_norm_act"
-    index, dt, f32 = _gn_args(what, x, groups, weight, bias, lengths, act)
-    n, t, c = x.shape
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
-        _same(what, x, out=out)
-        if out.shape != x.shape or (out.numel() and out.stride(2) != 1):
-            raise ValueError(f"{what}: out must have shape {tuple(x.shape)} with contiguous channels")
-    mean = torch.empty((n, groups), dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
+    index, dt, f32, n, t, c = _gn_args(what, x, groups, weight, bias, lengths, act)
+    out = _gn_out(what, x, out)
+    mean, rstd = torch.empty((2, n, groups), dtype=torch.float32, device=x.device).unbind(0)
     if n == 0 or t == 0:
         mean.zero_()
         rstd.zero_()
         return out, mean, rstd
-    so = L.load()
+    so = _library()
     size = so.vtc_group_norm_act_workspace(n, t, c, groups, 0)
     if size < 0:
         L.check(int(size))
-    ws = _workspace(size, x.device)
-    L.check(so.vtc_group_norm_act(index, dt, C.byref(_rows3(x)), C.byref(_rows3(out)), n, t, c, int(groups), _ptr(weight), _ptr(bias), f32,
-                                  float(eps), ACTS[act], _ptr(lengths), _ptr(mean), _ptr(rstd), _ptr(ws), ws.numel(), _stream(x.device)))
+    ws = _workspace(size, x)
+    rc = so.vtc_group_norm_act(index, dt, _rows3(x), _rows3(out), n, t, c, groups, _ptr(weight), _ptr(bias), f32, eps, ACTS[act], _ptr(lengths),
+                               mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), size, _stream(index))
+    if rc:
+        L.check(rc)
     return out, mean, rstd
 
 
@@ -277,28 +316,25 @@ def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, groups: int, mean
     """(dx, dweight, dbias) for dy = dLoss / dy and the statistics of the forward call; dweight / dbias have the affine's type (None
     where there is none).  out: where dx goes (dy or x for in place)."""
     what = "group_norm_act_backward"
-    index, dt, f32 = _gn_args(what, x, groups, weight, bias, lengths, act)
-    n, t, c = x.shape
-    _same(what, x, dy=dy, out=out)
-    if dy.shape != x.shape or (dy.numel() and dy.stride(2) != 1):
+    index, dt, f32, n, t, c = _gn_args(what, x, groups, weight, bias, lengths, act)
+    _same(what, x, "dy", dy)
+    if dy.shape != x.shape or (dy.stride(2) != 1 and dy.numel()):
         raise ValueError(f"{what}: dy must have shape {tuple(x.shape)} with contiguous channels")
     for s in (mean, rstd):
-        if s.device != x.device or s.dtype != torch.float32 or s.shape != (n, groups) or not s.is_contiguous():
+        if not s.is_cuda or s.get_device() != index or s.dtype is not torch.float32 or s.shape != (n, groups) or not s.is_contiguous():
             raise ValueError(f"{what}: mean and rstd are the forward call's, float32 of shape ({n}, {groups})")
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or (out.numel() and out.stride(2) != 1):
-        raise ValueError(f"{what}: out must have shape {tuple(x.shape)} with contiguous channels")
+    out = _gn_out(what, x, out)
     dw = None if weight is None else torch.empty_like(weight)
     db = None if bias is None else torch.empty_like(bias)
-    so = L.load()
+    so = _library()
     size = so.vtc_group_norm_act_workspace(n, t, c, groups, 1)
     if size < 0:
         L.check(int(size))
-    ws = _workspace(size, x.device)
-    L.check(so.vtc_group_norm_act_backward(index, dt, C.byref(_rows3(dy)), C.byref(_rows3(x)), C.byref(_rows3(out)), n, t, c, int(groups),
-                                           _ptr(weight), _ptr(bias), f32, ACTS[act], _ptr(lengths), _ptr(mean), _ptr(rstd), _ptr(dw),
-                                           _ptr(db), _ptr(ws), ws.numel(), _stream(x.device)))
+    ws = _workspace(size, x)
+    rc = so.vtc_group_norm_act_backward(index, dt, _rows3(dy), _rows3(x), _rows3(out), n, t, c, groups, _ptr(weight), _ptr(bias), f32, ACTS[act],
+                                        _ptr(lengths), mean.data_ptr(), rstd.data_ptr(), _ptr(dw), _ptr(db), ws.data_ptr(), size, _stream(index))
+    if rc:
+        L.check(rc)
     return out, dw, db
 
 
@@ -329,39 +365,49 @@ def group_norm_act(x: torch.Tensor, groups: int, weight=None, bias=None, eps: fl
 
 
 # ------------------------------------------------------------------------------------------------ gated feed-forward
-def _mat(t):
-    return L.VtcMat(p=t.data_ptr(), row=max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0))
+_FFN_TYPES = {torch.float16: 1, torch.bfloat16: 2}
+
+
+def _mat(t, cols):
+    row = t.stride(0)
+    return L.VtcMat(t.data_ptr(), row if row > cols else cols)   # a single row may have any stride
 
 
 def _ffn_args(what, x, w_gate, w_up, w_down, biases, act):
     index = _need_gpu(x, what)
-    dt = _dtype(x, what, (torch.float16, torch.bfloat16))
-    _same(what, x, w_gate=w_gate, w_up=w_up, w_down=w_down)
-    if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.dim() != 2 or w_down.shape[1] != w_gate.shape[0] or x.dim() < 1 or x.shape[-1] != w_gate.shape[1]:
+    dt = _dtype(x, what, _FFN_TYPES)
+    _same(what, x, "w_gate", w_gate)
+    _same(what, x, "w_up", w_up)
+    _same(what, x, "w_down", w_down)
+    sg, su, sd = w_gate.shape, w_up.shape, w_down.shape
+    if len(sg) != 2 or su != sg or len(sd) != 2 or sd[1] != sg[0] or x.dim() < 1 or x.shape[-1] != sg[1]:
         raise ValueError(f"{what}: x (.., width), w_gate and w_up (inner, width), w_down (out, inner) do not go together: {tuple(x.shape)}, "
-                         f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
+                         f"{tuple(sg)}, {tuple(su)}, {tuple(sd)}")
     for name, t in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
-        if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        row, col = t.stride()
+        if col != 1 or (row < t.shape[1] and t.shape[0] > 1):
             raise ValueError(f"{what}: {name} must be stored row by row")
     if act not in ACTS:
         raise ValueError(f"{what}: act must be one of {list(ACTS)}, got {act!r}")
-    f32, kinds = 0, set()
-    for name, b, n in zip(("b_gate", "b_up", "b_down"), biases, (w_gate.shape[0], w_gate.shape[0], w_down.shape[0])):
+    kind = None
+    for i, b in enumerate(biases):
         if b is None:
             continue
-        if b.device != x.device or b.shape != (n,) or not b.is_contiguous() or b.dtype not in (x.dtype, torch.float32):
-            raise ValueError(f"{what}: {name} must be contiguous, of shape ({n},) and type {x.dtype} or float32 on {x.device}")
-        kinds.add(b.dtype)
-        f32 = int(b.dtype == torch.float32)
-    if len(kinds) > 1:
-        raise ValueError(f"{what}: the biases must have one type")
-    return index, dt, f32
+        if not b.is_cuda or b.get_device() != index or b.shape != ((sg[0],) if i < 2 else (sd[0],)) or not b.is_contiguous() or (
+                b.dtype is not x.dtype and b.dtype is not torch.float32):
+            raise ValueError(f"{what}: {('b_gate', 'b_up', 'b_down')[i]} must be contiguous, of shape ({sg[0] if i < 2 else sd[0]},) and type "
+                             f"{x.dtype} or float32 on {x.device}")
+        if kind is not None and b.dtype is not kind:
+            raise ValueError(f"{what}: the biases must have one type")
+        kind = b.dtype
+    return index, dt, 1 if kind is torch.float32 else 0, sg[1], sg[0], sd[0]
 
 
-def _rows2(t, what):
+def _rows2(t):
     """t (.., n) as rows (m, n) whose elements are contiguous; a view where the strides allow it."""
-    r = t.reshape(-1, t.shape[-1])
-    if r.numel() and (r.stride(1) != 1 or (r.shape[0] > 1 and r.stride(0) < r.shape[1])):
+    r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    row, col = r.stride()
+    if (col != 1 or (row < r.shape[1] and r.shape[0] > 1)) and r.numel():
         r = r.contiguous()
     return r
 
@@ -369,24 +415,27 @@ def _rows2(t, what):
 def gated_ffn_forward(x: torch.Tensor, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu", save: bool = False):
     """(y, saved): y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down on rows x (.., width) in float16 or bfloat16,
     sums in fp32; w_gate, w_up (inner, width), w_down (out, inner); biases of x's type or float32.  With save, `saved` is what
-    gated_ffn_backward needs (three times rows x inner in x's type), else None."""
+    gated_ffn_backward needs, an opaque buffer of vtc_gated_ffn_saved bytes; else None."""
     what = "gated_ffn"
-    index, dt, f32 = _ffn_args(what, x, w_gate, w_up, w_down, (b_gate, b_up, b_down), act)
-    rows = _rows2(x, what)
-    m, k = rows.shape
-    f, n = w_gate.shape[0], w_down.shape[0]
+    index, dt, f32, k, f, n = _ffn_args(what, x, w_gate, w_up, w_down, (b_gate, b_up, b_down), act)
+    rows = _rows2(x)
+    m = rows.shape[0]
     y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-    so = L.load()
+    so = _library()
     size = so.vtc_gated_ffn_workspace(m, k, f, n, 0)
     if size < 0:
         L.check(int(size))
-    saved = _workspace(so.vtc_gated_ffn_saved(m, f), x.device) if save else None
+    saved, saved_size = None, 0
+    if save:
+        saved_size = so.vtc_gated_ffn_saved(m, f)
+        saved = _workspace(saved_size, x)
     if m == 0:
         return y, saved
-    ws = _workspace(size, x.device)
-    L.check(so.vtc_gated_ffn(index, dt, m, k, f, n, C.byref(_mat(rows)), C.byref(_mat(w_gate)), C.byref(_mat(w_up)), C.byref(_mat(w_down)),
-                             _ptr(b_gate), _ptr(b_up), _ptr(b_down), f32, ACTS[act], C.byref(L.VtcMat(y.data_ptr(), n)), _ptr(saved),
-                             0 if saved is None else saved.numel(), _ptr(ws), ws.numel(), _stream(x.device)))
+    ws = _workspace(size, x)
+    rc = so.vtc_gated_ffn(index, dt, m, k, f, n, _mat(rows, k), _mat(w_gate, k), _mat(w_up, k), _mat(w_down, f), _ptr(b_gate), _ptr(b_up),
+                          _ptr(b_down), f32, ACTS[act], L.VtcMat(y.data_ptr(), n), _ptr(saved), saved_size, ws.data_ptr(), size, _stream(index))
+    if rc:
+        L.check(rc)
     return y, saved
 
 
@@ -395,16 +444,15 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate, w_up, w_down, 
     """(dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down) for dy = dLoss / dy and the forward call's `saved`; what is not asked for
     (biases, need_dx, need_dw) is None.  Gradients have the type of what they belong to (biases: bias_dtype, default x's)."""
     what = "gated_ffn_backward"
-    index, dt, _ = _ffn_args(what, x, w_gate, w_up, w_down, (None, None, None), act)
-    _same(what, x, dy=dy)
-    f, n = w_gate.shape[0], w_down.shape[0]
+    index, dt, _, k, f, n = _ffn_args(what, x, w_gate, w_up, w_down, (), act)
+    _same(what, x, "dy", dy)
     if dy.shape != x.shape[:-1] + (n,):
         raise ValueError(f"{what}: dy must have shape {tuple(x.shape[:-1] + (n,))}, got {tuple(dy.shape)}")
     bias_dtype = bias_dtype or x.dtype
     if bias_dtype not in (x.dtype, torch.float32):
         raise ValueError(f"{what}: bias_dtype must be {x.dtype} or float32")
-    rows, drows = _rows2(x, what), _rows2(dy, what)
-    m, k = rows.shape
+    rows, drows = _rows2(x), _rows2(dy)
+    m = rows.shape[0]
     new = lambda shape, kind: torch.empty(shape, dtype=kind, device=x.device)  # noqa: E731
     dx = new(x.shape, x.dtype) if need_dx else None
     dw = tuple(new(w.shape, x.dtype) if need_dw else None for w in (w_gate, w_up, w_down))
@@ -414,18 +462,19 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate, w_up, w_down, 
             if t is not None:
                 t.zero_()
         return (dx,) + dw + db
-    so = L.load()
+    so = _library()
     size = so.vtc_gated_ffn_workspace(m, k, f, n, 1)
     if size < 0:
         L.check(int(size))
-    if saved is None or saved.device != x.device or saved.dtype != torch.uint8 or saved.numel() < so.vtc_gated_ffn_saved(m, f):
+    if saved is None or not saved.is_cuda or saved.get_device() != index or saved.dtype is not torch.uint8 or saved.numel() < so.vtc_gated_ffn_saved(m, f):
         raise ValueError(f"{what}: saved is the forward call's (with save=True)")
-    ws = _workspace(size, x.device)
-    adr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    grads = L.VtcFfnGrads(adr(dx), k, *(adr(t) for t in dw + db))
-    L.check(so.vtc_gated_ffn_backward(index, dt, m, k, f, n, C.byref(_mat(drows)), C.byref(_mat(rows)), C.byref(_mat(w_gate)),
-                                      C.byref(_mat(w_up)), C.byref(_mat(w_down)), _ptr(saved), saved.numel(),
-                                      int(bias_dtype == torch.float32), ACTS[act], C.byref(grads), _ptr(ws), ws.numel(), _stream(x.device)))
+    ws = _workspace(size, x)
+    grads = L.VtcFfnGrads(_ptr(dx), k, *(_ptr(t) for t in dw + db))
+    rc = so.vtc_gated_ffn_backward(index, dt, m, k, f, n, _mat(drows, n), _mat(rows, k), _mat(w_gate, k), _mat(w_up, k), _mat(w_down, f),
+                                   saved.data_ptr(), saved.numel(), 1 if bias_dtype is torch.float32 else 0, ACTS[act], grads, ws.data_ptr(), size,
+                                   _stream(index))
+    if rc:
+        L.check(rc)
     return (dx,) + dw + db
 
 
