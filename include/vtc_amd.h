@@ -300,8 +300,8 @@ int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows3* dy, cons
  * h = act(g) * u (NONE, GELU, SILU, SIGMOID), y = h W_down^T + b_down.  x [rows][width], W_gate and W_up [inner][width], W_down
  * [out_width][inner] (as torch.nn.Linear keeps them), y [rows][out_width]; any sizes and row pitches (elements; operands whose
  * rows are not made of aligned 16-byte pieces are copied into the workspace first).  Biases may be NULL; of the operands' type, or
- * fp32 with bias_f32 = 1.  h, and with `saved` g, u and h for the backward call (vtc_gated_ffn_saved bytes, 256-byte aligned), are
- * rounded to the operands' type.
+ * fp32 with bias_f32 = 1.  h is rounded to the operands' type.  `saved` (vtc_gated_ffn_saved bytes, 256-byte aligned; NULL: no
+ * backward call follows) receives h and, in 24 bits, act(g) and u act'(g): the backward call needs no activation.
  * Backward: dy [rows][out_width] -> any of dx (row pitch dx_row), the weights' gradients (all three or none; dense, in the weights'
  * layout and type) and the biases' (of the biases' type); NULL leaves one out.  dx may not overlap x or dy. */
 typedef struct {
@@ -322,7 +322,7 @@ int vtc_gated_ffn(int device, int dtype, int64_t rows, int32_t width, int32_t in
                   int64_t workspace_bytes, void* stream);
 int vtc_gated_ffn_backward(int device, int dtype, int64_t rows, int32_t width, int32_t inner, int32_t out_width, const vtc_mat* dy,
                            const vtc_mat* x, const vtc_mat* w_gate, const vtc_mat* w_up, const vtc_mat* w_down, const void* saved,
-                           int64_t saved_bytes, int32_t bias_f32, int32_t act, const vtc_ffn_grads* grads, void* workspace,
+                           int64_t saved_bytes, int32_t bias_f32, const vtc_ffn_grads* grads, void* workspace,
                            int64_t workspace_bytes, void* stream);
 
 /* A model whose encoder differs from HuBERT-base in one or more of these pieces (everything else, and every call on the model, is

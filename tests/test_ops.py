@@ -735,7 +735,7 @@ def _ffn_c(backward=False, **over):
     mats = [ref(a[n]) for n in ("x", "wg", "wu", "wd")]
     if backward:
         grads = L.VtcFfnGrads(a["dx"], a["dx_row"], a["dw"], a["dw2"], a["dw"])
-        rc = so.vtc_gated_ffn_backward(0, a["dtype"], a["m"], a["k"], a["f"], a["n"], ref(a["y"]), *mats, a["saved"], a["saved_size"], a["f32"], a["act"],
+        rc = so.vtc_gated_ffn_backward(0, a["dtype"], a["m"], a["k"], a["f"], a["n"], ref(a["y"]), *mats, a["saved"], a["saved_size"], a["f32"],
                                        C.byref(grads), a["ws"], a["size"], None)
     else:
         rc = so.vtc_gated_ffn(0, a["dtype"], a["m"], a["k"], a["f"], a["n"], *mats, None, None, None, a["f32"], a["act"], ref(a["y"]), a["saved"],
@@ -745,7 +745,7 @@ def _ffn_c(backward=False, **over):
 
 @pytest.mark.parametrize("backward", [False, True])
 @pytest.mark.parametrize("over,text,code", [
-    (dict(dtype=0), "f16 or bf16", L.ERR_ARG), (dict(act=4), "activation", L.ERR_ARG), (dict(f32=2), "bias_f32", L.ERR_ARG),
+    (dict(dtype=0), "f16 or bf16", L.ERR_ARG), (dict(f32=2), "bias_f32", L.ERR_ARG),
     (dict(m=-1), "rows", L.ERR_ARG), (dict(m=1 << 31), "rows", L.ERR_ARG), (dict(k=0), "width", L.ERR_ARG), (dict(f=(1 << 18) + 1), "width", L.ERR_ARG),
     (dict(x=None), "x is null", L.ERR_ARG), (dict(wg=L.VtcMat(None, 64)), "w_gate is null", L.ERR_ARG), (dict(wd=L.VtcMat(4 << 20, 127)), "pitch", L.ERR_ARG),
     (dict(x=L.VtcMat(1 << 20, (1 << 20) + 1)), "pitch", L.ERR_ARG), (dict(x=L.VtcMat((1 << 20) + 1, 64)), "aligned", L.ERR_ARG),
@@ -757,7 +757,7 @@ def test_gated_ffn_refusals_of_the_library(backward, over, text, code):
 
 
 def test_gated_ffn_refusals_of_one_direction():
-    for backward, over, text in ((False, dict(y=L.VtcMat((1 << 20) + 64, 64)), "overlaps x"), (True, dict(dx=1 << 20), "overlaps"),
+    for backward, over, text in ((False, dict(y=L.VtcMat((1 << 20) + 64, 64)), "overlaps x"), (False, dict(act=4), "activation"), (True, dict(dx=1 << 20), "overlaps"),
                                  (True, dict(dx=5 << 20), "overlaps"), (True, dict(dx_row=63), "pitch"), (True, dict(dw=None), "go together"),
                                  (True, dict(m=0), "no rows"), (True, dict(dx=(7 << 20) + 1), "aligned")):
         rc, msg = _ffn_c(backward, **over)

@@ -4,11 +4,12 @@
 // Both projections, the activation and the product are one kernel: a tile holds the same columns of W_gate (first half) and W_up
 // (second half), so a lane's two accumulators are g and u of the same elements and only h leaves the chip (g and u as well when a
 // backward pass will want them).  Backward: dh never exists in memory (its tile turns into dg and du in the epilogue).
-// Rounding: h, and for the backward pass g, u, dg, du, are stored in the operands' 16-bit type, since they are operands of the
-// next matrix product; every sum is fp32 (fp64 where K-split partials and column sums are joined).
+// Rounding: h, dg and du are stored in the operands' 16-bit type, since they are operands of the next matrix product; what the
+// forward pass keeps for the backward one (s = u act'(g) and a = act(g), so that no activation is computed twice) has 24 bits;
+// every sum is fp32 (column sums are joined in fp64).
 //
 // Few rows (at most 64: single frames, live streams) are bound by reading the weights once, and by latency: skinny_kernel
-// below.  Everything else runs on op_gemm_kernel.
+// below.  Everything else runs on op_gemm_kernel or, where that would leave CUs idle, op_small_kernel.
 #pragma once
 #include "common.hip.h"
 #include "op_act.hip.h"
@@ -72,9 +73,9 @@ __global__ __launch_bounds__(256) void col_reduce_kernel(const ColReduceParams p
   else ((h16*)q.out)[c] = p.f16 ? to_h16<true>(v) : to_h16<false>(v);
 }
 
-// K-split partials -> 16-bit result; up to three matrices in one launch
-struct SplitReduce { const float* part; h16* out; long long ldo, pitch, rows; int cols, vec; };
-struct SplitReduceParams { SplitReduce r[3]; int n, splits; long long stride; };
+// K-split partials (+ bias) -> 16-bit result; up to three matrices in one launch
+struct SplitReduce { const float* part; h16* out; long long ldo, pitch, rows; int cols, vec; const void* bias; };
+struct SplitReduceParams { SplitReduce r[3]; int n, splits, bias_f32; long long stride; };
 template <bool F16>
 __global__ __launch_bounds__(256) void split_reduce_kernel(const SplitReduceParams p) {
   const SplitReduce& q = p.r[blockIdx.y];
@@ -88,6 +89,12 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const SplitReducePara
     for (int k = 1; k < p.splits; ++k) {
       const float4 t = *(const float4*)(src + k * p.stride);
       s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+    }
+    if (q.bias) {
+      s.x += op_bias(q.bias, c, p.bias_f32, F16);
+      if (c + 1 < q.cols) s.y += op_bias(q.bias, c + 1, p.bias_f32, F16);
+      if (c + 2 < q.cols) s.z += op_bias(q.bias, c + 2, p.bias_f32, F16);
+      if (c + 3 < q.cols) s.w += op_bias(q.bias, c + 3, p.bias_f32, F16);
     }
     h16* o = q.out + r * q.ldo + c;
     if (q.vec) {
@@ -108,8 +115,9 @@ struct SkinnyParams {
   long long ldx, ldw;
   int M, K, N, Nb;            // N: columns written (padding included), Nb: rows of w
   const void *b0, *b1;
-  int bias_f32, act, cvec;
-  h16 *out, *g, *u;
+  int bias_f32, act;
+  h16* out;
+  Saved24 s, a;               // GATE: kept for the backward pass (s.hi null: nothing is)
   long long ldo;
 };
 template <bool F16, int MT, bool GATE>
@@ -169,12 +177,20 @@ __global__ __launch_bounds__(512) void skinny_kernel(const SkinnyParams p) {
     if (col < p.Nb) v0 += op_bias(p.b0, col, p.bias_f32, F16);
     if constexpr (GATE) {
       if (col < p.Nb) v1 += op_bias(p.b1, col, p.bias_f32, F16);
-      if (p.g) { p.g[r * p.ldo + col] = to_h16<F16>(v0); p.u[r * p.ldo + col] = to_h16<F16>(v1); }
-      float a;
-      if (p.act == ACT_GELU) a = op_act<ACT_GELU, false>(v0);
-      else if (p.act == ACT_SILU) a = op_act<ACT_SILU, false>(v0);
-      else if (p.act == ACT_SIGMOID) a = op_act<ACT_SIGMOID, false>(v0);
-      else a = v0;
+      float a = v0, d = 1.f;
+      if (p.s.hi) {
+        if (p.act == ACT_GELU) op_act_grad<ACT_GELU, false>(v0, a, d);
+        else if (p.act == ACT_SILU) op_act_grad<ACT_SILU, false>(v0, a, d);
+        else if (p.act == ACT_SIGMOID) op_act_grad<ACT_SIGMOID, false>(v0, a, d);
+        const unsigned bs = __float_as_uint(v1 * d) + 0x80u, ba = __float_as_uint(a) + 0x80u;   // see OpTile::store24
+        const long long at = r * p.ldo + col;
+        p.s.hi[at] = (unsigned short)(bs >> 16); p.s.lo[at] = (unsigned char)(bs >> 8);
+        p.a.hi[at] = (unsigned short)(ba >> 16); p.a.lo[at] = (unsigned char)(ba >> 8);
+      } else {
+        if (p.act == ACT_GELU) a = op_act<ACT_GELU, false>(v0);
+        else if (p.act == ACT_SILU) a = op_act<ACT_SILU, false>(v0);
+        else if (p.act == ACT_SIGMOID) a = op_act<ACT_SIGMOID, false>(v0);
+      }
       v0 = a * v1;
     }
     p.out[r * p.ldo + col] = to_h16<F16>(v0);

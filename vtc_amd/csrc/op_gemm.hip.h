@@ -21,6 +21,11 @@ namespace vtc {
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
+// What the backward pass multiplies dh by, kept in 24 bits (the upper ones of fp32: 16 in one array, 8 in another).  Rounded to
+// the operands' type, dx and the weights' gradients would carry that rounding on top of dg's own and the result's
+// (bf16: 3.1e-3 of the norm instead of 2.4e-3, the result's own being 1.7e-3); a byte more per value removes it.
+struct Saved24 { unsigned short* hi; unsigned char* lo; };
+
 struct OpMat {
   const h16* p;
   long long ld;   // elements between rows of the stored matrix (a multiple of 8)
@@ -36,8 +41,10 @@ struct OpProb {
 };
 enum : int { OG_PLAIN = 0,   // 16-bit C (+ bias)
              OG_PART = 1,    // fp32 partial of a K split
-             OG_GATE = 2,    // b[0] = W_gate, b[1] = W_up: h = act(g) u, g and u stored when asked for
-             OG_DGATE = 3 }; // C = dh: dg = dh u act'(g), du = dh act(g), and their column sums
+             OG_GATE = 2,    // b[0] = W_gate, b[1] = W_up: h = act(g) u
+             OG_GATE_SAVE = 3,   // the same, and what the backward pass needs: s = u act'(g) and a = act(g)
+             OG_DGATE = 4 }; // C = dh: dg = dh s, du = dh a, and their column sums
+constexpr bool og_gate(int epi) { return epi == OG_GATE || epi == OG_GATE_SAVE; }
 struct OpGemmParams {
   OpProb prob[3];
   int nprob, ntiles;          // ntiles: tiles of all problems
@@ -46,10 +53,11 @@ struct OpGemmParams {
   long long split_stride;     // elements between partials
   const void *bias, *bias2;   // OG_PLAIN: bias; OG_GATE: b_gate, b_up (type: bias_f32 ? fp32 : the operands')
   int bias_f32, act;
-  h16 *g, *u;                 // OG_GATE: stored pre-activations (may be null); OG_DGATE: read
+  Saved24 s, a;               // OG_GATE_SAVE: written, OG_DGATE: read
   h16 *dg, *du;               // OG_DGATE
-  long long ldg;              // of g, u, dg, du (and h)
-  float* colsum;              // OG_DGATE: [2][2 tiles_m][N] sums of dg, du over the 128 rows of a wave row, or null
+  long long ldg;              // pitch of h, s, a, dg, du
+  float* colsum;              // OG_DGATE: [2][parts][ldg] sums of dg, du over the rows of a tile that one wave row holds (two parts per
+                              // 256-row tile, four per 128-row tile), or null
 };
 
 __device__ __forceinline__ float op_bias(const void* b, int i, int f32, bool f16) {
@@ -59,12 +67,176 @@ __device__ __forceinline__ float op_bias(const void* b, int i, int f32, bool f16
   return f16 ? from_h16<true>(v) : from_h16<false>(v);
 }
 
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+constexpr unsigned kOob = 0x80000000u;   // a buffer offset that is out of range of every descriptor used here
+
+// The output side of a tile: descriptors of [rows x cols left] windows, stores that drop what lies outside.
+template <bool F16> struct OpTile {
+  long long m0;
+  int n0, rows, cols, bcols;   // rows of the tile that exist; columns left from n0, and those of them that have a bias
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, long long ld, int es) const {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + (m0 * ld + n0) * es), 0, ((rows - 1) * (int)ld + cols) * es, 0x00020000);
+  }
+  __device__ __forceinline__ unsigned off(long long ld, int r, int c, int es) const {
+    return (r < rows && c < cols) ? (unsigned)((r * (int)ld + c) * es) : kOob;
+  }
+  // N (4 or 8) consecutive values: one store where rows start aligned, else one by one
+  template <int N> __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t rs, long long ld, int vec, int r, int c, const float* v) const {
+    if (vec) {
+      const unsigned o = off(ld, r, c, 2);
+      if constexpr (N == 8)
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]), pack2<F16>(v[4], v[5]), pack2<F16>(v[6], v[7])}, rs, o, 0, 0);
+      else
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3])}, rs, o, 0, 0);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) __builtin_amdgcn_raw_buffer_store_b16(to_h16<F16>(v[k]), rs, off(ld, r, c + k, 2), 0, 0);
+    }
+  }
+  template <int N> __device__ __forceinline__ void store32(__amdgpu_buffer_rsrc_t rs, long long ld, int r, int c, const float* v) const {
+#pragma unroll
+    for (int h = 0; h < N / 4; ++h)
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3])},
+                                             rs, off(ld, r, c + 4 * h, 4), 0, 0);
+  }
+  // 8 values in 24 bits (round half away; inf and NaN keep their upper bits)
+  __device__ __forceinline__ void store24(__amdgpu_buffer_rsrc_t hi, __amdgpu_buffer_rsrc_t lo, long long ld, int r, int c, const float* v) const {
+    unsigned b[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) b[k] = __float_as_uint(v[k]) + 0x80u;
+    u32x4 h;
+    u32x2 l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = (b[2 * k] >> 16) | (b[2 * k + 1] & 0xffff0000u);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      l[k] = (b[4 * k] >> 8 & 0xffu) | (b[4 * k + 1] & 0xff00u) | (b[4 * k + 2] << 8 & 0xff0000u) | (b[4 * k + 3] << 16 & 0xff000000u);
+    __builtin_amdgcn_raw_buffer_store_b128(h, hi, off(ld, r, c, 2), 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b64(l, lo, off(ld, r, c, 1), 0, 0);
+  }
+  static __device__ __forceinline__ float value24(const u32x4& h, const u32x2& l, int k) {
+    const unsigned top = k & 1 ? h[k >> 1] & 0xffff0000u : h[k >> 1] << 16;
+    return __uint_as_float(top | ((l[k >> 2] >> (8 * (k & 3)) & 0xffu) << 8));
+  }
+};
+// run(integral_constant<ACT>) for the run-time activation
+template <typename F> __device__ __forceinline__ void og_by_act(int act, F&& run) {
+  if (act == ACT_GELU) run(std::integral_constant<int, ACT_GELU>{});
+  else if (act == ACT_SILU) run(std::integral_constant<int, ACT_SILU>{});
+  else if (act == ACT_SIGMOID) run(std::integral_constant<int, ACT_SIGMOID>{});
+  else run(std::integral_constant<int, ACT_NONE>{});
+}
+// One row group of the gate / up epilogue: 8 columns of g and u (without bias) -> h, and s, a where they are kept
+template <bool F16, bool SAVE> struct OgGate {
+  const OpGemmParams& p;
+  const OpTile<F16>& t;
+  float bg[8], bu[8];
+  __amdgpu_buffer_rsrc_t rh, rsh, rsl, rah, ral;
+  __device__ __forceinline__ OgGate(const OpGemmParams& p_, const OpTile<F16>& t_, void* h, int c) : p(p_), t(t_) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      bg[k] = c + k < t.bcols ? op_bias(p.bias, t.n0 + c + k, p.bias_f32, F16) : 0.f;
+      bu[k] = c + k < t.bcols ? op_bias(p.bias2, t.n0 + c + k, p.bias_f32, F16) : 0.f;
+    }
+    rh = t.rsrc(h, p.ldg, 2);
+    if constexpr (SAVE) { rsh = t.rsrc(p.s.hi, p.ldg, 2); rsl = t.rsrc(p.s.lo, p.ldg, 1); rah = t.rsrc(p.a.hi, p.ldg, 2); ral = t.rsrc(p.a.lo, p.ldg, 1); }
+  }
+  template <int ACT> __device__ __forceinline__ void row(int r, int c, const float* g_, const float* u_) const {
+    float h[8], a[8], s[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float g = g_[k] + bg[k], u = u_[k] + bu[k];
+      if constexpr (SAVE) {
+        float d;
+        op_act_grad<ACT, false>(g, a[k], d);
+        s[k] = u * d;
+        h[k] = a[k] * u;
+      } else {
+        h[k] = op_act<ACT, false>(g) * u;
+      }
+    }
+    if constexpr (SAVE) { t.store24(rsh, rsl, p.ldg, r, c, s); t.store24(rah, ral, p.ldg, r, c, a); }
+    t.template store<8>(rh, p.ldg, 1, r, c, h);
+  }
+};
+// Gradient epilogue of 8 columns, G row groups at a time (row(g) is a group's row, dh(g, k) its value): dg, du and their column sums
+template <bool F16> struct OgDgate {
+  const OpGemmParams& p;
+  const OpTile<F16>& t;
+  __amdgpu_buffer_rsrc_t rsh, rsl, rah, ral, rdg, rdu;
+  float sg[8], su[8];
+  __device__ __forceinline__ OgDgate(const OpGemmParams& p_, const OpTile<F16>& t_) : p(p_), t(t_) {
+    rsh = t.rsrc(p.s.hi, p.ldg, 2); rsl = t.rsrc(p.s.lo, p.ldg, 1); rah = t.rsrc(p.a.hi, p.ldg, 2); ral = t.rsrc(p.a.lo, p.ldg, 1);
+    rdg = t.rsrc(p.dg, p.ldg, 2); rdu = t.rsrc(p.du, p.ldg, 2);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sg[k] = su[k] = 0.f;
+  }
+  template <int G, int N, typename R, typename D> __device__ __forceinline__ void groups(int c, R&& row, D&& dh) {
+    u32x4 sh[G], ah[G];
+    u32x2 sl[G], al[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const unsigned o2 = t.off(p.ldg, row(g), c, 2), o1 = o2 == kOob ? kOob : o2 >> 1;
+      if constexpr (N == 8) {
+        sh[g] = __builtin_amdgcn_raw_buffer_load_b128(rsh, o2, 0, 0);
+        ah[g] = __builtin_amdgcn_raw_buffer_load_b128(rah, o2, 0, 0);
+        sl[g] = __builtin_amdgcn_raw_buffer_load_b64(rsl, o1, 0, 0);
+        al[g] = __builtin_amdgcn_raw_buffer_load_b64(ral, o1, 0, 0);
+      } else {
+        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rsh, o2, 0, 0), y = __builtin_amdgcn_raw_buffer_load_b64(rah, o2, 0, 0);
+        sh[g] = u32x4{x[0], x[1], 0u, 0u};
+        ah[g] = u32x4{y[0], y[1], 0u, 0u};
+        sl[g] = u32x2{__builtin_amdgcn_raw_buffer_load_b32(rsl, o1, 0, 0), 0u};
+        al[g] = u32x2{__builtin_amdgcn_raw_buffer_load_b32(ral, o1, 0, 0), 0u};
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float dg[N], du[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float d = dh(g, k);
+        dg[k] = d * OpTile<F16>::value24(sh[g], sl[g], k);
+        du[k] = d * OpTile<F16>::value24(ah[g], al[g], k);
+        sg[k] += dg[k];
+        su[k] += du[k];
+      }
+      t.template store<N>(rdg, p.ldg, 1, row(g), c, dg);
+      t.template store<N>(rdu, p.ldg, 1, row(g), c, du);
+    }
+  }
+  // sums over the 16 rows that lanes hold, into row `part` of the partial sums (rows outside contributed 0: dh is 0 there)
+  template <int N> __device__ __forceinline__ void finish(int c, int fr, long long part, long long parts) {
+    if (!p.colsum) return;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) { sg[k] += __shfl_xor(sg[k], o); su[k] += __shfl_xor(su[k], o); }
+    }
+    if (fr == 0 && c < t.cols) {
+      float* dst = p.colsum + part * p.ldg + t.n0 + c;
+#pragma unroll
+      for (int k = 0; k < N; ++k) { dst[k] = sg[k]; dst[parts * p.ldg + k] = su[k]; }
+    }
+  }
+};
+
+// Two transposed LDS reads: 4 + 4 contraction indices of the lane's column.  The restrict parameters give the reads alias
+// information; without any, the compiler drains every copy to LDS in flight (vmcnt(0)) in front of each of them.
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+__device__ __forceinline__ u16x8 tr_frag(const lds_s16x4* __restrict__ a, const lds_s16x4* __restrict__ b) {
+  const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a);
+  const s16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)b);
+  return __builtin_bit_cast(u16x8, __builtin_shufflevector(v1, v2, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 template <bool F16, bool AKS, bool BKS, int EPI, int BN>
 __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
   using TC = Tile256<BN>;
   constexpr int NJ1 = TC::NJ1;
-  static_assert(!BKS || BN == 256, "a KS operand B is staged in halves of 128 columns");
-  static_assert(EPI != OG_GATE || BN == 256, "gate and up columns sit in the two halves of a tile");
+  static_assert(!og_gate(EPI) || BN == 256, "gate and up columns sit in the two halves of a tile");
   __shared__ __attribute__((aligned(16))) char smem[TC::SMEM];
 
   const int tid = threadIdx.x;
@@ -72,17 +244,21 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
   const int fr = lane & 15, fq = lane >> 4;
-  constexpr unsigned OOB = 0x80000000u;
-
-  // ---- staging: lane offsets (bytes from the half-tile's origin) and the scalar description of the tile being staged
+  // ---- staging.  Lane offsets are bytes from a half-tile's origin and the same for every tile; what changes per tile and K-tile is
+  // scalar: the origin, the bytes that exist behind it and the contraction that is left.
   const int lr = lane >> 3, lc = lane & 7;
-  unsigned va[2], vb[2], vb1[NJ1];   // offsets of the two instructions of a half-tile (B1: NJ1)
-  int kca[2], kcb[2], kcb1[NJ1];     // KC operands: first k of the lane's piece inside the K-tile
-  struct Src { const char *a, *b0, *b1; int am, bn0, bn1; long long lda, ldb, ldb1; int K; };   // am / bn: rows or columns left in the half
+  unsigned va[2], vb[2], vb1[1];     // of the two instructions of a half-tile (vb1: B1's one instruction where BN = 192)
+  int pca[2], pcb[2], pcb1[1];       // what a lane's 16-byte piece has to stay below: KC: k inside the K-tile, KS: column
   constexpr int NSEG = (EPI == OG_PLAIN && BKS) ? 2 : 1;   // dx sums over two operand pairs
   constexpr bool MULTI = AKS;                              // several problems in one launch: the weights' gradients
-  Src src[NSEG];
-  int kt_base = 0, nk_cur = 0;       // first K-tile of the tile being staged
+  struct Stream {
+    const char* p;    // origin of the next K-tile's half
+    int size, left;   // KC: bytes of all rows but the last (negative: no rows), k left (in pieces).  KS: last row's bytes less a
+                      // pitch, k-rows left
+    int seg;
+  };
+  Stream sa0, sa1, sb0, sb1;
+  int lda2 = 0, ldb2 = 0, am = 0, bn0 = 0, bn1 = 0;   // pitches in bytes; rows or columns left in the tile from the half's first
 
   auto unit = [&](unsigned t, int& pi, int& tm, int& tn, int& k0, int& k1) {   // work unit -> problem, tile, K-tiles
     const unsigned ti = t / (unsigned)p.splits;
@@ -100,108 +276,99 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
     k0 = s * p.kps;
     k1 = min(p.nk, k0 + p.kps);
   };
-
-  auto set_sources = [&](int pi, int tm, int tn) {
-    const OpProb& q = p.prob[pi];
-    const int m0 = tm * 256;
-    const int n0 = EPI == OG_GATE ? tn * 128 : tn * BN;
-    const int n1 = EPI == OG_GATE ? n0 : n0 + 128;
-#pragma unroll
-    for (int s = 0; s < NSEG; ++s) {
-      Src& d = src[s];
-      const OpMat A = q.a[s], B = EPI == OG_GATE ? q.b[0] : q.b[s], B1 = EPI == OG_GATE ? q.b[1] : q.b[s];
-      d.K = p.K[s];
-      d.lda = A.ld; d.ldb = B.ld; d.ldb1 = B1.ld;
-      d.am = q.M - m0; d.bn0 = q.Nb - n0; d.bn1 = q.Nb - n1;
-      d.a = (const char*)A.p + (AKS ? (long long)m0 * 2 : (long long)m0 * A.ld * 2);
-      d.b0 = (const char*)B.p + (BKS ? (long long)n0 * 2 : (long long)n0 * B.ld * 2);
-      d.b1 = (const char*)B1.p + (BKS ? (long long)n1 * 2 : (long long)n1 * B1.ld * 2);
-    }
+  auto half_kc = [&](Stream& d, const h16* base, long long ld, int row0, int rows, int k0, int K) {   // rows: left from row0
+    d.p = (const char*)(base + (long long)row0 * ld + k0);
+    d.size = rows > 0 ? (min(rows, 128) - 1) * (int)ld * 2 : -(1 << 30);
+    d.left = ((K + 7) & ~7) - k0;
   };
-  // lane offsets do not depend on the tile (both segments of a product have the same pitch per side)
-  {
-    const OpProb& q = p.prob[0];
+  auto half_ks = [&](Stream& d, const h16* base, long long ld, int col0, int cols, int k0, int K) {   // cols: left from col0
+    d.p = (const char*)(base + (long long)k0 * ld + col0);
+    d.size = ((min(cols, 128) + 7) & ~7) * 2 - (int)ld * 2;
+    d.left = K - k0;
+  };
+  int cur_tm = 0, cur_tn = 0;   // tile being staged
+  // operand A (half h) / B (half h) of segment s from contraction index k0 on
+  auto set_a = [&](Stream& d, const OpProb& q, int h, int s, int k0) {
+    const int r0 = cur_tm * 256 + h * 128;
+    if constexpr (AKS) half_ks(d, q.a[s].p, q.a[s].ld, r0, q.M - r0, k0, p.K[s]);
+    else half_kc(d, q.a[s].p, q.a[s].ld, r0, q.M - r0, k0, p.K[s]);
+    d.seg = s;
+  };
+  auto set_b = [&](Stream& d, const OpProb& q, int h, int s, int k0) {
+    const OpMat B = og_gate(EPI) ? q.b[h] : q.b[s];
+    const int c0 = og_gate(EPI) ? cur_tn * 128 : cur_tn * BN + h * 128;
+    if constexpr (BKS) half_ks(d, B.p, B.ld, c0, q.Nb - c0, k0, p.K[s]);
+    else half_kc(d, B.p, B.ld, c0, q.Nb - c0, k0, p.K[s]);
+    d.seg = s;
+  };
+  auto lane_offsets = [&](int pi) {
+    const OpProb& q = p.prob[MULTI ? pi : 0];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = (wave * 2 + i) * 8 + lr;                 // KC: row of the half-tile, piece lc holds chunk lc ^ swz(r)
+      const int r = (wave * 2 + i) * 8 + lr;                 // KC: row of the half-tile, place lc holds piece lc ^ swz(r)
       const int ch = lc ^ lds_swz(r);
       const int kr = (wave * 2 + i) * 4 + (lane >> 4);       // KS: k-row of the half-tile
       const int sw = (kr & 3) | ((kr >> 3 & 1) << 2);
-      const int cc = ((((lane & 15) >> 1) ^ sw) << 1) | (lane & 1);   // 16-byte column piece
-      kca[i] = AKS ? cc * 8 : ch * 8;
+      const int cc = ((((lane & 15) >> 1) ^ sw) << 1) | (lane & 1);
+      pca[i] = AKS ? cc * 8 : ch * 8;
       va[i] = AKS ? (unsigned)(kr * (int)q.a[0].ld * 2 + cc * 16) : (unsigned)(r * (int)q.a[0].ld * 2 + ch * 16);
       const int wr = (r & ~31) + perm32(r & 31);
-      kcb[i] = BKS ? cc * 8 : ch * 8;
+      pcb[i] = BKS ? cc * 8 : ch * 8;
       vb[i] = BKS ? (unsigned)(kr * (int)q.b[0].ld * 2 + cc * 16) : (unsigned)(wr * (int)q.b[0].ld * 2 + ch * 16);
     }
-#pragma unroll
-    for (int i = 0; i < NJ1; ++i) {
-      const int r = (wave * NJ1 + i) * 8 + lr;
-      const int ch = lc ^ lds_swz(r);
-      const int wr = NJ1 == 2 ? (r & ~31) + perm32(r & 31) : r;
-      kcb1[i] = BKS ? kcb[i] : ch * 8;
-      vb1[i] = BKS ? vb[i] : (unsigned)(wr * (int)q.b[0].ld * 2 + ch * 16);
+    if constexpr (NJ1 == 1) {                                // B1 of 64 columns: 16-column groups need no permutation
+      const int r = wave * 8 + lr, ch = lc ^ lds_swz(r);
+      const int sw = (r >> 1 & 1) | ((r >> 3 & 1) << 1);     // KS: k-rows of 128 bytes, four 32-byte pieces
+      const int cc = (((lc >> 1) ^ sw) << 1) | (lc & 1);
+      pcb1[0] = (BKS ? cc : ch) * 8;
+      vb1[0] = (unsigned)(r * (int)q.b[0].ld * 2 + (BKS ? cc : ch) * 16);
     }
-  }
-  // (several problems of one launch may have different pitches: recomputed at a switch, see `repitch`)
-  auto repitch = [&](int pi) {
-    const OpProb& q = p.prob[pi];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int kr = (wave * 2 + i) * 4 + (lane >> 4);
-      if constexpr (AKS) va[i] = (unsigned)(kr * (int)q.a[0].ld * 2 + kca[i] * 2);
-      if constexpr (BKS) { vb[i] = (unsigned)(kr * (int)q.b[0].ld * 2 + kcb[i] * 2); vb1[i] = vb[i]; }
-    }
+  };
+  lane_offsets(0);
+  auto set_tile = [&](int pi, int tm, int tn, int k0) {   // (only products of one segment are split)
+    const OpProb& q = p.prob[MULTI ? pi : 0];
+    cur_tm = tm; cur_tn = tn;
+    lda2 = (int)q.a[0].ld * 2; ldb2 = (int)q.b[0].ld * 2;
+    am = q.M - tm * 256;
+    bn0 = q.Nb - (og_gate(EPI) ? tn * 128 : tn * BN);
+    bn1 = og_gate(EPI) ? bn0 : bn0 - 128;
+    set_a(sa0, q, 0, 0, k0 * 64); set_a(sa1, q, 1, 0, k0 * 64);
+    set_b(sb0, q, 0, 0, k0 * 64); set_b(sb1, q, 1, 0, k0 * 64);
+    if constexpr (MULTI) lane_offsets(pi);
   };
 
-  // one 16-byte-per-lane copy to LDS.  KC: rows beyond the matrix lie behind num_records, k beyond K is masked per lane.
-  // KS: k-rows beyond K lie behind num_records, columns beyond the matrix are masked per lane.
-  auto fetch = [&](bool ks, const char* base, long long ld, int left, int K, int kt, unsigned vo, int piece, char* lds) {
-    int rows, cols, lim;
-    const char* b;
-    if (ks) {
-      rows = min(64, K - kt * 64);
-      cols = min(left, 128);
-      b = base + (long long)kt * 64 * ld * 2;
-      lim = left;
-    } else {
-      rows = min(left, 128);
-      cols = K - kt * 64;          // > 0 wherever the piece is not masked
-      b = base + (long long)kt * 128;
-      lim = K - kt * 64;
-    }
-    const int n = (rows > 0 && cols > 0) ? (int)(((long long)(rows - 1) * ld + ((cols + 7) & ~7)) * 2) : 0;   // rows are padded to 16 bytes
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, n, 0x00020000);
-    const unsigned off = piece < lim ? vo : OOB;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LPTR(lds), 16, (int)off, 0, 0, 0);
+  // one 16-byte-per-lane copy to LDS.  KC: rows beyond the matrix lie behind the descriptor's end, k beyond K is masked per lane.
+  // KS: k-rows beyond K lie behind its end, columns beyond the matrix are masked per lane.  Both arrive as zeros.
+  auto rsrc_kc = [&](const Stream& d) { return __builtin_amdgcn_make_buffer_rsrc((void*)d.p, 0, max(d.size + d.left * 2, 0), 0x00020000); };
+  auto rsrc_ks = [&](const Stream& d, int ld2) { return __builtin_amdgcn_make_buffer_rsrc((void*)d.p, 0, max(min(d.left, 64) * ld2 + d.size, 0), 0x00020000); };
+  auto copy16 = [&](__amdgpu_buffer_rsrc_t rs, unsigned vo, int piece, int lim, char* lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LPTR(lds), 16, (int)(piece < lim ? vo : kOob), 0, 0, 0);
   };
-  auto seg = [&](int& kt) -> const Src& {   // K-tile of the tile -> segment and K-tile inside it
-    if constexpr (NSEG == 2) {
-      if (kt >= p.nk0) { kt -= p.nk0; return src[1]; }
-    }
-    return src[0];
-  };
-  auto issue_a = [&](int h, int buf, int kt_) {
-    int kt = kt_ + kt_base;
-    const Src& s = seg(kt);
-    char* d = smem + buf * TC::BUF + (h ? TC::OFF_A1 : TC::OFF_A0) + wave * 2048;
-    const char* base = s.a + (h ? (AKS ? 256ll : 128 * s.lda * 2) : 0ll);
+  auto step = [&](Stream& d, bool ks, int ld2) { d.p += ks ? (long long)64 * ld2 : 128ll; d.left -= 64; };
+  auto issue_a = [&](int h, int buf, int) {
+    Stream& d = h ? sa1 : sa0;
+    if constexpr (NSEG == 2) { if (d.left <= 0 && d.seg == 0) set_a(d, p.prob[0], h, 1, 0); }
+    char* l = smem + buf * TC::BUF + (h ? TC::OFF_A1 : TC::OFF_A0) + wave * 2048;
+    const __amdgpu_buffer_rsrc_t rs = AKS ? rsrc_ks(d, lda2) : rsrc_kc(d);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) fetch(AKS, base, s.lda, s.am - h * 128, s.K, kt, va[i], kca[i], d + i * 1024);
+    for (int i = 0; i < 2; ++i) copy16(rs, va[i], pca[i], AKS ? am - h * 128 : d.left, l + i * 1024);
+    step(d, AKS, lda2);
   };
-  auto issue_b0 = [&](int buf, int kt_) {
-    int kt = kt_ + kt_base;
-    const Src& s = seg(kt);
-    char* d = smem + buf * TC::BUF + TC::OFF_B0 + wave * 2048;
+  auto issue_b0 = [&](int buf, int) {
+    if constexpr (NSEG == 2) { if (sb0.left <= 0 && sb0.seg == 0) set_b(sb0, p.prob[0], 0, 1, 0); }
+    char* l = smem + buf * TC::BUF + TC::OFF_B0 + wave * 2048;
+    const __amdgpu_buffer_rsrc_t rs = BKS ? rsrc_ks(sb0, ldb2) : rsrc_kc(sb0);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) fetch(BKS, s.b0, s.ldb, s.bn0, s.K, kt, vb[i], kcb[i], d + i * 1024);
+    for (int i = 0; i < 2; ++i) copy16(rs, vb[i], pcb[i], BKS ? bn0 : sb0.left, l + i * 1024);
+    step(sb0, BKS, ldb2);
   };
-  auto issue_b1 = [&](int buf, int kt_) {
-    int kt = kt_ + kt_base;
-    const Src& s = seg(kt);
-    char* d = smem + buf * TC::BUF + TC::OFF_B1 + wave * (NJ1 * 1024);
+  auto issue_b1 = [&](int buf, int) {
+    if constexpr (NSEG == 2) { if (sb1.left <= 0 && sb1.seg == 0) set_b(sb1, p.prob[0], 1, 1, 0); }
+    char* l = smem + buf * TC::BUF + TC::OFF_B1 + wave * (NJ1 * 1024);
+    const __amdgpu_buffer_rsrc_t rs = BKS ? rsrc_ks(sb1, ldb2) : rsrc_kc(sb1);
 #pragma unroll
-    for (int i = 0; i < NJ1; ++i) fetch(BKS, s.b1, s.ldb1, s.bn1, s.K, kt, vb1[i], kcb1[i], d + i * 1024);
+    for (int i = 0; i < NJ1; ++i) copy16(rs, NJ1 == 2 ? vb[i] : vb1[0], NJ1 == 2 ? pcb[i] : pcb1[0], BKS ? bn1 : sb1.left, l + i * 1024);
+    step(sb1, BKS, ldb2);
   };
 
   // ---- fragments
@@ -223,16 +390,12 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
 #pragma unroll
   for (int j = 0; j < NJ1; ++j) {
     const int r = wn * (16 * NJ1) + j * 16 + fr;
-    if constexpr (BKS) { b1_off[j] = b0_off[j]; b1_sw[j] = 0; }
+    if constexpr (BKS && NJ1 == 2) { b1_off[j] = b0_off[j]; b1_sw[j] = 0; }
+    else if constexpr (BKS) { b1_off[j] = (fq * 8 + tq) * 128 + ((wn ^ ((tq >> 1) | ((fq & 1) << 1))) << 5) + 8 * tp; b1_sw[j] = 0; }
     else { b1_off[j] = r * 128; b1_sw[j] = lds_swz(r); }
   }
   auto frag_kc = [&](const char* base, int off, int sw, int ks) { return *(const u16x8*)(base + off + (((ks * 4 + fq) ^ sw) << 4)); };
-  auto frag_ks = [&](const char* base, int off, int ks) {
-    const char* a = base + off + ks * 8192;
-    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
-    const s16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 1024));
-    return __builtin_bit_cast(u16x8, __builtin_shufflevector(v1, v2, 0, 1, 2, 3, 4, 5, 6, 7));
-  };
+  auto frag_ks = [&](const char* base, int off, int ks) { return tr_frag((const lds_s16x4*)(base + off + ks * 8192), (const lds_s16x4*)(base + off + ks * 8192 + 1024)); };
 
   f32x4 acc0[2][4][2], acc1[2][4][NJ1];
   u16x8 fa[2][4], fb0[2][2], fb1[2][NJ1];
@@ -255,7 +418,11 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int j = 0; j < NJ1; ++j) { if constexpr (BKS) fb1[ks][j] = frag_ks(base, b1_off[j], ks); else fb1[ks][j] = frag_kc(base, b1_off[j], b1_sw[j], ks); }
+      for (int j = 0; j < NJ1; ++j) {
+        if constexpr (BKS && NJ1 == 2) fb1[ks][j] = frag_ks(base, b1_off[j], ks);
+        else if constexpr (BKS) fb1[ks][j] = tr_frag((const lds_s16x4*)(base + b1_off[j] + ks * 4096), (const lds_s16x4*)(base + b1_off[j] + ks * 4096 + 512));
+        else fb1[ks][j] = frag_kc(base, b1_off[j], b1_sw[j], ks);
+      }
   };
   auto mma0 = [&](int mq) {
     __builtin_amdgcn_s_setprio(1);
@@ -327,9 +494,7 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
   {
     int pi, tm, tn, k0, k1;
     unit(xcd_remap(tl, nunits), pi, tm, tn, k0, k1);
-    set_sources(pi, tm, tn);
-    if constexpr (MULTI) repitch(pi);
-    kt_base = k0;
+    set_tile(pi, tm, tn, k0);
     issue_a(0, 0, 0); issue_b0(0, 0); issue_b1(0, 0); issue_a(1, 0, 0);
     issue_a(0, 1, 1); issue_b0(1, 1);
   }
@@ -338,7 +503,7 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
     int pi, tile_m, tile_n, k0, k1;
     const unsigned ucur = xcd_remap(tl, nunits);
     unit(ucur, pi, tile_m, tile_n, k0, k1);
-    nk_cur = k1 - k0;
+    const int nk_cur = k1 - k0;
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -363,47 +528,28 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
     VTC_OG_KTILE(0, true, nk_cur - 1, has_next, 0, if (has_next) {
       int pn; int tmn; int tnn; int kn; int kn1;
       unit(xcd_remap(tl_next, nunits), pn, tmn, tnn, kn, kn1);
-      set_sources(pn, tmn, tnn);
-      if constexpr (MULTI) repitch(pn);
-      kt_base = kn;
+      set_tile(pn, tmn, tnn, kn);
     })
     VTC_OG_KTILE(1, has_next, 0, has_next, 1, )
     if (wm == 0) __builtin_amdgcn_s_barrier();
     tl = tl_next;
 
     // ---- epilogue.  Global accesses through descriptors of the tile: rows outside are dropped by the hardware, columns per lane.
-    const OpProb& q = p.prob[pi];
-    const int rows = min(256, q.M - tile_m * 256);
-    const int n0 = EPI == OG_GATE ? tile_n * 128 : tile_n * BN;
-    const int cols = q.N - n0, bcols = q.Nb - n0;                // columns left from the tile's first; those that have a bias
+    // The lane id comes from an opaque source: what is derived from it must not be kept in registers across the K loop.
+    int el;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(el));
+    const int fr = el & 15, fq = el >> 4;
+    const OpProb& q = p.prob[MULTI ? pi : 0];
+    OpTile<F16> t;
+    t.m0 = (long long)tile_m * 256;
+    t.n0 = og_gate(EPI) ? tile_n * 128 : tile_n * BN;
+    t.rows = min(256, q.M - tile_m * 256);
+    t.cols = q.N - t.n0;
+    t.bcols = q.Nb - t.n0;
     constexpr int W1 = 4 * NJ1;
     const int c0 = wn * 32 + 8 * fq;                             // columns of the tile: B0 group, B1 group
-    const int c1 = EPI == OG_GATE ? c0 : 128 + wn * (16 * NJ1) + W1 * fq;
-    auto tile_rsrc = [&](const void* base, long long ld, int es) {
-      const char* b = (const char*)base + ((long long)tile_m * 256 * ld + n0) * es;
-      return __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, (int)(((long long)(rows - 1) * ld + cols) * es), 0x00020000);
-    };
+    const int c1 = og_gate(EPI) ? c0 : 128 + wn * (16 * NJ1) + W1 * fq;
     auto row_of = [&](int g) { return (g >> 2) * 128 + wm * 64 + (g & 3) * 16 + fr; };
-    // N consecutive values of row r from column c: one store where rows start aligned, else one by one
-    auto store16 = [&](__amdgpu_buffer_rsrc_t rs, long long ld, int vec, int r, int c, const float* v, auto count) {
-      constexpr int N = decltype(count)::value;
-      const unsigned off = (unsigned)((r * (int)ld + c) * 2);
-      if (vec) {
-        const unsigned o = (r < rows && c < cols) ? off : OOB;
-        if constexpr (N == 8)
-          __builtin_amdgcn_raw_buffer_store_b128(u32x4{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]), pack2<F16>(v[4], v[5]), pack2<F16>(v[6], v[7])}, rs, o, 0, 0);
-        else {
-          typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-          __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3])}, rs, o, 0, 0);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-          __builtin_amdgcn_raw_buffer_store_b16(to_h16<F16>(v[k]), rs, (r < rows && c + k < cols) ? off + 2 * k : OOB, 0, 0);
-      }
-    };
-    using I8 = std::integral_constant<int, 8>;
-    using IW1 = std::integral_constant<int, W1>;
     float v0[8], v1[W1];
     auto take = [&](int g) {
       const int mq = g >> 2, i = g & 3;
@@ -419,10 +565,10 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
     if constexpr (EPI == OG_PLAIN) {
       float b0[8], b1[W1];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) b0[k] = c0 + k < bcols ? op_bias(p.bias, n0 + c0 + k, p.bias_f32, F16) : 0.f;
+      for (int k = 0; k < 8; ++k) b0[k] = c0 + k < t.bcols ? op_bias(p.bias, t.n0 + c0 + k, p.bias_f32, F16) : 0.f;
 #pragma unroll
-      for (int k = 0; k < W1; ++k) b1[k] = c1 + k < bcols ? op_bias(p.bias, n0 + c1 + k, p.bias_f32, F16) : 0.f;
-      const __amdgpu_buffer_rsrc_t rc = tile_rsrc(q.c, q.ldc, 2);
+      for (int k = 0; k < W1; ++k) b1[k] = c1 + k < t.bcols ? op_bias(p.bias, t.n0 + c1 + k, p.bias_f32, F16) : 0.f;
+      const __amdgpu_buffer_rsrc_t rc = t.rsrc(q.c, q.ldc, 2);
 #pragma unroll
       for (int g = 0; g < 8; ++g) {
         take(g);
@@ -430,125 +576,246 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
         for (int k = 0; k < 8; ++k) v0[k] += b0[k];
 #pragma unroll
         for (int k = 0; k < W1; ++k) v1[k] += b1[k];
-        store16(rc, q.ldc, q.cvec, row_of(g), c0, v0, I8{});
-        store16(rc, q.ldc, q.cvec, row_of(g), c1, v1, IW1{});
+        t.template store<8>(rc, q.ldc, q.cvec, row_of(g), c0, v0);
+        t.template store<W1>(rc, q.ldc, q.cvec, row_of(g), c1, v1);
       }
     } else if constexpr (EPI == OG_PART) {
-      // partial s of the problem: [M][N] fp32 with the pitch ldc (a multiple of 8)
-      const int s = (int)(ucur % (unsigned)p.splits);
-      const __amdgpu_buffer_rsrc_t rc = tile_rsrc((const float*)q.c + s * p.split_stride, q.ldc, 4);
+      // partial of this split: [M][N] fp32 with the pitch ldc (a multiple of 8)
+      const __amdgpu_buffer_rsrc_t rc = t.rsrc((const float*)q.c + (long long)(ucur % (unsigned)p.splits) * p.split_stride, q.ldc, 4);
 #pragma unroll
       for (int g = 0; g < 8; ++g) {
         take(g);
-        const int r = row_of(g);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(v0[4 * h]), __float_as_uint(v0[4 * h + 1]), __float_as_uint(v0[4 * h + 2]), __float_as_uint(v0[4 * h + 3])},
-                                                 rc, (r < rows && c0 + 4 * h < cols) ? (unsigned)((r * (int)q.ldc + c0 + 4 * h) * 4) : OOB, 0, 0);
-#pragma unroll
-        for (int h = 0; h < NJ1; ++h)
-          __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(v1[4 * h]), __float_as_uint(v1[4 * h + 1]), __float_as_uint(v1[4 * h + 2]), __float_as_uint(v1[4 * h + 3])},
-                                                 rc, (r < rows && c1 + 4 * h < cols) ? (unsigned)((r * (int)q.ldc + c1 + 4 * h) * 4) : OOB, 0, 0);
+        t.template store32<8>(rc, q.ldc, row_of(g), c0, v0);
+        t.template store32<W1>(rc, q.ldc, row_of(g), c1, v1);
       }
-    } else if constexpr (EPI == OG_GATE) {
+    } else if constexpr (og_gate(EPI)) {
       if constexpr (NJ1 == 2) {
-        float bg[8], bu[8];
+        const OgGate<F16, EPI == OG_GATE_SAVE> gate(p, t, q.c, c0);
+        og_by_act(p.act, [&](auto act) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          bg[k] = c0 + k < bcols ? op_bias(p.bias, n0 + c0 + k, p.bias_f32, F16) : 0.f;
-          bu[k] = c0 + k < bcols ? op_bias(p.bias2, n0 + c0 + k, p.bias_f32, F16) : 0.f;
-        }
-        const __amdgpu_buffer_rsrc_t rh = tile_rsrc(q.c, p.ldg, 2);
-        auto run = [&](auto act) {
-          constexpr int ACT = decltype(act)::value;
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            take(g);
-            float h[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              v0[k] += bg[k];
-              v1[k] += bu[k];
-              h[k] = op_act<ACT, false>(v0[k]) * v1[k];
-            }
-            if (p.g) {
-              store16(tile_rsrc(p.g, p.ldg, 2), p.ldg, 1, row_of(g), c0, v0, I8{});
-              store16(tile_rsrc(p.u, p.ldg, 2), p.ldg, 1, row_of(g), c0, v1, I8{});
-            }
-            store16(rh, p.ldg, 1, row_of(g), c0, h, I8{});
-          }
-        };
-        if (p.act == ACT_GELU) run(std::integral_constant<int, ACT_GELU>{});
-        else if (p.act == ACT_SILU) run(std::integral_constant<int, ACT_SILU>{});
-        else if (p.act == ACT_SIGMOID) run(std::integral_constant<int, ACT_SIGMOID>{});
-        else run(std::integral_constant<int, ACT_NONE>{});
+          for (int g = 0; g < 8; ++g) { take(g); gate.template row<decltype(act)::value>(row_of(g), c0, v0, v1); }
+        });
       }
     } else {   // OG_DGATE
-      if constexpr (NJ1 == 2) {
-        const __amdgpu_buffer_rsrc_t rg = tile_rsrc(p.g, p.ldg, 2), ru = tile_rsrc(p.u, p.ldg, 2), rdg = tile_rsrc(p.dg, p.ldg, 2),
-                                     rdu = tile_rsrc(p.du, p.ldg, 2);
-        auto run = [&](auto act) {
-          constexpr int ACT = decltype(act)::value;
+      OgDgate<F16> grad(p, t);
+      auto half = [&](auto which, auto width) {
+        constexpr bool SECOND = decltype(which)::value;
+        constexpr int N = decltype(width)::value;
+        grad.clear();
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int c = half ? c1 : c0;
-            float sg[8], su[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) sg[k] = su[k] = 0.f;
-#pragma unroll
-            for (int g0 = 0; g0 < 8; g0 += 4) {
-              __builtin_amdgcn_sched_barrier(0);   // the loads of four row groups at a time: all sixteen would not fit the registers
-              u32x4 xg[4], xu[4];
-#pragma unroll
-              for (int gg = 0; gg < 4; ++gg) {
-                const int r = row_of(g0 + gg);
-                const unsigned off = (r < rows && c < cols) ? (unsigned)((r * (int)p.ldg + c) * 2) : OOB;
-                xg[gg] = __builtin_amdgcn_raw_buffer_load_b128(rg, off, 0, 0);
-                xu[gg] = __builtin_amdgcn_raw_buffer_load_b128(ru, off, 0, 0);
-              }
-#pragma unroll
-              for (int gg = 0; gg < 4; ++gg) {
-                const int mq = g0 >> 2, i = gg, r = row_of(g0 + gg);
-                float dg[8], du[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  const float dh = half ? acc1[mq][i][k >> 2][k & 3] : acc0[mq][i][k >> 2][k & 3];
-                  const float gv = from_h16<F16>((h16)(k & 1 ? xg[gg][k >> 1] >> 16 : xg[gg][k >> 1] & 0xffffu));
-                  const float uv = from_h16<F16>((h16)(k & 1 ? xu[gg][k >> 1] >> 16 : xu[gg][k >> 1] & 0xffffu));
-                  float a, d;
-                  op_act_grad<ACT, false>(gv, a, d);
-                  dg[k] = dh * uv * d;
-                  du[k] = dh * a;
-                  sg[k] += dg[k];
-                  su[k] += du[k];
-                }
-                store16(rdg, p.ldg, 1, r, c, dg, I8{});
-                store16(rdu, p.ldg, 1, r, c, du, I8{});
-              }
-            }
-            if (p.colsum) {   // rows outside contributed 0: dh is 0 there
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-#pragma unroll
-                for (int o = 1; o < 16; o <<= 1) { sg[k] += __shfl_xor(sg[k], o); su[k] += __shfl_xor(su[k], o); }
-              }
-              if (fr == 0 && c < cols) {
-                float* dst = p.colsum + (long long)(tile_m * 2 + wm) * p.ldg + n0 + c;
-                const long long second = (long long)q.tiles_m * 2 * p.ldg;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) { dst[k] = sg[k]; dst[second + k] = su[k]; }
-              }
-            }
-          }
-        };
-        if (p.act == ACT_GELU) run(std::integral_constant<int, ACT_GELU>{});
-        else if (p.act == ACT_SILU) run(std::integral_constant<int, ACT_SILU>{});
-        else if (p.act == ACT_SIGMOID) run(std::integral_constant<int, ACT_SIGMOID>{});
-        else run(std::integral_constant<int, ACT_NONE>{});
-      }
+        for (int g0 = 0; g0 < 8; g0 += 4) {
+          __builtin_amdgcn_sched_barrier(0);   // the loads of four row groups at a time: all of them would not fit the registers
+          grad.template groups<4, N>(SECOND ? c1 : c0, [&](int g) { return row_of(g0 + g); }, [&](int g, int k) {
+            if constexpr (SECOND) return acc1[(g0 + g) >> 2][(g0 + g) & 3][k >> 2][k & 3];
+            else return acc0[(g0 + g) >> 2][(g0 + g) & 3][k >> 2][k & 3];
+          });
+        }
+        grad.template finish<N>(SECOND ? c1 : c0, fr, tile_m * 2 + wm, q.tiles_m * 2ll);
+      };
+      half(std::false_type{}, std::integral_constant<int, 8>{});
+      half(std::true_type{}, std::integral_constant<int, W1>{});
     }
   }
 #undef VTC_OG_KTILE
+}
+
+// ---- small products: 128 x 64 tiles, 4 waves of 32 x 64, one tile per block, two blocks per CU.  A product with few 256-wide tiles
+// leaves most CUs idle there; with an eighth of the tile (and K splits) the same work spreads over all of them.  Three K-tile
+// buffers (A 16 KB, B 8 KB each), two in flight, one barrier per K-tile.  The contraction runs in the same order as in the kernel
+// above, so an unsplit product has the same bits in either.
+constexpr int kOsA = 16384, kOsStage = 24576;
+template <bool F16, bool AKS, bool BKS, int EPI>
+__global__ __launch_bounds__(256, 2) void op_small_kernel(const OpGemmParams p) {
+  __shared__ __attribute__((aligned(16))) char smem[3 * kOsStage];
+  constexpr bool MULTI = AKS;
+  constexpr int NSEG = (EPI == OG_PLAIN || EPI == OG_PART) && BKS && !AKS ? 2 : 1;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int fr = lane & 15, fq = lane >> 4, lr = lane >> 3, lc = lane & 7;
+  const unsigned u = xcd_remap(blockIdx.x, gridDim.x);
+  const unsigned ti = u / (unsigned)p.splits;
+  const int split = (int)(u - ti * (unsigned)p.splits);
+  int pi = 0;
+  if constexpr (MULTI) {
+    if (p.nprob > 1 && (int)ti >= p.prob[1].tile0) pi = 1;
+    if (p.nprob > 2 && (int)ti >= p.prob[2].tile0) pi = 2;
+  }
+  const OpProb& q = p.prob[pi];
+  const int tile_m = (int)((ti - (unsigned)q.tile0) / (unsigned)q.tiles_n), tile_n = (int)((ti - (unsigned)q.tile0) % (unsigned)q.tiles_n);
+  const int m0 = tile_m * 128, n0 = og_gate(EPI) ? tile_n * 32 : tile_n * 64;
+  const int k0 = split * p.kps, nk = min(p.nk, k0 + p.kps) - k0;
+
+  // ---- staging (see op_gemm_kernel): wave w fetches A pieces 4 w .. + 4 and B pieces 2 w, 2 w + 1 of 1 KiB; with gate and up
+  // columns side by side, waves 0 and 1 fetch W_gate rows, 2 and 3 W_up's
+  unsigned va[4], vb[2];
+  int pca[4], pcb[2];
+  const int lda2 = (int)q.a[0].ld * 2, ldb2 = (int)q.b[0].ld * 2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (AKS) {
+      const int kr = (wave * 4 + i) * 4 + (lane >> 4), sw = (kr & 3) | ((kr >> 3 & 1) << 2);
+      const int cc = ((((lane & 15) >> 1) ^ sw) << 1) | (lane & 1);
+      pca[i] = cc * 8; va[i] = (unsigned)(kr * lda2 + cc * 16);
+    } else {
+      const int r = (wave * 4 + i) * 8 + lr, ch = lc ^ lds_swz(r);
+      pca[i] = ch * 8; va[i] = (unsigned)(r * lda2 + ch * 16);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (wave * 2 + i) * 8 + lr;
+    if constexpr (BKS) {   // 64 k-rows x 64 columns: 128-byte rows, four 32-byte pieces each
+      const int sw = (r >> 1 & 1) | ((r >> 3 & 1) << 1);
+      const int cc = (((lc >> 1) ^ sw) << 1) | (lc & 1);
+      pcb[i] = cc * 8; vb[i] = (unsigned)(r * ldb2 + cc * 16);
+    } else {
+      const int ch = lc ^ lds_swz(r), wr = (og_gate(EPI) ? 0 : (r & ~31)) + perm32(r & 31);
+      pcb[i] = ch * 8; vb[i] = (unsigned)(wr * ldb2 + ch * 16);
+    }
+  }
+  struct Stream { const char* p; int size, left; };
+  Stream sa, sb;
+  [[maybe_unused]] int seg = 0;
+  const int a_left = q.M - m0, b_left = q.Nb - n0;
+  auto set_a = [&](int s, int kk) {
+    const OpMat A = q.a[s];
+    if constexpr (AKS) sa = Stream{(const char*)(A.p + (long long)kk * A.ld + m0), ((min(a_left, 128) + 7) & ~7) * 2 - lda2, p.K[s] - kk};
+    else sa = Stream{(const char*)(A.p + (long long)m0 * A.ld + kk), a_left > 0 ? (min(a_left, 128) - 1) * lda2 : -(1 << 30), ((p.K[s] + 7) & ~7) - kk};
+    seg = s;
+  };
+  auto set_b = [&](int s, int kk) {
+    const OpMat B = og_gate(EPI) ? (wave >= 2 ? q.b[1] : q.b[0]) : q.b[s];
+    if constexpr (BKS) sb = Stream{(const char*)(B.p + (long long)kk * B.ld + n0), ((min(b_left, 64) + 7) & ~7) * 2 - ldb2, p.K[s] - kk};
+    else sb = Stream{(const char*)(B.p + (long long)n0 * B.ld + kk), b_left > 0 ? (min(b_left, og_gate(EPI) ? 32 : 64) - 1) * ldb2 : -(1 << 30), ((p.K[s] + 7) & ~7) - kk};
+  };
+  {
+    const int nk0 = (p.K[0] + 63) / 64;
+    if (NSEG == 2 && k0 >= nk0) { set_a(1, (k0 - nk0) * 64); set_b(1, (k0 - nk0) * 64); }
+    else { set_a(0, k0 * 64); set_b(0, k0 * 64); }
+  }
+  auto issue = [&](int stage) {
+    if constexpr (NSEG == 2) {
+      if (sa.left <= 0 && seg == 0) { set_a(1, 0); set_b(1, 0); }
+    }
+    char* l = smem + stage * kOsStage;
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)sa.p, 0, max(AKS ? min(sa.left, 64) * lda2 + sa.size : sa.size + sa.left * 2, 0), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)sb.p, 0, max(BKS ? min(sb.left, 64) * ldb2 + sb.size : sb.size + sb.left * 2, 0), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, LPTR(l + (wave * 4 + i) * 1024), 16, (int)(pca[i] < (AKS ? a_left : sa.left) ? va[i] : kOob), 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, LPTR(l + kOsA + (wave * 2 + i) * 1024), 16, (int)(pcb[i] < (BKS ? b_left : sb.left) ? vb[i] : kOob), 0, 0, 0);
+    sa.p += AKS ? (long long)64 * lda2 : 128ll; sa.left -= 64;
+    sb.p += BKS ? (long long)64 * ldb2 : 128ll; sb.left -= 64;
+  };
+
+  // ---- fragments
+  const int tq = (lane & 15) >> 2, tp = lane & 3;
+  int a_off[2], a_sw[2], b_off[4], b_sw[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = wave * 32 + i * 16 + fr;
+    if constexpr (AKS) { a_off[i] = (fq * 8 + tq) * 256 + (((wave * 2 + i) ^ (tq | ((fq & 1) << 2))) << 5) + 8 * tp; a_sw[i] = 0; }
+    else { a_off[i] = r * 128; a_sw[i] = lds_swz(r); }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {   // tiles 2 g, 2 g + 1 of the 32-column group g
+    const int r = j * 16 + fr;
+    if constexpr (BKS) {
+      const int sw = (tq >> 1) | ((fq & 1) << 1);
+      b_off[j] = kOsA + (fq * 8 + tq) * 128 + ((((j >> 1) * 2 + (tp >> 1)) ^ sw) << 5) + (tp & 1) * 16 + 8 * (j & 1);
+      b_sw[j] = 0;
+    } else { b_off[j] = kOsA + r * 128; b_sw[j] = lds_swz(r); }
+  }
+  f32x4 acc[2][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  issue(0);
+  if (nk > 1) issue(1);
+  int cur = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    if (kt + 1 < nk) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");   // the 6 copies of the next K-tile may stay in flight
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();   // this K-tile is in LDS for everybody; everybody has read the one before last's buffer
+    __builtin_amdgcn_sched_barrier(0);
+    const int nxt = cur == 0 ? 2 : cur - 1;   // (cur + 2) % 3
+    if (kt + 2 < nk) issue(nxt);
+    const char* base = smem + cur * kOsStage;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      u16x8 fa[2], fb[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (BKS) fb[j] = tr_frag((const lds_s16x4*)(base + b_off[j] + ks * 4096), (const lds_s16x4*)(base + b_off[j] + ks * 4096 + 512));
+        else fb[j] = *(const u16x8*)(base + b_off[j] + (((ks * 4 + fq) ^ b_sw[j]) << 4));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (AKS) fa[i] = tr_frag((const lds_s16x4*)(base + a_off[i] + ks * 8192), (const lds_s16x4*)(base + a_off[i] + ks * 8192 + 1024));
+        else fa[i] = *(const u16x8*)(base + a_off[i] + (((ks * 4 + fq) ^ a_sw[i]) << 4));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = mfma16<F16>(fb[j], fa[i], acc[i][j]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    cur = cur == 2 ? 0 : cur + 1;
+  }
+
+  // ---- epilogue
+  OpTile<F16> t;
+  t.m0 = m0; t.n0 = n0;
+  t.rows = min(128, q.M - m0);
+  t.cols = q.N - n0;
+  t.bcols = q.Nb - n0;
+  const int c0 = 8 * fq, c1 = og_gate(EPI) ? c0 : 32 + 8 * fq;
+  auto row_of = [&](int i) { return wave * 32 + i * 16 + fr; };
+  float v0[8], v1[8];
+  auto take = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) { v0[k] = acc[i][k >> 2][k & 3]; v1[k] = acc[i][2 + (k >> 2)][k & 3]; }
+  };
+  if constexpr (EPI == OG_PLAIN) {
+    const __amdgpu_buffer_rsrc_t rc = t.rsrc(q.c, q.ldc, 2);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      take(i);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v0[k] += c0 + k < t.bcols ? op_bias(p.bias, n0 + c0 + k, p.bias_f32, F16) : 0.f;
+        v1[k] += c1 + k < t.bcols ? op_bias(p.bias, n0 + c1 + k, p.bias_f32, F16) : 0.f;
+      }
+      t.template store<8>(rc, q.ldc, q.cvec, row_of(i), c0, v0);
+      t.template store<8>(rc, q.ldc, q.cvec, row_of(i), c1, v1);
+    }
+  } else if constexpr (EPI == OG_PART) {
+    const __amdgpu_buffer_rsrc_t rc = t.rsrc((const float*)q.c + (long long)split * p.split_stride, q.ldc, 4);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      take(i);
+      t.template store32<8>(rc, q.ldc, row_of(i), c0, v0);
+      t.template store32<8>(rc, q.ldc, row_of(i), c1, v1);
+    }
+  } else if constexpr (og_gate(EPI)) {
+    const OgGate<F16, EPI == OG_GATE_SAVE> gate(p, t, q.c, c0);
+    og_by_act(p.act, [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) { take(i); gate.template row<decltype(act)::value>(row_of(i), c0, v0, v1); }
+    });
+  } else {
+    OgDgate<F16> grad(p, t);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      grad.clear();
+      grad.template groups<2, 8>(half ? c1 : c0, row_of, [&](int i, int k) { return acc[i][half * 2 + (k >> 2)][k & 3]; });
+      grad.template finish<8>(half ? c1 : c0, fr, (long long)tile_m * 4 + wave, q.tiles_m * 4ll);
+    }
+  }
 }
 
 }  // namespace vtc

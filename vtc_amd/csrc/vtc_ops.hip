@@ -494,22 +494,50 @@ int group_of(int tiles_m, int tiles_n, double a_bytes, double w_bytes, double w_
   return r;
 }
 
-void finish_prob(OpProb& q, int bn, int K, int tile0) {
-  q.tiles_m = (q.M + 255) / 256;
-  q.tiles_n = (q.N + bn - 1) / bn;
-  q.group_n = group_of(q.tiles_m, q.tiles_n, 2.0 * q.M * K, 2.0 * q.N * K, 2.0 * bn * K);
+// How a product runs: tile size and K splits.  The times are measured ones (us): a K-tile of 256 x 256 x 64 takes a CU 2.2 and
+// a tile's start and epilogue 4; of 128 x 64 x 64 0.6 with two blocks on the CU, and 3; partials cross memory twice at 4 TB/s and
+// cost a launch.  Crossovers seen: 499 x 768 -> 2 x 2048 gate / up 26 us in 256-wide tiles, 11 in small ones; 31936 rows 227 / 340.
+struct OgPlan { bool small; int splits, kps; };
+OgPlan og_plan(long long tiles_big, double width, long long tiles_small, int nk, int splits_big, int splits_small, double out_elems) {
+  OgPlan best{false, 1, (nk + 1) & ~1};
+  double cost = 1e300;
+  for (int small = 0; small < 2; ++small)
+    for (int sp = 1; sp <= (small ? splits_small : splits_big); ++sp) {
+      int k = (nk + sp - 1) / sp;
+      if (!small) k = (k + 1) & ~1;
+      if ((nk + k - 1) / k != sp || (sp > 1 && k < 4)) continue;
+      const double units = (double)(small ? tiles_small : tiles_big) * sp;
+      const double rounds = std::ceil(units / (small ? 512.0 : 256.0));
+      double c = small ? rounds * (k * 0.6 + 3.0) : rounds * (k * 2.2 * width + 4.0);
+      if (sp > 1) c += 4.0 + sp * out_elems * 8.0 / 4.0e6;
+      if (c < cost) { cost = c; best = OgPlan{small != 0, sp, k}; }
+    }
+  return best;
+}
+int div_up(long long a, int b) { return (int)((a + b - 1) / b); }
+
+void finish_prob(OpProb& q, bool small, int bm, int bn, int K, int tile0) {
+  q.tiles_m = div_up(q.M, bm);
+  q.tiles_n = div_up(q.N, bn);
+  q.group_n = small ? q.tiles_n : group_of(q.tiles_m, q.tiles_n, 2.0 * q.M * K, 2.0 * q.N * K, 2.0 * bn * K);
   q.tile0 = tile0;
 }
-void set_k(OpGemmParams& p, int k0, int k1 = 0) {
+void set_k(OpGemmParams& p, const OgPlan& plan, int k0, int k1 = 0) {
   p.K[0] = k0; p.K[1] = k1;
-  p.nk0 = (k0 + 63) / 64;
-  p.nk = (p.nk0 + (k1 + 63) / 64 + 1) & ~1;   // the kernel takes K-tiles in pairs; one behind the end reads as zero
-  if (!k1) p.nk0 = p.nk;
-  p.splits = 1; p.kps = p.nk;
+  p.nk = div_up(k0, 64) + div_up(k1, 64);
+  if (!plan.small) p.nk = (p.nk + 1) & ~1;   // op_gemm_kernel takes K-tiles in pairs; one behind the end reads as zero
+  p.splits = plan.splits; p.kps = plan.splits == 1 ? p.nk : plan.kps;
 }
-template <bool F16, bool AKS, bool BKS, int EPI, int BN> void launch_op_gemm(OpGemmParams& p, hipStream_t s) {
+template <bool F16, bool AKS, bool BKS, int EPI, int BN> void launch_og(const OpGemmParams& p, bool small, hipStream_t s) {
   const int units = p.ntiles * p.splits;
-  hipLaunchKernelGGL((op_gemm_kernel<F16, AKS, BKS, EPI, BN>), dim3((unsigned)std::min(units, 256)), dim3(512), 0, s, p);
+  if (small) hipLaunchKernelGGL((op_small_kernel<F16, AKS, BKS, EPI>), dim3((unsigned)units), dim3(256), 0, s, p);
+  else if constexpr (EPI != OG_PART || AKS)   // 256-wide tiles are split over K for the weights' gradients only
+    hipLaunchKernelGGL((op_gemm_kernel<F16, AKS, BKS, EPI, BN>), dim3((unsigned)std::min(units, 256)), dim3(512), 0, s, p);
+}
+template <bool F16> void launch_reduce(const SplitReduceParams& r, hipStream_t s) {
+  long long most = 1;
+  for (int i = 0; i < r.n; ++i) most = std::max(most, r.r[i].rows * (r.r[i].pitch / 4));
+  hipLaunchKernelGGL((split_reduce_kernel<F16>), dim3((unsigned)std::min<long long>((most + 255) / 256, 16384), (unsigned)r.n), dim3(256), 0, s, r);
 }
 template <bool F16, bool GATE> void launch_skinny(const SkinnyParams& p, hipStream_t s) {
   const dim3 grid((unsigned)((p.N + 15) / 16)), block(512);
@@ -522,48 +550,72 @@ template <typename F> void by_f16(int dtype, F&& f) {
   else f(std::false_type{});
 }
 
-struct GateOut { h16 *h, *g, *u; };   // g, u: null where no backward pass follows
-template <bool F16> void gate_up(int64_t M, int K, int F, OpMat x, OpMat wg, OpMat wu, const void* bg, const void* bu, int bias_f32, int act, GateOut o, hipStream_t s) {
+struct GateOut { h16* h; Saved24 s, a; };   // s.hi: null where no backward pass follows
+template <bool F16> void gate_up(int64_t M, int K, int F, OpMat x, OpMat wg, OpMat wu, const void* bg, const void* bu, int bias_f32, int act, GateOut o,
+                                 bool skinny, hipStream_t s) {
   const int F8 = up8(F);
-  if (M <= kSkinnyRows) {
+  if (skinny) {
     SkinnyParams p{};
     p.x = x.p; p.ldx = x.ld; p.w0 = wg.p; p.w1 = wu.p; p.ldw = wg.ld;
     p.M = (int)M; p.K = K; p.N = F8; p.Nb = F; p.b0 = bg; p.b1 = bu; p.bias_f32 = bias_f32; p.act = act;
-    p.out = o.h; p.g = o.g; p.u = o.u; p.ldo = F8;
+    p.out = o.h; p.s = o.s; p.a = o.a; p.ldo = F8;
     launch_skinny<F16, true>(p, s);
     return;
   }
+  const OgPlan plan = og_plan((long long)div_up(M, 256) * div_up(F8, 128), 1.0, (long long)div_up(M, 128) * div_up(F8, 32), div_up(K, 64), 1, 1, 0);
   OpGemmParams p{};
   p.nprob = 1;
   OpProb& q = p.prob[0];
   q.a[0] = x; q.b[0] = wg; q.b[1] = wu; q.c = o.h; q.ldc = F8; q.M = (int)M; q.N = F8; q.Nb = F; q.cvec = 1;
-  finish_prob(q, 128, K, 0);
+  finish_prob(q, plan.small, plan.small ? 128 : 256, plan.small ? 32 : 128, K, 0);
   p.ntiles = q.tiles_m * q.tiles_n;
-  set_k(p, K);
-  p.bias = bg; p.bias2 = bu; p.bias_f32 = bias_f32; p.act = act; p.g = o.g; p.u = o.u; p.ldg = F8;
-  launch_op_gemm<F16, false, false, OG_GATE, 256>(p, s);
+  set_k(p, plan, K);
+  p.bias = bg; p.bias2 = bu; p.bias_f32 = bias_f32; p.act = act; p.s = o.s; p.a = o.a; p.ldg = F8;
+  if (o.s.hi) launch_og<F16, false, false, OG_GATE_SAVE, 256>(p, plan.small, s);
+  else launch_og<F16, false, false, OG_GATE, 256>(p, plan.small, s);
 }
-template <bool F16> void down(int64_t M, int F, int N, OpMat h, OpMat wd, const void* bd, int bias_f32, void* y, long long ldy, hipStream_t s) {
-  const int cvec = N % 8 == 0 && ldy % 8 == 0 && (uintptr_t)y % 16 == 0;
-  if (M <= kSkinnyRows) {
-    SkinnyParams p{};
-    p.x = h.p; p.ldx = h.ld; p.w0 = p.w1 = wd.p; p.ldw = wd.ld;
-    p.M = (int)M; p.K = F; p.N = p.Nb = N; p.b0 = bd; p.bias_f32 = bias_f32; p.out = (h16*)y; p.ldo = ldy;
-    launch_skinny<F16, false>(p, s);
-    return;
-  }
+
+// C = A B^T (+ bias) in 16 bits for one or two operand pairs; with few tiles in K splits whose partials lie in the workspace
+struct OutPlan { OgPlan plan; int N8; float* part; };
+OutPlan plan_out(Arena& ar, int64_t M, int N, int nk) {
+  OutPlan o{og_plan((long long)div_up(M, 256) * div_up(N, 192), 0.75, (long long)div_up(M, 128) * div_up(N, 64), nk, 1, 32, (double)M * N), up8(N), nullptr};
+  if (o.plan.splits > 1) o.part = ar.take<float>((size_t)o.plan.splits * M * o.N8);
+  return o;
+}
+template <bool F16, bool BKS> void product_out(const OutPlan& o, int64_t M, int N, const OpMat* a, const OpMat* b, const int* k, int segs, const void* bias,
+                                               int bias_f32, void* c, long long ldc, hipStream_t s) {
+  const bool small = o.plan.small;
+  const int cvec = N % 8 == 0 && ldc % 8 == 0 && (uintptr_t)c % 16 == 0;
   OpGemmParams p{};
   p.nprob = 1;
   OpProb& q = p.prob[0];
-  q.a[0] = h; q.b[0] = wd; q.c = y; q.ldc = ldy; q.M = (int)M; q.N = q.Nb = N; q.cvec = cvec;
-  finish_prob(q, 192, F, 0);
+  for (int i = 0; i < segs; ++i) { q.a[i] = a[i]; q.b[i] = b[i]; }
+  q.M = (int)M; q.Nb = N; q.cvec = cvec;
+  if (o.part) { q.c = o.part; q.ldc = o.N8; q.N = o.N8; }
+  else { q.c = c; q.ldc = ldc; q.N = N; }
+  finish_prob(q, small, small ? 128 : 256, small ? 64 : 192, k[0] + (segs > 1 ? k[1] : 0), 0);
   p.ntiles = q.tiles_m * q.tiles_n;
-  set_k(p, F);
-  p.bias = bd; p.bias_f32 = bias_f32;
-  launch_op_gemm<F16, false, false, OG_PLAIN, 192>(p, s);
+  set_k(p, o.plan, k[0], segs > 1 ? k[1] : 0);
+  p.bias = bias; p.bias_f32 = bias_f32;
+  if (!o.part) { launch_og<F16, false, BKS, OG_PLAIN, 192>(p, small, s); return; }
+  p.split_stride = M * o.N8;
+  launch_og<F16, false, BKS, OG_PART, 192>(p, true, s);
+  SplitReduceParams r{};
+  r.r[0] = SplitReduce{o.part, (h16*)c, ldc, o.N8, M, N, cvec, bias};
+  r.n = 1; r.splits = p.splits; r.stride = p.split_stride; r.bias_f32 = bias_f32;
+  launch_reduce<F16>(r, s);
 }
 
-size_t ffn_forward(const FfnArgs& a, const vtc_mat* y, h16* save_g, h16* save_u, h16* save_h, char* ws, bool launch, hipStream_t s) {
+// Layout of what the forward call keeps: h, then the upper 16 bits of s and of a, then their next 8 bits
+struct FfnSaved { h16* h; Saved24 s, a; };
+FfnSaved ffn_saved(void* base, int64_t rows, int inner) {
+  if (!base) return FfnSaved{};
+  const size_t n = (size_t)rows * up8(inner), two = align256(2 * n), one = align256(n);
+  char* b = (char*)base;
+  return FfnSaved{(h16*)b, {(unsigned short*)(b + two), (unsigned char*)(b + 3 * two)}, {(unsigned short*)(b + 2 * two), (unsigned char*)(b + 3 * two + one)}};
+}
+
+size_t ffn_forward(const FfnArgs& a, const vtc_mat* y, void* saved, char* ws, bool launch, hipStream_t s) {
   Arena ar{ws};
   const int F8 = up8(a.F);
   const OpMat x = operand(ar, a.x, a.M, a.K, false, s, launch);
@@ -571,34 +623,29 @@ size_t ffn_forward(const FfnArgs& a, const vtc_mat* y, h16* save_g, h16* save_u,
   const bool copy_w = a.wg->row != a.wu->row || !pieces_ok(a.wg, a.K) || !pieces_ok(a.wu, a.K);
   const OpMat wg = operand(ar, a.wg, a.F, a.K, copy_w, s, launch), wu = operand(ar, a.wu, a.F, a.K, copy_w, s, launch);
   const OpMat wd = operand(ar, a.wd, a.N, a.F, false, s, launch);
-  h16* h = save_h ? save_h : ar.take<h16>((size_t)a.M * F8);
+  const FfnSaved sv = ffn_saved(saved, a.M, a.F);
+  h16* h = saved ? sv.h : ar.take<h16>((size_t)a.M * F8);
+  const bool skinny = a.M <= kSkinnyRows;
+  OutPlan out{};
+  if (!skinny) out = plan_out(ar, a.M, a.N, div_up(a.F, 64));
   if (!launch) return ar.used;
   by_f16(a.dtype, [&](auto f) {
     constexpr bool F16 = decltype(f)::value;
-    gate_up<F16>(a.M, a.K, a.F, x, wg, wu, a.bg, a.bu, a.bias_f32, a.act, GateOut{h, save_g, save_u}, s);
-    down<F16>(a.M, a.F, a.N, OpMat{h, F8}, wd, a.bd, a.bias_f32, (void*)y->p, y->row, s);
+    gate_up<F16>(a.M, a.K, a.F, x, wg, wu, a.bg, a.bu, a.bias_f32, a.act, GateOut{h, sv.s, sv.a}, skinny, s);
+    if (skinny) {
+      SkinnyParams p{};
+      p.x = h; p.ldx = F8; p.w0 = p.w1 = wd.p; p.ldw = wd.ld;
+      p.M = (int)a.M; p.K = a.F; p.N = p.Nb = a.N; p.b0 = a.bd; p.bias_f32 = a.bias_f32; p.out = (h16*)y->p; p.ldo = y->row;
+      launch_skinny<F16, false>(p, s);
+    } else {
+      const OpMat hm{h, F8};
+      product_out<F16, false>(out, a.M, a.N, &hm, &wd, &a.F, 1, a.bd, a.bias_f32, (void*)y->p, y->row, s);
+    }
   });
   return ar.used;
 }
 
-// K splits of the weights' gradients: few output tiles, a long contraction over the rows.  Enough units for every CU, no split
-// shorter than 8 K-tiles (512 rows: below that the fp32 partials cost more than they save).
-void ffn_splits(int tiles, int nk, int* splits, int* kps) {
-  int best = 1;
-  double cost = 1e300;
-  for (int sp = 1; sp <= 64; ++sp) {
-    const int k = (((nk + sp - 1) / sp) + 1) & ~1;
-    const int real = (nk + k - 1) / k;
-    if (real != sp || (sp > 1 && k < 8)) continue;
-    const double rounds = std::ceil((double)tiles * sp / 256.0);
-    const double c = rounds * (k + 4.0) + 0.35 * sp * tiles / 256.0 * 4.0;   // K-tile times; a tile's partial costs ~1.4 of them to write and read
-    if (c < cost) { cost = c; best = sp; }
-  }
-  *kps = (((nk + best - 1) / best) + 1) & ~1;
-  *splits = best;
-}
-
-size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const h16* g, const h16* u, const h16* h, const vtc_ffn_grads* o, char* ws, bool launch, hipStream_t s) {
+size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, const vtc_ffn_grads* o, char* ws, bool launch, hipStream_t s) {
   Arena ar{ws};
   const int K8 = up8(a.K), F8 = up8(a.F), N8 = up8(a.N);
   const int M = (int)a.M;
@@ -607,81 +654,78 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const h16* g, const h16
   const OpMat wg = operand(ar, a.wg, a.F, a.K, copy_w, s, launch), wu = operand(ar, a.wu, a.F, a.K, copy_w, s, launch);
   const OpMat wd = operand(ar, a.wd, a.N, a.F, false, s, launch);
   h16 *dg = ar.take<h16>((size_t)a.M * F8), *du = ar.take<h16>((size_t)a.M * F8);
-  const int tiles_m = (M + 255) / 256, row_blocks = (M + 255) / 256;
-  float* cs_f = (o->db_gate || o->db_up) || !launch ? ar.take<float>((size_t)2 * 2 * tiles_m * F8) : nullptr;
+  // dh and what it turns into
+  const OgPlan dplan = og_plan((long long)div_up(M, 256) * div_up(F8, 192), 0.75, (long long)div_up(M, 128) * div_up(F8, 64), div_up(a.N, 64), 1, 1, 0);
+  const long long parts = dplan.small ? 4ll * div_up(M, 128) : 2ll * div_up(M, 256);
+  const int row_blocks = div_up(M, 256);
+  float* cs_f = (o->db_gate || o->db_up) || !launch ? ar.take<float>((size_t)2 * parts * F8) : nullptr;
   float* cs_n = o->db_down || !launch ? ar.take<float>((size_t)row_blocks * N8) : nullptr;
-  // weights' gradients
+  const OutPlan xplan = plan_out(ar, M, a.K, 2 * div_up(a.F, 64));
+  // weights' gradients: few output tiles, a long contraction over the rows, so in K splits
   OpGemmParams w{};
   w.nprob = 3;
   const h16* as[3] = {dg, du, y.p};
   const long long lda[3] = {F8, F8, y.ld};
-  const h16* bs[3] = {x.p, x.p, h};
+  const h16* bs[3] = {x.p, x.p, launch ? ffn_saved((void*)saved, a.M, a.F).h : nullptr};
   const long long ldb[3] = {x.ld, x.ld, F8};
   const int rows[3] = {a.F, a.F, a.N}, cols[3] = {a.K, a.K, a.F}, pitch[3] = {K8, K8, F8};
+  long long tb = 0, ts = 0;
+  for (int i = 0; i < 3; ++i) { tb += (long long)div_up(rows[i], 256) * div_up(pitch[i], 256); ts += (long long)div_up(rows[i], 128) * div_up(pitch[i], 64); }
+  const long long one = (long long)a.F * K8;
+  w.split_stride = 2 * one + (long long)a.N * F8;
+  const OgPlan wplan = og_plan(tb, 1.0, ts, div_up(M, 64), 32, 32, (double)w.split_stride);
   int tiles = 0;
   for (int i = 0; i < 3; ++i) {
     OpProb& q = w.prob[i];
     q.a[0] = OpMat{as[i], lda[i]}; q.b[0] = OpMat{bs[i], ldb[i]};
     q.M = rows[i]; q.N = pitch[i]; q.Nb = cols[i]; q.ldc = pitch[i];
-    finish_prob(q, 256, M, tiles);
+    finish_prob(q, wplan.small, wplan.small ? 128 : 256, wplan.small ? 64 : 256, M, tiles);
     tiles += q.tiles_m * q.tiles_n;
   }
   w.ntiles = tiles;
-  set_k(w, M);
-  ffn_splits(tiles, w.nk, &w.splits, &w.kps);
-  const long long one = (long long)a.F * K8;
-  w.split_stride = 2 * one + (long long)a.N * F8;
-  float* part = ar.take<float>((size_t)w.splits * w.split_stride);
+  set_k(w, wplan, M);
+  float* part = o->dw_gate || !launch ? ar.take<float>((size_t)w.splits * w.split_stride) : nullptr;
   if (!launch) return ar.used;
   for (int i = 0; i < 3; ++i) w.prob[i].c = part + i * one;
 
+  const FfnSaved sv = ffn_saved((void*)saved, a.M, a.F);
   by_f16(a.dtype, [&](auto f) {
     constexpr bool F16 = decltype(f)::value;
     OpGemmParams d{};
     d.nprob = 1;
     OpProb& e = d.prob[0];
     e.a[0] = y; e.b[0] = wd; e.M = M; e.N = F8; e.Nb = a.F; e.ldc = F8;
-    finish_prob(e, 256, a.N, 0);
+    finish_prob(e, dplan.small, dplan.small ? 128 : 256, dplan.small ? 64 : 192, a.N, 0);
     d.ntiles = e.tiles_m * e.tiles_n;
-    set_k(d, a.N);
-    d.act = a.act; d.g = (h16*)g; d.u = (h16*)u; d.dg = dg; d.du = du; d.ldg = F8; d.colsum = cs_f;
-    launch_op_gemm<F16, false, true, OG_DGATE, 256>(d, s);
+    set_k(d, dplan, a.N);
+    d.s = sv.s; d.a = sv.a; d.dg = dg; d.du = du; d.ldg = F8; d.colsum = cs_f;
+    launch_og<F16, false, true, OG_DGATE, 192>(d, dplan.small, s);
     if (o->dx) {
-      OpGemmParams c{};
-      c.nprob = 1;
-      OpProb& q = c.prob[0];
-      q.a[0] = OpMat{dg, F8}; q.a[1] = OpMat{du, F8}; q.b[0] = wg; q.b[1] = wu;
-      q.c = o->dx; q.ldc = o->dx_row; q.M = M; q.N = q.Nb = a.K;
-      q.cvec = a.K % 8 == 0 && o->dx_row % 8 == 0 && (uintptr_t)o->dx % 16 == 0;
-      finish_prob(q, 256, 2 * a.F, 0);
-      c.ntiles = q.tiles_m * q.tiles_n;
-      set_k(c, a.F, a.F);
-      launch_op_gemm<F16, false, true, OG_PLAIN, 256>(c, s);
+      const OpMat xa[2] = {{dg, F8}, {du, F8}}, xb[2] = {wg, wu};
+      const int xk[2] = {a.F, a.F};
+      product_out<F16, true>(xplan, M, a.K, xa, xb, xk, 2, nullptr, 0, o->dx, o->dx_row, s);
     }
-    if (o->dw_gate) {
-      launch_op_gemm<F16, true, true, OG_PART, 256>(w, s);
+    if (part) {
+      launch_og<F16, true, true, OG_PART, 256>(w, wplan.small, s);
       SplitReduceParams r{};
       void* outs[3] = {o->dw_gate, o->dw_up, o->dw_down};
-      long long most = 0;
-      for (int i = 0; i < 3; ++i) {
-        r.r[i] = SplitReduce{part + i * one, (h16*)outs[i], cols[i], pitch[i], rows[i], cols[i], cols[i] % 8 == 0 && (uintptr_t)outs[i] % 16 == 0};
-        most = std::max(most, (long long)rows[i] * (pitch[i] / 4));
-      }
+      for (int i = 0; i < 3; ++i)
+        r.r[i] = SplitReduce{part + i * one, (h16*)outs[i], cols[i], pitch[i], rows[i], cols[i], cols[i] % 8 == 0 && (uintptr_t)outs[i] % 16 == 0, nullptr};
       r.n = 3; r.splits = w.splits; r.stride = w.split_stride;
-      hipLaunchKernelGGL((split_reduce_kernel<F16>), dim3((unsigned)std::min<long long>((most + 255) / 256, 16384), 3), dim3(256), 0, s, r);
+      launch_reduce<F16>(r, s);
     }
     if (cs_n) hipLaunchKernelGGL((colsum_kernel<F16>), dim3((unsigned)row_blocks, (unsigned)((N8 / 8 + 63) / 64)), dim3(256), 0, s, y.p, y.ld, cs_n, N8,
                                  (long long)M, a.N);
     if (cs_f || cs_n) {
       ColReduceParams r{};
       int n = 0, widest = 1;
-      auto add = [&](float* src, void* out, long long parts, int pitch_, int c) {
+      auto add = [&](float* src, void* out, long long count, int pitch_, int c) {
         if (!out) return;
-        r.r[n++] = ColReduce{src, out, parts, pitch_, c};
+        r.r[n++] = ColReduce{src, out, count, pitch_, c};
         widest = std::max(widest, c);
       };
-      add(cs_f, o->db_gate, 2ll * tiles_m, F8, a.F);
-      add(cs_f ? cs_f + (size_t)2 * tiles_m * F8 : nullptr, o->db_up, 2ll * tiles_m, F8, a.F);
+      add(cs_f, o->db_gate, parts, F8, a.F);
+      add(cs_f ? cs_f + (size_t)parts * F8 : nullptr, o->db_up, parts, F8, a.F);
       add(cs_n, o->db_down, row_blocks, N8, a.N);
       r.f16 = F16; r.out_f32 = a.bias_f32;
       hipLaunchKernelGGL(col_reduce_kernel, dim3((unsigned)((widest + 63) / 64), (unsigned)n), dim3(256), 0, s, r);
@@ -695,7 +739,7 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const h16* g, const h16
 void vtc::launch_gated_up(int dtype, int64_t M, int K, int F, const unsigned short* x, const unsigned short* wg, const unsigned short* wu, const float* bg,
                           const float* bu, int act, unsigned short* h, hipStream_t s) {
   by_f16(dtype, [&](auto f) {
-    gate_up<decltype(f)::value>(M, K, F, OpMat{x, K}, OpMat{wg, K}, OpMat{wu, K}, bg, bu, 1, act, GateOut{h, nullptr, nullptr}, s);
+    gate_up<decltype(f)::value>(M, K, F, OpMat{x, K}, OpMat{wg, K}, OpMat{wu, K}, bg, bu, 1, act, GateOut{h, {}, {}}, false, s);
   });
 }
 
@@ -705,18 +749,16 @@ extern "C" int64_t vtc_gated_ffn_workspace(int64_t rows, int32_t width, int32_t 
     return VTC_ERR_ARG;
   }
   if (rows == 0) return 0;
-  const vtc_mat m{nullptr, 0};   // a null matrix counts as one that has to be copied: enough for every alignment
-  FfnArgs a{OP_F16, 0, 0, rows, width, inner, out_width, &m, &m, &m, &m, nullptr, nullptr, nullptr};
-  vtc_mat odd{(const void*)2, 1};
-  a.x = a.wg = a.wu = a.wd = &odd;
+  const vtc_mat odd{(const void*)2, 1};   // operands that all have to be copied: enough for every alignment
+  const FfnArgs a{OP_F16, 0, 0, rows, width, inner, out_width, &odd, &odd, &odd, &odd, nullptr, nullptr, nullptr};
   vtc_ffn_grads o{};
-  return (int64_t)(backward ? ffn_backward(a, &odd, nullptr, nullptr, nullptr, &o, nullptr, false, nullptr)
-                            : ffn_forward(a, nullptr, nullptr, nullptr, nullptr, nullptr, false, nullptr));
+  return (int64_t)(backward ? ffn_backward(a, &odd, nullptr, &o, nullptr, false, nullptr) : ffn_forward(a, nullptr, nullptr, nullptr, false, nullptr));
 }
 
 extern "C" int64_t vtc_gated_ffn_saved(int64_t rows, int32_t inner) {
   if (rows < 0 || inner < 1 || inner > kFfnMaxDim || rows > (1ll << 31) - 256) { fail_handleless(VTC_ERR_ARG, "gated ffn: bad sizes"); return VTC_ERR_ARG; }
-  return 3 * (int64_t)align256((size_t)rows * up8(inner) * 2);
+  const size_t n = (size_t)rows * up8(inner);
+  return (int64_t)(3 * align256(2 * n) + 2 * align256(n));
 }
 
 extern "C" int vtc_gated_ffn(int device, int dtype, int64_t rows, int32_t width, int32_t inner, int32_t out_width, const vtc_mat* x,
@@ -732,25 +774,21 @@ extern "C" int vtc_gated_ffn(int device, int dtype, int64_t rows, int32_t width,
   if (overlap(x->p, end_of(x->p, {{rows, x->row}}, width, 2), y->p, y_end)) return fail_handleless(VTC_ERR_ARG, "%s: y overlaps x", what);
   const int64_t need_s = vtc_gated_ffn_saved(rows, inner);
   if (saved && saved_bytes < need_s) return fail_handleless(VTC_ERR_CAPACITY, "%s: the saved buffer holds %lld bytes, %lld needed", what, (long long)saved_bytes, (long long)need_s);
-  const size_t need = ffn_forward(a, nullptr, nullptr, nullptr, (h16*)saved, nullptr, false, nullptr);
+  const size_t need = ffn_forward(a, nullptr, saved, nullptr, false, nullptr);
   if (need && (!workspace || workspace_bytes < (int64_t)need)) return fail_handleless(VTC_ERR_CAPACITY, "%s: the workspace holds %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
   if ((uintptr_t)workspace % 256 || (uintptr_t)saved % 256) return fail_handleless(VTC_ERR_ARG, "%s: workspace and saved buffer must be aligned to 256 bytes", what);
   DeviceGuard guard(device);
   if (guard.rc) return guard.rc;
-  const size_t part = align256((size_t)rows * up8(inner) * 2);
-  h16* sg = (h16*)saved;
-  h16* su = saved ? (h16*)((char*)saved + part) : nullptr;
-  h16* sh = saved ? (h16*)((char*)saved + 2 * part) : nullptr;
-  ffn_forward(a, y, sg, su, sh, (char*)workspace, true, (hipStream_t)stream);
+  ffn_forward(a, y, saved, (char*)workspace, true, (hipStream_t)stream);
   return launched(what);
 }
 
 extern "C" int vtc_gated_ffn_backward(int device, int dtype, int64_t rows, int32_t width, int32_t inner, int32_t out_width, const vtc_mat* dy,
                                       const vtc_mat* x, const vtc_mat* w_gate, const vtc_mat* w_up, const vtc_mat* w_down, const void* saved,
-                                      int64_t saved_bytes, int32_t bias_f32, int32_t act, const vtc_ffn_grads* grads, void* workspace,
+                                      int64_t saved_bytes, int32_t bias_f32, const vtc_ffn_grads* grads, void* workspace,
                                       int64_t workspace_bytes, void* stream) {
   const char* what = "gated ffn backward";
-  FfnArgs a{dtype, act, bias_f32, rows, width, inner, out_width, x, w_gate, w_up, w_down, nullptr, nullptr, nullptr};
+  FfnArgs a{dtype, ACT_NONE, bias_f32, rows, width, inner, out_width, x, w_gate, w_up, w_down, nullptr, nullptr, nullptr};
   if (int rc = ffn_check(what, a)) return rc;
   if (int rc = ffn_check_mat(what, "dy", dy, rows, out_width)) return rc;
   if (!grads) return fail_handleless(VTC_ERR_ARG, "%s: null argument", what);
@@ -767,13 +805,11 @@ extern "C" int vtc_gated_ffn_backward(int device, int dtype, int64_t rows, int32
   }
   const int64_t need_s = vtc_gated_ffn_saved(rows, inner);
   if (!saved || saved_bytes < need_s) return fail_handleless(VTC_ERR_CAPACITY, "%s: the saved buffer of the forward call holds %lld bytes, %lld needed", what, (long long)saved_bytes, (long long)need_s);
-  const size_t need = ffn_backward(a, dy, nullptr, nullptr, nullptr, grads, nullptr, false, nullptr);
+  const size_t need = ffn_backward(a, dy, nullptr, grads, nullptr, false, nullptr);
   if (!workspace || workspace_bytes < (int64_t)need) return fail_handleless(VTC_ERR_CAPACITY, "%s: the workspace holds %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
   if ((uintptr_t)workspace % 256 || (uintptr_t)saved % 256) return fail_handleless(VTC_ERR_ARG, "%s: workspace and saved buffer must be aligned to 256 bytes", what);
   DeviceGuard guard(device);
   if (guard.rc) return guard.rc;
-  const size_t part = align256((size_t)rows * up8(inner) * 2);
-  ffn_backward(a, dy, (const h16*)saved, (const h16*)((const char*)saved + part), (const h16*)((const char*)saved + 2 * part), grads, (char*)workspace, true,
-               (hipStream_t)stream);
+  ffn_backward(a, dy, saved, grads, (char*)workspace, true, (hipStream_t)stream);
   return launched(what);
 }

@@ -133,7 +133,7 @@ SYMBOLS = {
                                 C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, _matp, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
                                 C.c_void_p]),
     "vtc_gated_ffn_backward": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int32, C.c_int32, C.c_int32, _matp, _matp, _matp, _matp, _matp,
-                                         C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.POINTER(VtcFfnGrads), C.c_void_p, C.c_int64,
+                                         C.c_void_p, C.c_int64, C.c_int32, C.POINTER(VtcFfnGrads), C.c_void_p, C.c_int64,
                                          C.c_void_p]),
 }
 

@@ -442,7 +442,8 @@ def gated_ffn_forward(x: torch.Tensor, w_gate, w_up, w_down, b_gate=None, b_up=N
 def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate, w_up, w_down, saved, act: str = "silu", biases: bool = True,
                        bias_dtype=None, need_dx: bool = True, need_dw: bool = True):
     """(dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down) for dy = dLoss / dy and the forward call's `saved`; what is not asked for
-    (biases, need_dx, need_dw) is None.  Gradients have the type of what they belong to (biases: bias_dtype, default x's)."""
+    (biases, need_dx, need_dw) is None.  Gradients have the type of what they belong to (biases: bias_dtype, default x's).  act is the
+    forward call's; its slopes are part of `saved`."""
     what = "gated_ffn_backward"
     index, dt, _, k, f, n = _ffn_args(what, x, w_gate, w_up, w_down, (), act)
     _same(what, x, "dy", dy)
@@ -471,7 +472,7 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate, w_up, w_down, 
     ws = _workspace(size, x)
     grads = L.VtcFfnGrads(_ptr(dx), k, *(_ptr(t) for t in dw + db))
     rc = so.vtc_gated_ffn_backward(index, dt, m, k, f, n, _mat(drows, n), _mat(rows, k), _mat(w_gate, k), _mat(w_up, k), _mat(w_down, f),
-                                   saved.data_ptr(), saved.numel(), 1 if bias_dtype is torch.float32 else 0, ACTS[act], grads, ws.data_ptr(), size,
+                                   saved.data_ptr(), saved.numel(), 1 if bias_dtype is torch.float32 else 0, grads, ws.data_ptr(), size,
                                    _stream(index))
     if rc:
         L.check(rc)
