@@ -30,15 +30,16 @@ __global__ __launch_bounds__(256) void pad_copy_kernel(const h16* src, long long
   }
 }
 
-// column sums of 256 rows (dy -> partial sums of d b_down); part [blocks of rows][pitch]
+// column sums of kColRows rows (dy -> partial sums of d b_down); part [blocks of rows][pitch]
+constexpr int kColRows = 64;
 template <bool F16>
 __global__ __launch_bounds__(256) void colsum_kernel(const h16* x, long long ld, float* part, int pitch, long long rows, int cols) {
   __shared__ float red[4][64 * 8];
   const int v = blockIdx.y * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-  const long long r0 = (long long)blockIdx.x * 256, r1 = min(rows, r0 + 256);
+  const long long r0 = (long long)blockIdx.x * kColRows, r1 = min(rows, r0 + kColRows);
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (v * 8 < cols)
-#pragma unroll 4
+#pragma unroll 8
     for (long long r = r0 + w; r < r1; r += 4) {
       const u16x8 f = *(const u16x8*)(x + r * ld + v * 8);
 #pragma unroll
@@ -58,17 +59,19 @@ __global__ __launch_bounds__(256) void colsum_kernel(const h16* x, long long ld,
 struct ColReduce { const float* part; void* out; long long n; int pitch, cols; };
 // bias gradients: out[c] = sum over n partial rows, in order, fp64; up to three of them in one launch (blockIdx.y)
 struct ColReduceParams { ColReduce r[3]; int f16, out_f32; };
-__global__ __launch_bounds__(256) void col_reduce_kernel(const ColReduceParams p) {
-  __shared__ double red[4][64];
+__global__ __launch_bounds__(1024) void col_reduce_kernel(const ColReduceParams p) {
+  __shared__ double red[16][64];
   const ColReduce& q = p.r[blockIdx.y];
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
   double s = 0.0;
   if (c < q.cols)
-    for (long long i = w; i < q.n; i += 4) s += (double)q.part[i * q.pitch + c];
+#pragma unroll 8
+    for (long long i = w; i < q.n; i += 16) s += (double)q.part[i * q.pitch + c];
   red[w][threadIdx.x & 63] = s;
   __syncthreads();
   if (w || c >= q.cols) return;
-  const float v = (float)((red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]));
+  for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
+  const float v = (float)s;
   if (p.out_f32) ((float*)q.out)[c] = v;
   else ((h16*)q.out)[c] = p.f16 ? to_h16<true>(v) : to_h16<false>(v);
 }

@@ -1,9 +1,9 @@
 // Matrix products of the gated feed-forward block, any sizes: 256 x BN x 64 tiles, 8 waves, persistent, the schedule of
 // gemm256.hip.h (two K-tile buffers in LDS, four half-tiles, one half-tile prefetched per phase, counted vmcnt, staggered wave
 // rows) with three differences:
-//   * operands are fetched through buffer descriptors rebuilt per half-tile (scalar work): rows, columns and K beyond the matrix
-//     read as zero, so no size has to divide anything but 8 (16-byte pieces), and the 32-bit offsets are relative to the tile
-//     (matrices beyond 4 GiB work);
+//   * operands are fetched through buffer descriptors of the half-tile: rows and K beyond the matrix read as zero, so no size has to
+//     divide anything but 8 (16-byte pieces), and the 32-bit offsets are relative to the tile (matrices beyond 4 GiB work).  Only
+//     the descriptor's base moves along K;
 //   * an operand may be stored with the contraction index along its ROWS ("KS": dy^T h, dg^T x, dy W_down).  Its half-tile is 64
 //     k-rows x 128 columns (256 B each); ds_read_b64_tr_b16 hands every lane 4 k of one column, so two of them make the fragment
 //     that one ds_read_b128 reads from the other layout and nothing is transposed in memory.  32-byte pieces of a k-row are
@@ -68,6 +68,8 @@ __device__ __forceinline__ float op_bias(const void* b, int i, int f32, bool f16
 }
 
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+// k-rows a descriptor of a K-strided half-tile spans: 64, and the most that 128 columns can run over at the least pitch of 8
+constexpr int kRowsAhead = 192;
 constexpr unsigned kOob = 0x80000000u;   // a buffer offset that is out of range of every descriptor used here
 
 // The output side of a tile: descriptors of [rows x cols left] windows, stores that drop what lies outside.
@@ -248,17 +250,19 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
   // scalar: the origin, the bytes that exist behind it and the contraction that is left.
   const int lr = lane >> 3, lc = lane & 7;
   unsigned va[2], vb[2], vb1[1];     // of the two instructions of a half-tile (vb1: B1's one instruction where BN = 192)
-  int pca[2], pcb[2], pcb1[1];       // what a lane's 16-byte piece has to stay below: KC: k inside the K-tile, KS: column
+  int pca[2], pcb[2], pcb1[1];       // KC: k of the lane's 16-byte piece inside the K-tile
   constexpr int NSEG = (EPI == OG_PLAIN && BKS) ? 2 : 1;   // dx sums over two operand pairs
   constexpr bool MULTI = AKS;                              // several problems in one launch: the weights' gradients
-  struct Stream {
+  struct Stream {     // what a half-tile's copies need, all scalar; a step is a 64-bit add and a subtraction
     const char* p;    // origin of the next K-tile's half
-    int size, left;   // KC: bytes of all rows but the last (negative: no rows), k left (in pieces).  KS: last row's bytes less a
-                      // pitch, k-rows left
+    int end;          // KC: descriptor size, up to the end of the last row's pieces (rows beyond read as zero, k beyond K is masked per
+                      // lane).  KS: bytes of the last k-row less a pitch; k-rows beyond K read as zero, columns beyond the matrix run
+                      // into the next k-row and end in rows or columns of C that are not stored.
+    int left;         // KC: k left, in whole pieces; KS: k-rows left
     int seg;
   };
   Stream sa0, sa1, sb0, sb1;
-  int lda2 = 0, ldb2 = 0, am = 0, bn0 = 0, bn1 = 0;   // pitches in bytes; rows or columns left in the tile from the half's first
+  int lda2 = 0, ldb2 = 0;   // pitches in bytes
 
   auto unit = [&](unsigned t, int& pi, int& tm, int& tn, int& k0, int& k1) {   // work unit -> problem, tile, K-tiles
     const unsigned ti = t / (unsigned)p.splits;
@@ -277,14 +281,15 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
     k1 = min(p.nk, k0 + p.kps);
   };
   auto half_kc = [&](Stream& d, const h16* base, long long ld, int row0, int rows, int k0, int K) {   // rows: left from row0
+    const int K8 = (K + 7) & ~7;
     d.p = (const char*)(base + (long long)row0 * ld + k0);
-    d.size = rows > 0 ? (min(rows, 128) - 1) * (int)ld * 2 : -(1 << 30);
-    d.left = ((K + 7) & ~7) - k0;
+    d.end = rows > 0 ? (min(rows, 128) - 1) * (int)ld * 2 + K8 * 2 : 0;
+    d.left = K8 - k0;
   };
   auto half_ks = [&](Stream& d, const h16* base, long long ld, int col0, int cols, int k0, int K) {   // cols: left from col0
     d.p = (const char*)(base + (long long)k0 * ld + col0);
-    d.size = ((min(cols, 128) + 7) & ~7) * 2 - (int)ld * 2;
-    d.left = K - k0;
+    d.end = __builtin_amdgcn_readfirstlane(((max(min(cols, 128), 0) + 7) & ~7) * 2 - (int)ld * 2);   // (clamps are vector instructions)
+    d.left = cols > 0 ? K - k0 : 0;
   };
   int cur_tm = 0, cur_tn = 0;   // tile being staged
   // operand A (half h) / B (half h) of segment s from contraction index k0 on
@@ -329,46 +334,38 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
     const OpProb& q = p.prob[MULTI ? pi : 0];
     cur_tm = tm; cur_tn = tn;
     lda2 = (int)q.a[0].ld * 2; ldb2 = (int)q.b[0].ld * 2;
-    am = q.M - tm * 256;
-    bn0 = q.Nb - (og_gate(EPI) ? tn * 128 : tn * BN);
-    bn1 = og_gate(EPI) ? bn0 : bn0 - 128;
     set_a(sa0, q, 0, 0, k0 * 64); set_a(sa1, q, 1, 0, k0 * 64);
     set_b(sb0, q, 0, 0, k0 * 64); set_b(sb1, q, 1, 0, k0 * 64);
     if constexpr (MULTI) lane_offsets(pi);
   };
 
-  // one 16-byte-per-lane copy to LDS.  KC: rows beyond the matrix lie behind the descriptor's end, k beyond K is masked per lane.
-  // KS: k-rows beyond K lie behind its end, columns beyond the matrix are masked per lane.  Both arrive as zeros.
-  auto rsrc_kc = [&](const Stream& d) { return __builtin_amdgcn_make_buffer_rsrc((void*)d.p, 0, max(d.size + d.left * 2, 0), 0x00020000); };
-  auto rsrc_ks = [&](const Stream& d, int ld2) { return __builtin_amdgcn_make_buffer_rsrc((void*)d.p, 0, max(min(d.left, 64) * ld2 + d.size, 0), 0x00020000); };
-  auto copy16 = [&](__amdgpu_buffer_rsrc_t rs, unsigned vo, int piece, int lim, char* lds) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LPTR(lds), 16, (int)(piece < lim ? vo : kOob), 0, 0, 0);
+  // N copies of 16 bytes per lane to LDS (everything that does not exist arrives as zero), then one K-tile on
+  auto copies = [&](auto ks, auto count, Stream& d, int ld2, const unsigned* vo, const int* piece, char* lds) {
+    constexpr bool KS = decltype(ks)::value;
+    const int end = KS ? __builtin_amdgcn_readfirstlane(max(min(d.left, kRowsAhead) * ld2 + d.end, 0)) : d.end;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)d.p, 0, end, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < decltype(count)::value; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LPTR(lds + i * 1024), 16, (int)(KS || piece[i] < d.left ? vo[i] : kOob), 0, 0, 0);
+    d.p += KS ? (long long)64 * ld2 : 128ll;
+    d.left -= 64;
   };
-  auto step = [&](Stream& d, bool ks, int ld2) { d.p += ks ? (long long)64 * ld2 : 128ll; d.left -= 64; };
+  using AK = std::integral_constant<bool, AKS>;
+  using BK = std::integral_constant<bool, BKS>;
+  using Two = std::integral_constant<int, 2>;
   auto issue_a = [&](int h, int buf, int) {
     Stream& d = h ? sa1 : sa0;
     if constexpr (NSEG == 2) { if (d.left <= 0 && d.seg == 0) set_a(d, p.prob[0], h, 1, 0); }
-    char* l = smem + buf * TC::BUF + (h ? TC::OFF_A1 : TC::OFF_A0) + wave * 2048;
-    const __amdgpu_buffer_rsrc_t rs = AKS ? rsrc_ks(d, lda2) : rsrc_kc(d);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) copy16(rs, va[i], pca[i], AKS ? am - h * 128 : d.left, l + i * 1024);
-    step(d, AKS, lda2);
+    copies(AK{}, Two{}, d, lda2, va, pca, smem + buf * TC::BUF + (h ? TC::OFF_A1 : TC::OFF_A0) + wave * 2048);
   };
   auto issue_b0 = [&](int buf, int) {
     if constexpr (NSEG == 2) { if (sb0.left <= 0 && sb0.seg == 0) set_b(sb0, p.prob[0], 0, 1, 0); }
-    char* l = smem + buf * TC::BUF + TC::OFF_B0 + wave * 2048;
-    const __amdgpu_buffer_rsrc_t rs = BKS ? rsrc_ks(sb0, ldb2) : rsrc_kc(sb0);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) copy16(rs, vb[i], pcb[i], BKS ? bn0 : sb0.left, l + i * 1024);
-    step(sb0, BKS, ldb2);
+    copies(BK{}, Two{}, sb0, ldb2, vb, pcb, smem + buf * TC::BUF + TC::OFF_B0 + wave * 2048);
   };
   auto issue_b1 = [&](int buf, int) {
     if constexpr (NSEG == 2) { if (sb1.left <= 0 && sb1.seg == 0) set_b(sb1, p.prob[0], 1, 1, 0); }
-    char* l = smem + buf * TC::BUF + TC::OFF_B1 + wave * (NJ1 * 1024);
-    const __amdgpu_buffer_rsrc_t rs = BKS ? rsrc_ks(sb1, ldb2) : rsrc_kc(sb1);
-#pragma unroll
-    for (int i = 0; i < NJ1; ++i) copy16(rs, NJ1 == 2 ? vb[i] : vb1[0], NJ1 == 2 ? pcb[i] : pcb1[0], BKS ? bn1 : sb1.left, l + i * 1024);
-    step(sb1, BKS, ldb2);
+    copies(BK{}, std::integral_constant<int, NJ1>{}, sb1, ldb2, NJ1 == 2 ? vb : vb1, NJ1 == 2 ? pcb : pcb1,
+           smem + buf * TC::BUF + TC::OFF_B1 + wave * (NJ1 * 1024));
   };
 
   // ---- fragments
@@ -673,39 +670,43 @@ __global__ __launch_bounds__(256, 2) void op_small_kernel(const OpGemmParams p) 
       pcb[i] = ch * 8; vb[i] = (unsigned)(wr * ldb2 + ch * 16);
     }
   }
-  struct Stream { const char* p; int size, left; };
+  struct Stream { const char* p; int end, left; };   // as in op_gemm_kernel
   Stream sa, sb;
   [[maybe_unused]] int seg = 0;
   const int a_left = q.M - m0, b_left = q.Nb - n0;
-  auto set_a = [&](int s, int kk) {
-    const OpMat A = q.a[s];
-    if constexpr (AKS) sa = Stream{(const char*)(A.p + (long long)kk * A.ld + m0), ((min(a_left, 128) + 7) & ~7) * 2 - lda2, p.K[s] - kk};
-    else sa = Stream{(const char*)(A.p + (long long)m0 * A.ld + kk), a_left > 0 ? (min(a_left, 128) - 1) * lda2 : -(1 << 30), ((p.K[s] + 7) & ~7) - kk};
-    seg = s;
+  auto stream = [&](auto ks, const OpMat& A, int at, int exist, int most, int kk, int K) {
+    const int ld2 = (int)A.ld * 2, K8 = (K + 7) & ~7;
+    if constexpr (decltype(ks)::value)
+      return Stream{(const char*)(A.p + (long long)kk * A.ld + at), ((max(min(exist, most), 0) + 7) & ~7) * 2 - ld2, exist > 0 ? K - kk : 0};
+    else
+      return Stream{(const char*)(A.p + (long long)at * A.ld + kk), exist > 0 ? (min(exist, most) - 1) * ld2 + K8 * 2 : 0, K8 - kk};
   };
-  auto set_b = [&](int s, int kk) {
-    const OpMat B = og_gate(EPI) ? (wave >= 2 ? q.b[1] : q.b[0]) : q.b[s];
-    if constexpr (BKS) sb = Stream{(const char*)(B.p + (long long)kk * B.ld + n0), ((min(b_left, 64) + 7) & ~7) * 2 - ldb2, p.K[s] - kk};
-    else sb = Stream{(const char*)(B.p + (long long)n0 * B.ld + kk), b_left > 0 ? (min(b_left, og_gate(EPI) ? 32 : 64) - 1) * ldb2 : -(1 << 30), ((p.K[s] + 7) & ~7) - kk};
+  using AK = std::integral_constant<bool, AKS>;
+  using BK = std::integral_constant<bool, BKS>;
+  auto set_seg = [&](int s, int kk) {
+    sa = stream(AK{}, q.a[s], m0, a_left, 128, kk, p.K[s]);
+    sb = stream(BK{}, og_gate(EPI) ? (wave >= 2 ? q.b[1] : q.b[0]) : q.b[s], n0, b_left, og_gate(EPI) ? 32 : 64, kk, p.K[s]);
+    seg = s;
   };
   {
     const int nk0 = (p.K[0] + 63) / 64;
-    if (NSEG == 2 && k0 >= nk0) { set_a(1, (k0 - nk0) * 64); set_b(1, (k0 - nk0) * 64); }
-    else { set_a(0, k0 * 64); set_b(0, k0 * 64); }
+    if (NSEG == 2 && k0 >= nk0) set_seg(1, (k0 - nk0) * 64);
+    else set_seg(0, k0 * 64);
   }
   auto issue = [&](int stage) {
     if constexpr (NSEG == 2) {
-      if (sa.left <= 0 && seg == 0) { set_a(1, 0); set_b(1, 0); }
+      if (sa.left <= 0 && seg == 0) set_seg(1, 0);
     }
     char* l = smem + stage * kOsStage;
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)sa.p, 0, max(AKS ? min(sa.left, 64) * lda2 + sa.size : sa.size + sa.left * 2, 0), 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)sb.p, 0, max(BKS ? min(sb.left, 64) * ldb2 + sb.size : sb.size + sb.left * 2, 0), 0x00020000);
+    auto end = [](bool ks, const Stream& d, int ld2) { return ks ? __builtin_amdgcn_readfirstlane(max(min(d.left, kRowsAhead) * ld2 + d.end, 0)) : d.end; };
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)sa.p, 0, end(AKS, sa, lda2), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)sb.p, 0, end(BKS, sb, ldb2), 0x00020000);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, LPTR(l + (wave * 4 + i) * 1024), 16, (int)(pca[i] < (AKS ? a_left : sa.left) ? va[i] : kOob), 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, LPTR(l + (wave * 4 + i) * 1024), 16, (int)(AKS || pca[i] < sa.left ? va[i] : kOob), 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, LPTR(l + kOsA + (wave * 2 + i) * 1024), 16, (int)(pcb[i] < (BKS ? b_left : sb.left) ? vb[i] : kOob), 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, LPTR(l + kOsA + (wave * 2 + i) * 1024), 16, (int)(BKS || pcb[i] < sb.left ? vb[i] : kOob), 0, 0, 0);
     sa.p += AKS ? (long long)64 * lda2 : 128ll; sa.left -= 64;
     sb.p += BKS ? (long long)64 * ldb2 : 128ll; sb.left -= 64;
   };

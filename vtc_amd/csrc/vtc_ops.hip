@@ -657,7 +657,7 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, cons
   // dh and what it turns into
   const OgPlan dplan = og_plan((long long)div_up(M, 256) * div_up(F8, 192), 0.75, (long long)div_up(M, 128) * div_up(F8, 64), div_up(a.N, 64), 1, 1, 0);
   const long long parts = dplan.small ? 4ll * div_up(M, 128) : 2ll * div_up(M, 256);
-  const int row_blocks = div_up(M, 256);
+  const int row_blocks = div_up(M, kColRows);
   float* cs_f = (o->db_gate || o->db_up) || !launch ? ar.take<float>((size_t)2 * parts * F8) : nullptr;
   float* cs_n = o->db_down || !launch ? ar.take<float>((size_t)row_blocks * N8) : nullptr;
   const OutPlan xplan = plan_out(ar, M, a.K, 2 * div_up(a.F, 64));
@@ -728,7 +728,7 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, cons
       add(cs_f ? cs_f + (size_t)parts * F8 : nullptr, o->db_up, parts, F8, a.F);
       add(cs_n, o->db_down, row_blocks, N8, a.N);
       r.f16 = F16; r.out_f32 = a.bias_f32;
-      hipLaunchKernelGGL(col_reduce_kernel, dim3((unsigned)((widest + 63) / 64), (unsigned)n), dim3(256), 0, s, r);
+      hipLaunchKernelGGL(col_reduce_kernel, dim3((unsigned)((widest + 63) / 64), (unsigned)n), dim3(1024), 0, s, r);
     }
   });
   return ar.used;
