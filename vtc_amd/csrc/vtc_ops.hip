@@ -494,11 +494,19 @@ int group_of(int tiles_m, int tiles_n, double a_bytes, double w_bytes, double w_
   return r;
 }
 
-// How a product runs: tile size and K splits.  The times are measured ones (us): a K-tile of 256 x 256 x 64 takes a CU 2.2 and
-// a tile's start and epilogue 4; of 128 x 64 x 64 0.6 with two blocks on the CU, and 3; partials cross memory twice at 4 TB/s and
-// cost a launch.  Crossovers seen: 499 x 768 -> 2 x 2048 gate / up 26 us in 256-wide tiles, 11 in small ones; 31936 rows 227 / 340.
+// How a product runs: tile size and K splits, by a model of its time (us) fitted to kernel times measured at 768 x 2048.  A round is
+// as many tiles as the chip holds at once (256 of 256 rows, one per CU; 512 of 128 x 64, two per CU); `fill` is its share in use,
+// since K-tiles slow down as more CUs fetch.  Per K-tile: 1.35 + 0.75 fill for 256 x 256 (x 3/4 for 192 columns), 0.42 + 0.38 fill
+// for 128 x 64; per tile the epilogue's share.  Partials cross memory twice at 4 TB/s and cost a launch.  Measured, 256-wide / small:
+//   gate and up      512 rows 22 / 10   2048 26 / 24   4096 30 / 43   16384 109 / 183
+//   ..., slopes kept 512 rows 29 / 13   2048 33 / 31   4096 38 / 54   16384 147 / 236
+//   down             512 rows 36 / 12   2048 37 / 18   8192 43 / 39   16384  59 / 81
+//   dx               512 rows 72 / 16   2048 74 / 30   8192 86 / 82   16384 109 / 173
+//   dg and du        512 rows 36 / 13   2048 37 / 20   8192 88 / 73   16384 149 / 162
+//   weights          512 rows 31 / 22   2048 46 / 44   8192 91 / 137  16384 165 / 290
 struct OgPlan { bool small; int splits, kps; };
-OgPlan og_plan(long long tiles_big, double width, long long tiles_small, int nk, int splits_big, int splits_small, double out_elems) {
+struct OgCost { long long tiles_big, tiles_small; double width, end_big, end_small; };   // tiles; epilogue of a tile
+OgPlan og_plan(const OgCost& o, int nk, int splits_big, int splits_small, double out_elems) {
   OgPlan best{false, 1, (nk + 1) & ~1};
   double cost = 1e300;
   for (int small = 0; small < 2; ++small)
@@ -506,9 +514,10 @@ OgPlan og_plan(long long tiles_big, double width, long long tiles_small, int nk,
       int k = (nk + sp - 1) / sp;
       if (!small) k = (k + 1) & ~1;
       if ((nk + k - 1) / k != sp || (sp > 1 && k < 4)) continue;
-      const double units = (double)(small ? tiles_small : tiles_big) * sp;
-      const double rounds = std::ceil(units / (small ? 512.0 : 256.0));
-      double c = small ? rounds * (k * 0.6 + 3.0) : rounds * (k * 2.2 * width + 4.0);
+      const double cap = small ? 512.0 : 256.0, units = (double)(small ? o.tiles_small : o.tiles_big) * sp;
+      auto round = [&](double fill) { return small ? k * (0.42 + 0.38 * fill) + o.end_small : k * o.width * (1.35 + 0.75 * fill) + o.end_big; };
+      const double full = std::floor(units / cap), rest = units / cap - full;
+      double c = full * round(1.0) + (rest > 0.0 ? round(rest) : 0.0);
       if (sp > 1) c += 4.0 + sp * out_elems * 8.0 / 4.0e6;
       if (c < cost) { cost = c; best = OgPlan{small != 0, sp, k}; }
     }
@@ -562,7 +571,9 @@ template <bool F16> void gate_up(int64_t M, int K, int F, OpMat x, OpMat wg, OpM
     launch_skinny<F16, true>(p, s);
     return;
   }
-  const OgPlan plan = og_plan((long long)div_up(M, 256) * div_up(F8, 128), 1.0, (long long)div_up(M, 128) * div_up(F8, 32), div_up(K, 64), 1, 1, 0);
+  const bool save = o.s.hi != nullptr;
+  const OgPlan plan = og_plan({(long long)div_up(M, 256) * div_up(F8, 128), (long long)div_up(M, 128) * div_up(F8, 32), 1.0, save ? 12.0 : 5.0, save ? 6.0 : 4.0},
+                              div_up(K, 64), 1, 1, 0);
   OpGemmParams p{};
   p.nprob = 1;
   OpProb& q = p.prob[0];
@@ -571,14 +582,14 @@ template <bool F16> void gate_up(int64_t M, int K, int F, OpMat x, OpMat wg, OpM
   p.ntiles = q.tiles_m * q.tiles_n;
   set_k(p, plan, K);
   p.bias = bg; p.bias2 = bu; p.bias_f32 = bias_f32; p.act = act; p.s = o.s; p.a = o.a; p.ldg = F8;
-  if (o.s.hi) launch_og<F16, false, false, OG_GATE_SAVE, 256>(p, plan.small, s);
+  if (save) launch_og<F16, false, false, OG_GATE_SAVE, 256>(p, plan.small, s);
   else launch_og<F16, false, false, OG_GATE, 256>(p, plan.small, s);
 }
 
 // C = A B^T (+ bias) in 16 bits for one or two operand pairs; with few tiles in K splits whose partials lie in the workspace
 struct OutPlan { OgPlan plan; int N8; float* part; };
 OutPlan plan_out(Arena& ar, int64_t M, int N, int nk) {
-  OutPlan o{og_plan((long long)div_up(M, 256) * div_up(N, 192), 0.75, (long long)div_up(M, 128) * div_up(N, 64), nk, 1, 32, (double)M * N), up8(N), nullptr};
+  OutPlan o{og_plan({(long long)div_up(M, 256) * div_up(N, 192), (long long)div_up(M, 128) * div_up(N, 64), 0.75, 4.0, 2.0}, nk, 1, 32, (double)M * N), up8(N), nullptr};
   if (o.plan.splits > 1) o.part = ar.take<float>((size_t)o.plan.splits * M * o.N8);
   return o;
 }
@@ -655,7 +666,7 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, cons
   const OpMat wd = operand(ar, a.wd, a.N, a.F, false, s, launch);
   h16 *dg = ar.take<h16>((size_t)a.M * F8), *du = ar.take<h16>((size_t)a.M * F8);
   // dh and what it turns into
-  const OgPlan dplan = og_plan((long long)div_up(M, 256) * div_up(F8, 192), 0.75, (long long)div_up(M, 128) * div_up(F8, 64), div_up(a.N, 64), 1, 1, 0);
+  const OgPlan dplan = og_plan({(long long)div_up(M, 256) * div_up(F8, 192), (long long)div_up(M, 128) * div_up(F8, 64), 0.75, 20.0, 7.0}, div_up(a.N, 64), 1, 1, 0);
   const long long parts = dplan.small ? 4ll * div_up(M, 128) : 2ll * div_up(M, 256);
   const int row_blocks = div_up(M, kColRows);
   float* cs_f = (o->db_gate || o->db_up) || !launch ? ar.take<float>((size_t)2 * parts * F8) : nullptr;
@@ -673,7 +684,7 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, cons
   for (int i = 0; i < 3; ++i) { tb += (long long)div_up(rows[i], 256) * div_up(pitch[i], 256); ts += (long long)div_up(rows[i], 128) * div_up(pitch[i], 64); }
   const long long one = (long long)a.F * K8;
   w.split_stride = 2 * one + (long long)a.N * F8;
-  const OgPlan wplan = og_plan(tb, 1.0, ts, div_up(M, 64), 32, 32, (double)w.split_stride);
+  const OgPlan wplan = og_plan({tb, ts, 1.0, 6.0, 3.0}, div_up(M, 64), 32, 32, (double)w.split_stride);
   int tiles = 0;
   for (int i = 0; i < 3; ++i) {
     OpProb& q = w.prob[i];
