@@ -30,7 +30,9 @@ struct GnParams {
   double* sums;                 // backward: [N][C][2] sums over rows, then [N][G][2] (A / M, B / M)
   void *dw, *db;                // gradients of the affine, may be null
   long long N, L;
-  int C, G, cpg, cv, rows, chunks;   // cv = C / VEC; rows per row block (chunk)
+  int C, G, cpg, cv, rows, chunks;   // cv = C / VEC; rows per row block (chunk) of the sums, row blocks per sample
+  int arows, achunks;           // the same of the elementwise pass, which may follow the number of samples
+  int merge_here;               // forward: the elementwise pass merges the row blocks' partials itself (few of them)
   int cvb;                      // whole-sample kernels: 16-byte channel vectors of a block
   int affine_f32;               // w, b, dw, db are fp32 (else the tensors' type)
   float eps;
@@ -133,11 +135,9 @@ __device__ __forceinline__ void gn_merge(GnMoment& a, double mean, double m2, do
   a.m2 += m2 + d * d * (a.cnt * cnt / tot);
   a.cnt = tot;
 }
-__global__ __launch_bounds__(256) void gn_finalize_kernel(const GnParams p) {
-  __shared__ GnMoment sh[16][16];
-  const unsigned per = (unsigned)(p.G + 15) / 16;
-  const long long n = blockIdx.x / per;
-  const int g = (int)(blockIdx.x % per) * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
+// mean and rstd of 16 groups from g0 on, by a block of 256; stat: [16] results for the block
+__device__ __forceinline__ void gn_finalize(const GnParams& p, long long n, int g0, GnMoment (*sh)[16], float2* stat) {
+  const int in = threadIdx.x & 15, g = g0 + in, slice = threadIdx.x >> 4;
   const long long len = gn_length(p, n);
   GnMoment a{0.0, 0.0, 0.0};
   if (g < p.G) {
@@ -148,21 +148,44 @@ __global__ __launch_bounds__(256) void gn_finalize_kernel(const GnParams p) {
       gn_merge(a, t.x, t.y, (double)min((long long)p.rows, len - (long long)k * p.rows) * p.cpg);
     }
   }
-  sh[slice][threadIdx.x & 15] = a;
+  sh[slice][in] = a;
   __syncthreads();
-  if (slice || g >= p.G) return;
-  for (int i = 1; i < 16; ++i) { const GnMoment& o = sh[i][threadIdx.x]; gn_merge(a, o.mean, o.m2, o.cnt); }
-  p.mean[n * p.G + g] = (float)a.mean;
-  p.rstd[n * p.G + g] = a.cnt > 0.0 ? (float)(1.0 / sqrt(a.m2 / a.cnt + (double)p.eps)) : 0.f;
+  if (slice == 0 && g < p.G) {
+    for (int i = 1; i < 16; ++i) { const GnMoment& o = sh[i][in]; gn_merge(a, o.mean, o.m2, o.cnt); }
+    stat[in] = make_float2((float)a.mean, a.cnt > 0.0 ? (float)(1.0 / sqrt(a.m2 / a.cnt + (double)p.eps)) : 0.f);
+  }
+  __syncthreads();
 }
+__global__ __launch_bounds__(256) void gn_finalize_kernel(const GnParams p) {
+  __shared__ GnMoment sh[16][16];
+  __shared__ float2 stat[16];
+  const unsigned per = (unsigned)(p.G + 15) / 16;
+  const long long n = blockIdx.x / per;
+  const int g0 = (int)(blockIdx.x % per) * 16, g = g0 + threadIdx.x;
+  gn_finalize(p, n, g0, sh, stat);
+  if (threadIdx.x >= 16 || g >= p.G) return;
+  p.mean[n * p.G + g] = stat[threadIdx.x].x;
+  p.rstd[n * p.G + g] = stat[threadIdx.x].y;
+}
+constexpr int kGnMergeHere = 32;   // most groups whose partials the elementwise pass merges in every block
 
 // ---- y = act((x - mean) rstd w + b), row blocks again; rows behind the length become zero
 template <int DT, int VEC, int ACT>
 __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
   typedef typename OpType<DT>::T T;
-  const long long n = blockIdx.x / (unsigned)p.chunks;
-  const long long len = gn_length(p, n), r0 = (long long)(blockIdx.x % (unsigned)p.chunks) * p.rows;
-  const int rows = (int)min((long long)p.rows, p.L - r0);
+  const unsigned blk = gridDim.x - 1 - blockIdx.x;   // last rows first: they are what the statistics pass left in the last-level cache
+  const long long n = blk / (unsigned)p.achunks;
+  const long long len = gn_length(p, n), r0 = (long long)(blk % (unsigned)p.achunks) * p.arows;
+  const int rows = (int)min((long long)p.arows, p.L - r0);
+  __shared__ GnMoment sh[16][16];
+  __shared__ float2 stat[kGnMergeHere];
+  if (p.merge_here) {
+    for (int g0 = 0; g0 < p.G; g0 += 16) gn_finalize(p, n, g0, sh, stat + g0);
+    if (blk % (unsigned)p.achunks == 0 && (int)threadIdx.x < p.G) {
+      p.mean[n * p.G + threadIdx.x] = stat[threadIdx.x].x;
+      p.rstd[n * p.G + threadIdx.x] = stat[threadIdx.x].y;
+    }
+  }
   const int real = (int)max(0ll, min((long long)rows, len - r0));
   const T* x = (const T*)p.x + n * p.xn + r0 * p.xl;
   T* y = (T*)p.out + n * p.on + r0 * p.ol;
@@ -174,8 +197,9 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
       const int c = v * VEC + k, g = c / p.cpg;
-      mu[k] = p.mean[n * p.G + g];
-      a[k] = p.rstd[n * p.G + g] * gn_param<DT>(p.w, c, p.affine_f32, 1.f);
+      const float2 st = p.merge_here ? stat[g] : make_float2(p.mean[n * p.G + g], p.rstd[n * p.G + g]);
+      mu[k] = st.x;
+      a[k] = st.y * gn_param<DT>(p.w, c, p.affine_f32, 1.f);
       b[k] = gn_param<DT>(p.b, c, p.affine_f32, 0.f);
       // 16-bit inputs: the mean folded into the offset costs |mean| rstd |w| 2^-24, their own rounding is 2^11 times that
       if constexpr (DT != 0) b[k] = fmaf(-mu[k], a[k], b[k]);
@@ -266,77 +290,95 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(const GnParams p) {
   }
 }
 
-// ---- pass 2a: sums over the row blocks of a sample, fp64, 4 threads per channel
-__global__ __launch_bounds__(256) void gn_bwd_merge_kernel(const GnParams p) {
-  __shared__ double2 sh[4][64];
-  const unsigned per = (unsigned)(p.C + 63) / 64;
-  const long long n = blockIdx.x / per;
-  const int c = (int)(blockIdx.x % per) * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+// ---- pass 2: a sample's sums over its row blocks (fp64, 4 threads per channel) and its groups' A / M and B / M; a block per sample
+__global__ __launch_bounds__(1024) void gn_bwd_merge_kernel(const GnParams p) {
+  __shared__ double2 sh[4][256];
+  const long long n = blockIdx.x;
   const long long len = gn_length(p, n);
-  double s = 0.0, q = 0.0;
-  if (c < p.C) {
-    const float2* part = (const float2*)p.part + n * p.chunks * p.C + c;
-    const int live = (int)min((long long)p.chunks, (len + p.rows - 1) / p.rows);
+  const int in = threadIdx.x & 255, slice = threadIdx.x >> 8;
+  const int live = (int)min((long long)p.chunks, (len + p.rows - 1) / p.rows);
+  for (int c0 = 0; c0 < p.C; c0 += 256) {
+    const int c = c0 + in;
+    double s = 0.0, q = 0.0;
+    if (c < p.C) {
+      const float2* part = (const float2*)p.part + n * p.chunks * p.C + c;
 #pragma unroll 4
-    for (int k = slice; k < live; k += 4) {
-      const float2 t = part[(long long)k * p.C];
-      s += t.x;
-      q += t.y;
+      for (int k = slice; k < live; k += 4) {
+        const float2 t = part[(long long)k * p.C];
+        s += t.x;
+        q += t.y;
+      }
     }
+    sh[slice][in] = make_double2(s, q);
+    __syncthreads();
+    if (slice == 0 && c < p.C) {
+      for (int i = 1; i < 4; ++i) { s += sh[i][in].x; q += sh[i][in].y; }
+      p.sums[(n * p.C + c) * 2] = s;
+      p.sums[(n * p.C + c) * 2 + 1] = q;
+    }
+    __syncthreads();
   }
-  sh[slice][threadIdx.x & 63] = make_double2(s, q);
-  __syncthreads();
-  if (slice || c >= p.C) return;
-  for (int i = 1; i < 4; ++i) { s += sh[i][threadIdx.x].x; q += sh[i][threadIdx.x].y; }
-  p.sums[(n * p.C + c) * 2] = s;
-  p.sums[(n * p.C + c) * 2 + 1] = q;
+}
+// ... its groups: a wave per group (the blocks above have ended: their sums are visible)
+template <int DT>
+__global__ __launch_bounds__(256) void gn_bwd_groups_kernel(const GnParams p) {
+  const int lane = threadIdx.x & 63;
+  const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);   // n * G + g
+  if (i >= p.N * p.G) return;
+  const long long n = i / p.G;
+  const int g = (int)(i - n * p.G);
+  double a = 0.0, b = 0.0;
+  for (int c = lane; c < p.cpg; c += 64) {
+    const int ch = g * p.cpg + c;
+    const double w = gn_param<DT>(p.w, ch, p.affine_f32, 1.f);
+    a += w * p.sums[(n * p.C + ch) * 2];
+    b += w * p.sums[(n * p.C + ch) * 2 + 1];
+  }
+  a = wave_sum_d(a);
+  b = wave_sum_d(b);
+  const double m = (double)gn_length(p, n) * p.cpg;
+  if (lane == 0) {
+    double* o = p.sums + p.N * p.C * 2 + i * 2;
+    o[0] = m > 0 ? a / m : 0.0;
+    o[1] = m > 0 ? b / m : 0.0;
+  }
 }
 
-// ---- pass 2b: the group sums of every sample (blocks 0 .. N G / 4 - 1, a wave per group) and the affine's gradients
-template <int DT>
-__global__ __launch_bounds__(256) void gn_bwd_groups_kernel(const GnParams p, long long group_blocks) {
+// ---- the affine's gradients: sums over the samples, 64 channels by 256 threads (4 per channel), in a fixed order
+template <int DT> __device__ __forceinline__ void gn_affine_grads(const GnParams& p, int c0, double2 (*sh)[64]) {
   typedef typename OpType<DT>::T T;
-  const int lane = threadIdx.x & 63;
-  if ((long long)blockIdx.x < group_blocks) {
-    const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);   // n * G + g
-    if (i >= p.N * p.G) return;
-    const long long n = i / p.G;
-    const int g = (int)(i - n * p.G);
-    double a = 0.0, b = 0.0;
-    for (int c = lane; c < p.cpg; c += 64) {
-      const int ch = g * p.cpg + c;
-      const double w = gn_param<DT>(p.w, ch, p.affine_f32, 1.f);
-      a += w * p.sums[(n * p.C + ch) * 2];
-      b += w * p.sums[(n * p.C + ch) * 2 + 1];
-    }
-    a = wave_sum_d(a);
-    b = wave_sum_d(b);
-    const double m = (double)gn_length(p, n) * p.cpg;
-    if (lane == 0) {
-      double* o = p.sums + p.N * p.C * 2 + i * 2;
-      o[0] = m > 0 ? a / m : 0.0;
-      o[1] = m > 0 ? b / m : 0.0;
-    }
-    return;
-  }
-  const int c = (int)(((long long)blockIdx.x - group_blocks) * 256 + threadIdx.x);
-  if (c >= p.C) return;
+  const int in = threadIdx.x & 63, slice = threadIdx.x >> 6, c = c0 + in;
   double s = 0.0, q = 0.0;
-  for (long long n = 0; n < p.N; ++n) {
-    s += p.sums[(n * p.C + c) * 2];
-    q += p.sums[(n * p.C + c) * 2 + 1];
-  }
+  if (c < p.C)
+#pragma unroll 4
+    for (long long n = slice; n < p.N; n += 4) {
+      s += p.sums[(n * p.C + c) * 2];
+      q += p.sums[(n * p.C + c) * 2 + 1];
+    }
+  sh[slice][in] = make_double2(s, q);
+  __syncthreads();
+  if (slice || c >= p.C) return;
+  for (int i = 1; i < 4; ++i) { s += sh[i][in].x; q += sh[i][in].y; }
   if (p.db) { if (p.affine_f32) ((float*)p.db)[c] = (float)s; else ((T*)p.db)[c] = op_store<DT>((float)s); }
   if (p.dw) { if (p.affine_f32) ((float*)p.dw)[c] = (float)q; else ((T*)p.dw)[c] = op_store<DT>((float)q); }
+}
+template <int DT>
+__global__ __launch_bounds__(256) void gn_affine_grads_kernel(const GnParams p) {
+  __shared__ double2 sh[4][64];
+  gn_affine_grads<DT>(p, blockIdx.x * 64, sh);
 }
 
 // ---- pass 3: dx
 template <int DT, int VEC, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnParams p) {
   typedef typename OpType<DT>::T T;
-  const long long n = blockIdx.x / (unsigned)p.chunks;
-  const long long len = gn_length(p, n), r0 = (long long)(blockIdx.x % (unsigned)p.chunks) * p.rows;
-  const int rows = (int)min((long long)p.rows, p.L - r0);
+  __shared__ double2 sh[4][64];
+  const unsigned row_blocks = (unsigned)(p.N * p.achunks);
+  if (blockIdx.x >= row_blocks) { gn_affine_grads<DT>(p, (int)(blockIdx.x - row_blocks) * 64, sh); return; }
+  const unsigned blk = row_blocks - 1 - blockIdx.x;   // see gn_apply_kernel
+  const long long n = blk / (unsigned)p.achunks;
+  const long long len = gn_length(p, n), r0 = (long long)(blk % (unsigned)p.achunks) * p.arows;
+  const int rows = (int)min((long long)p.arows, p.L - r0);
   const int real = (int)max(0ll, min((long long)rows, len - r0));
   const T* x = (const T*)p.x + n * p.xn + r0 * p.xl;
   const T* dy = (const T*)p.dy + n * p.dn + r0 * p.dl;

@@ -248,7 +248,7 @@ int gn_check(const char* what, int dtype, int affine_f32, const vtc_rows3* const
   int rows, chunks;
   if (L > (long long)256 * 0x7ffffff) return fail_handleless(VTC_ERR_ARG, "%s: too many rows", what);
   gn_shape(L, &rows, &chunks);
-  if (N * (long long)chunks > 0x7fffffff || N * (long long)((C + 7) / 8) > 0x7fffffff) return fail_handleless(VTC_ERR_ARG, "%s: too many rows", what);
+  if (N * ((L + 3) / 4) > 0x7fff0000 || N * (long long)chunks > 0x7fffffff || N * (long long)((C + 7) / 8) > 0x7fffffff) return fail_handleless(VTC_ERR_ARG, "%s: too many rows", what);
   for (int i = 0; i < n_t; ++i) {
     const vtc_rows3& t = *ts[i];
     if (!t.p) return fail_handleless(VTC_ERR_ARG, "%s: null tensor", what);
@@ -291,6 +291,9 @@ GnParams gn_params(int64_t N, int64_t L, int C, int G, const void* w, const void
   p.N = N; p.L = L; p.C = C; p.G = G; p.cpg = C / G;
   p.w = w; p.b = b; p.affine_f32 = affine_f32; p.length = lengths;
   gn_shape(L, &p.rows, &p.chunks);
+  // the elementwise pass: ~2000 blocks where there are rows for it, at least 4 rows and at most 64
+  p.arows = (int)std::min<long long>(64, std::max<long long>(4, N * L / 2048));
+  p.achunks = (int)((L + p.arows - 1) / p.arows);
   return p;
 }
 long long eff(long long stride, long long count) { return count > 1 ? stride : 0; }
@@ -341,14 +344,17 @@ extern "C" int vtc_group_norm_act(int device, int dtype, const vtc_rows3* x, con
     return launched("group norm");
   }
   const unsigned blocks = (unsigned)(batch * p.chunks);
+  // few partials and few blocks to repeat it in: the elementwise pass merges them itself, a launch less (5 x 1531 rows, 3 groups:
+  // 12 us instead of 6 + 9; with 63 row blocks of 32 groups it would cost 64 x 3999 rows 20 us)
+  p.merge_here = groups <= kGnMergeHere && p.chunks * groups <= 256 && batch * p.achunks <= 4096;
   by_vec(dtype, vec, [&](auto d, auto v) {
     constexpr int DT = decltype(d)::value, VEC = decltype(v)::value;
     const size_t lds = ((size_t)2 * channels + 256 * 2 * VEC) * 4;
     hipLaunchKernelGGL((gn_stats_kernel<DT, VEC>), dim3(blocks), dim3(256), lds, s, p);
-    hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(batch * ((groups + 15) / 16))), dim3(256), 0, s, p);
+    if (!p.merge_here) hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(batch * ((groups + 15) / 16))), dim3(256), 0, s, p);
     by_act(act, [&](auto a) {
       if constexpr (decltype(a)::value != ACT_SIGMOID)
-        hipLaunchKernelGGL((gn_apply_kernel<DT, VEC, decltype(a)::value>), dim3(blocks), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((gn_apply_kernel<DT, VEC, decltype(a)::value>), dim3((unsigned)(batch * p.achunks)), dim3(256), 0, s, p);
     });
   });
   return launched("group norm");
@@ -366,11 +372,11 @@ extern "C" int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows
   GnParams p = gn_params(batch, length, channels, groups, weight, bias, affine_f32, lengths);
   p.dw = dweight; p.db = dbias;
   hipStream_t s = (hipStream_t)stream;
-  const unsigned grad_blocks = (unsigned)((channels + 255) / 256);
+  const unsigned grad_blocks = (unsigned)((channels + 63) / 64);
   if (batch == 0 || length == 0) {   // the affine's gradients are sums over nothing
     p.N = 0;
     if (dweight || dbias) by_vec(dtype, 1, [&](auto d, auto) {
-      hipLaunchKernelGGL((gn_bwd_groups_kernel<decltype(d)::value>), dim3(grad_blocks), dim3(256), 0, s, p, 0ll);
+      hipLaunchKernelGGL((gn_affine_grads_kernel<decltype(d)::value>), dim3(grad_blocks), dim3(256), 0, s, p);
     });
     return launched("group norm backward");
   }
@@ -397,7 +403,7 @@ extern "C" int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows
         else if (nv <= 4) hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 4, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
         else hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 8, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
       }
-      if (dweight || dbias) hipLaunchKernelGGL((gn_bwd_groups_kernel<DT>), dim3(grad_blocks), dim3(256), 0, s, p, 0ll);
+      if (dweight || dbias) hipLaunchKernelGGL((gn_affine_grads_kernel<DT>), dim3(grad_blocks), dim3(256), 0, s, p);
     }); });
     return launched("group norm backward");
   }
@@ -409,9 +415,10 @@ extern "C" int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows
       constexpr int ACT = decltype(a)::value;
       if constexpr (ACT != ACT_SIGMOID) {
         hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, VEC, ACT>), dim3(blocks), dim3(256), 0, s, p);
-        hipLaunchKernelGGL(gn_bwd_merge_kernel, dim3((unsigned)(batch * ((channels + 63) / 64))), dim3(256), 0, s, p);
-        hipLaunchKernelGGL((gn_bwd_groups_kernel<DT>), dim3((unsigned)(group_blocks + grad_blocks)), dim3(256), 0, s, p, group_blocks);
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, VEC, ACT>), dim3(blocks), dim3(256), 0, s, p);
+        hipLaunchKernelGGL(gn_bwd_merge_kernel, dim3((unsigned)batch), dim3(1024), 0, s, p);
+        hipLaunchKernelGGL((gn_bwd_groups_kernel<DT>), dim3((unsigned)group_blocks), dim3(256), 0, s, p);
+        // the blocks behind the rows' sum the affine's gradients
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, VEC, ACT>), dim3((unsigned)(batch * p.achunks + (dweight || dbias ? grad_blocks : 0))), dim3(256), 0, s, p);
       }
     });
   });

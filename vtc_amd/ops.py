@@ -160,7 +160,9 @@ def _rotary_call(tensors, spec: Rotary, positions, offset: int, inverse: bool, o
         if sx[-1] != 1 and not empty:
             raise ValueError("rotary: the elements of a head must be contiguous")
         if outs is None:
-            y = torch.empty(shape, dtype=x.dtype, device=x.device)
+            y = torch.empty_like(x)
+            if y.stride(-1) != 1:   # (sizes of one leave empty_like's order open)
+                y = torch.empty(shape, dtype=x.dtype, device=x.device)
         else:
             y = outs[i]
             _same("rotary", x0, "out", y)
@@ -278,7 +280,7 @@ def _rows3(t):
 
 def _gn_out(what, x, out):
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
     _same(what, x, "out", out)
     if out.shape != x.shape or (out.numel() and out.stride(2) != 1):
         raise ValueError(f"{what}: out must have shape {tuple(x.shape)} with contiguous channels")
@@ -420,7 +422,7 @@ def gated_ffn_forward(x: torch.Tensor, w_gate, w_up, w_down, b_gate=None, b_up=N
     index, dt, f32, k, f, n = _ffn_args(what, x, w_gate, w_up, w_down, (b_gate, b_up, b_down), act)
     rows = _rows2(x)
     m = rows.shape[0]
-    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format) if n == k else torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
     so = _library()
     size = so.vtc_gated_ffn_workspace(m, k, f, n, 0)
     if size < 0:
