@@ -142,7 +142,7 @@ def _q(x: torch.Tensor, emulate_bf16: bool) -> torch.Tensor:
 def rotate_heads(x: torch.Tensor, rotary) -> torch.Tensor:
     """Rotary positions 0, 1, .. on (batch, heads, frames, 64) from a rotation's frequencies (64 bits), layout and amplitude."""
     r = rotary.rotary_dim
-    a = torch.arange(x.shape[2], dtype=torch.float64)[:, None] * torch.from_numpy(np.asarray(rotary.frequency))
+    a = torch.arange(x.shape[2], dtype=torch.float64)[:, None] * torch.tensor(np.asarray(rotary.frequency))
     c, s = (torch.cos(a) * rotary.amplitude).float(), (torch.sin(a) * rotary.amplitude).float()
     first = slice(0, r // 2) if rotary.layout == "half" else slice(0, r, 2)
     second = slice(r // 2, r) if rotary.layout == "half" else slice(1, r, 2)

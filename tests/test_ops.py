@@ -33,7 +33,7 @@ def close(got, want, tol, what=""):
 # --------------------------------------------------------------------------------------------- rotary
 def rotary_64(x, spec, pos, inverse=False):
     x = x.double().cpu()
-    a = pos.double().cpu()[..., None] * torch.from_numpy(spec.frequency)
+    a = pos.double().cpu()[..., None] * torch.tensor(spec.frequency)
     c, s = (torch.cos(a) * spec.amplitude)[..., None, :], (torch.sin(a) * spec.amplitude * (-1 if inverse else 1))[..., None, :]
     y, r = x.clone(), spec.rotary_dim
     if spec.layout == "half":
@@ -53,7 +53,7 @@ def check_rotary(got, x, spec, pos, inverse=False):
     # cos and sin are within 2^-22 (argument 2^-24 pi / 4, five fp32 operations), each product and the sum round once more.
     # The angle itself: the definition rounds position * frequency to 53 bits and the library rounds the frequency in turns, each
     # 2^-53 of the angle, which is 1e-6 rad at the 2^33 rad of the farthest positions here
-    angle = (pos.double().cpu().abs()[..., None] * torch.from_numpy(np.abs(spec.frequency)))[..., None, :]
+    angle = (pos.double().cpu().abs()[..., None] * torch.tensor(np.abs(spec.frequency)))[..., None, :]
     angle = torch.cat([angle] * 2, -1) if spec.layout == "half" else torch.stack([angle] * 2, -1).flatten(-2)
     tol = half_step(x.dtype, want)[..., :r] + mag * spec.amplitude * (2.0 ** -21 + angle * 2.0 ** -52)
     close(got[..., :r], want[..., :r], tol, "rotated")
@@ -725,16 +725,81 @@ def test_gated_ffn_in_a_graph():
         (out[0].float() * 2).sum().item()
 
 
+@gpu
+def test_calls_on_two_streams_at_once_do_not_disturb_each_other():
+    """Each call brings its own workspace: interleaved calls on two streams give the bits of lone ones."""
+    g = torch.Generator(device="cuda").manual_seed(31)
+    sets = []
+    for i in range(2):
+        x, w, b, dy = make_ffn(torch.float16, 900, 264, 520, 264, True, seed=i)
+        n = torch.randn((4, 3000, 48), generator=g, device="cuda").half()
+        sets.append((x, w, b, dy, n))
+
+    def work(x, w, b, dy, n):
+        y, saved = ops.gated_ffn_forward(x, *w, *b, save=True)
+        out = (y,) + ops.gated_ffn_backward(dy, x, *w, saved)
+        z, m, r = ops.group_norm_act_forward(n, 3, act="silu")
+        return out + (z, ops.group_norm_act_backward(n, n, 3, m, r, act="silu")[0], ops.rotary(z.view(4, 3000, 3, 16), ops.Rotary(16)))
+
+    want = [[t.clone() for t in work(*s)] for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(work(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, c) for a, c in zip(out, want[i]))
+
+
+@gpu
+def test_rotary_and_group_norm_beyond_32_bit_offsets():
+    """More than 2^31 elements: the last rows are those of a call on them alone."""
+    spec = ops.Rotary(64)
+    x = torch.zeros((1, 130_000, 130, 128), dtype=torch.float16, device="cuda")
+    tail = torch.randn((1, 40, 130, 128), device="cuda").half()
+    x[:, -40:] = tail
+    y = ops.rotary(x, spec)
+    assert x.numel() > 2 ** 31 and torch.equal(y[:, -40:], ops.rotary(tail, spec, offset=130_000 - 40)) and not y[:, :40].any()
+    del x, y
+    z = torch.zeros((3, 1_450_000, 512), dtype=torch.bfloat16, device="cuda")
+    z[2].normal_()
+    y, m, r = ops.group_norm_act_forward(z, 16, act="gelu")
+    y2, m2, r2 = ops.group_norm_act_forward(z[2:], 16, act="gelu")
+    assert z.numel() > 2 ** 31 and torch.equal(y[2:], y2) and torch.equal(r[2:], r2) and not y[:2].any()
+    assert abs(float(y2.float().mean()) - 0.2821) < 1e-3      # E[gelu(standard normal)] = 1 / (2 sqrt(pi)); 7e8 values
+    del y
+    dx, _, _ = ops.group_norm_act_backward(z, z, 16, m, r, act="gelu")
+    assert torch.equal(dx[2:], ops.group_norm_act_backward(z[2:], z[2:], 16, m2, r2, act="gelu")[0])
+
+
+@gpu
+def test_rotary_between_columns_of_one_buffer():
+    """Input and output interleaved in the rows of one buffer share no element and are taken; shared ones are refused."""
+    g = torch.Generator(device="cuda").manual_seed(33)
+    rows = torch.randn((2, 30, 4 * 64 * 2), generator=g, device="cuda").half()
+    x, y = rows[..., :256].unflatten(-1, (4, 64)), rows[..., 256:].unflatten(-1, (4, 64))
+    keep = x.clone()
+    ops.rotary(x, ops.Rotary(64), out=y)
+    assert torch.equal(x, keep)
+    check_rotary(y, keep, ops.Rotary(64), torch.arange(30).expand(2, 30))
+    with pytest.raises(L.VtcError, match="overlap"):
+        ops.rotary(x, ops.Rotary(64), out=rows[..., 192:448].unflatten(-1, (4, 64)))
+
+
 def _ffn_c(backward=False, **over):
     a = dict(dtype=1, m=100, k=64, f=128, n=64, f32=0, act=2, x=L.VtcMat(1 << 20, 64), wg=L.VtcMat(2 << 20, 64), wu=L.VtcMat(3 << 20, 64),
              wd=L.VtcMat(4 << 20, 128), y=L.VtcMat(5 << 20, 64), saved=6 << 20, saved_size=1 << 20, ws=8 << 20, size=1 << 30, dx=7 << 20, dx_row=64, dw=1 << 28,
-             dw2=1 << 28)
+             dw2=(1 << 28) + (1 << 20), dw3=(1 << 28) + (2 << 20))
     a.update(over)
     ref = lambda s: None if s is None else C.byref(s)  # noqa: E731
     so = L.load()
     mats = [ref(a[n]) for n in ("x", "wg", "wu", "wd")]
     if backward:
-        grads = L.VtcFfnGrads(a["dx"], a["dx_row"], a["dw"], a["dw2"], a["dw"])
+        grads = L.VtcFfnGrads(a["dx"], a["dx_row"], a["dw"], a["dw2"], a["dw3"])
         rc = so.vtc_gated_ffn_backward(0, a["dtype"], a["m"], a["k"], a["f"], a["n"], ref(a["y"]), *mats, a["saved"], a["saved_size"], a["f32"],
                                        C.byref(grads), a["ws"], a["size"], None)
     else:
@@ -759,7 +824,9 @@ def test_gated_ffn_refusals_of_the_library(backward, over, text, code):
 def test_gated_ffn_refusals_of_one_direction():
     for backward, over, text in ((False, dict(y=L.VtcMat((1 << 20) + 64, 64)), "overlaps x"), (False, dict(act=4), "activation"), (True, dict(dx=1 << 20), "overlaps"),
                                  (True, dict(dx=5 << 20), "overlaps"), (True, dict(dx_row=63), "pitch"), (True, dict(dw=None), "go together"),
-                                 (True, dict(m=0), "no rows"), (True, dict(dx=(7 << 20) + 1), "aligned")):
+                                 (True, dict(m=0), "no rows"), (True, dict(dx=(7 << 20) + 1), "aligned"), (False, dict(y=L.VtcMat(4 << 20, 64)), "overlaps w_down"),
+                                 (True, dict(dw=2 << 20), "overlaps w_gate"), (True, dict(dw2=1 << 28), "overlaps dw_gate"),
+                                 (True, dict(dw3=5 << 20), "overlaps dy"), (False, dict(m=1 << 30, f=1 << 18, wd=L.VtcMat(4 << 20, 1 << 18)), "too many")):
         rc, msg = _ffn_c(backward, **over)
         assert rc == L.ERR_ARG and text in msg, (rc, msg)
     so = L.load()

@@ -166,7 +166,8 @@ extern "C" int vtc_rotary_heads(int device, int dtype, const vtc_rotary* r, int6
     if (int rc = rotary_check_tensor(name, t, *r, batch, length, dtype, &in_place)) return rc;
     ends[i][0] = end_of(t.x, {{batch, t.x_batch}, {length, t.x_row}, {t.heads, t.x_head}}, r->head_dim, esize(dtype));
     ends[i][1] = end_of(t.y, {{batch, t.y_batch}, {length, t.y_row}, {t.heads, t.y_head}}, r->head_dim, esize(dtype));
-    if (!in_place && overlap(t.x, ends[i][0], t.y, ends[i][1]))
+    if (!in_place && !apart(t.x, ends[i][0], t.x_batch, t.x_row, (t.heads - 1) * t.x_head + r->head_dim, t.y, ends[i][1], t.y_batch, t.y_row,
+                            (t.heads - 1) * t.y_head + r->head_dim, batch, esize(dtype)))
       return fail_handleless(VTC_ERR_ARG, "rotary: input and output of the %s overlap without being the same", name);
     copy_tail = copy_tail || !in_place;
     p.t[i] = RotaryTensor{t.x, t.y, t.x_batch, t.x_row, t.x_head, t.y_batch, t.y_row, t.y_head, t.heads};
@@ -466,12 +467,33 @@ int ffn_check(const char* what, const FfnArgs& a) {
   if (a.M < 0 || a.M > (1ll << 31) - 256) return fail_handleless(VTC_ERR_ARG, "%s: %lld rows not in 0..2^31 - 256", what, (long long)a.M);
   for (int64_t d : {(int64_t)a.K, (int64_t)a.F, (int64_t)a.N})
     if (d < 1 || d > kFfnMaxDim) return fail_handleless(VTC_ERR_ARG, "%s: width %lld not in 1..%lld", what, (long long)d, (long long)kFfnMaxDim);
+  // tiles of a launch are counted in 32 bits (the smallest are 128 x 32; with two sides at the limit of 2^18 rows are limited too)
+  const int64_t widest = std::max({a.K, a.F, a.N});
+  if ((a.M / 128 + 1) * (widest / 32 + 1) > (1ll << 30) || 3 * (widest / 128 + 1) * (widest / 64 + 1) > (1ll << 25))
+    return fail_handleless(VTC_ERR_ARG, "%s: %lld rows of width %lld are too many", what, (long long)a.M, (long long)widest);
+  for (const void* b : {a.bg, a.bu, a.bd})
+    if ((uintptr_t)b % (a.bias_f32 ? 4 : 2)) return fail_handleless(VTC_ERR_ARG, "%s: a bias is not aligned to its type", what);
   if (int rc = ffn_check_mat(what, "x", a.x, a.M, a.K)) return rc;
   if (int rc = ffn_check_mat(what, "w_gate", a.wg, a.F, a.K)) return rc;
   if (int rc = ffn_check_mat(what, "w_up", a.wu, a.F, a.K)) return rc;
   if (int rc = ffn_check_mat(what, "w_down", a.wd, a.N, a.F)) return rc;
   return VTC_OK;
 }
+// What a call writes (all of `outs`) shares no memory with what it reads, nor with the rest of what it writes.
+struct Span { const char* name; const void* p; const char* end; };
+int ffn_apart(const char* what, std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
+  for (auto o = outs.begin(); o != outs.end(); ++o) {
+    if (!o->p) continue;
+    for (auto i = ins.begin(); i != ins.end(); ++i)
+      if (i->p && overlap(o->p, o->end, i->p, i->end)) return fail_handleless(VTC_ERR_ARG, "%s: %s overlaps %s", what, o->name, i->name);
+    for (auto i = outs.begin(); i != o; ++i)
+      if (i->p && overlap(o->p, o->end, i->p, i->end)) return fail_handleless(VTC_ERR_ARG, "%s: %s overlaps %s", what, o->name, i->name);
+  }
+  return VTC_OK;
+}
+Span span(const char* name, const void* p, long long rows, long long pitch, long long cols, int es) { return {name, p, p ? end_of(p, {{rows, pitch}}, cols, es) : nullptr}; }
+Span span(const char* name, const vtc_mat* m, long long rows, long long cols) { return span(name, m->p, rows, m->row, cols, 2); }
+
 bool pieces_ok(const vtc_mat* m, int cols) { return cols % 8 == 0 && m->row % 8 == 0 && (uintptr_t)m->p % 16 == 0; }
 
 // An operand made of aligned 16-byte pieces: the caller's memory where it is, a padded copy in the workspace where it is not.
@@ -788,8 +810,10 @@ extern "C" int vtc_gated_ffn(int device, int dtype, int64_t rows, int32_t width,
   if (int rc = ffn_check(what, a)) return rc;
   if (int rc = ffn_check_mat(what, "y", y, rows, out_width)) return rc;
   if (rows == 0) return VTC_OK;
-  const char* y_end = end_of(y->p, {{rows, y->row}}, out_width, 2);
-  if (overlap(x->p, end_of(x->p, {{rows, x->row}}, width, 2), y->p, y_end)) return fail_handleless(VTC_ERR_ARG, "%s: y overlaps x", what);
+  const int bs = bias_f32 ? 4 : 2;
+  if (int rc = ffn_apart(what, {span("y", y, rows, out_width)}, {span("x", x, rows, width), span("w_gate", w_gate, inner, width), span("w_up", w_up, inner, width),
+                                span("w_down", w_down, out_width, inner), span("b_gate", b_gate, 1, 0, inner, bs), span("b_up", b_up, 1, 0, inner, bs),
+                                span("b_down", b_down, 1, 0, out_width, bs)})) return rc;
   const int64_t need_s = vtc_gated_ffn_saved(rows, inner);
   if (saved && saved_bytes < need_s) return fail_handleless(VTC_ERR_CAPACITY, "%s: the saved buffer holds %lld bytes, %lld needed", what, (long long)saved_bytes, (long long)need_s);
   const size_t need = ffn_forward(a, nullptr, saved, nullptr, false, nullptr);
@@ -817,10 +841,15 @@ extern "C" int vtc_gated_ffn_backward(int device, int dtype, int64_t rows, int32
     if ((uintptr_t)p % 2) return fail_handleless(VTC_ERR_ARG, "%s: a gradient is not aligned to its type", what);
   if (grads->dx) {
     if (grads->dx_row < width || grads->dx_row > kMaxPitch) return fail_handleless(VTC_ERR_ARG, "%s: dx has a row pitch of %lld for %d columns", what, (long long)grads->dx_row, width);
-    const char* e = end_of(grads->dx, {{rows, grads->dx_row}}, width, 2);
-    if (overlap(x->p, end_of(x->p, {{rows, x->row}}, width, 2), grads->dx, e) || overlap(dy->p, end_of(dy->p, {{rows, dy->row}}, out_width, 2), grads->dx, e))
-      return fail_handleless(VTC_ERR_ARG, "%s: dx overlaps x or dy", what);
   }
+  const int bs = bias_f32 ? 4 : 2;
+  for (const void* p : {grads->db_gate, grads->db_up, grads->db_down})
+    if ((uintptr_t)p % bs) return fail_handleless(VTC_ERR_ARG, "%s: a gradient is not aligned to its type", what);
+  if (int rc = ffn_apart(what, {span("dx", grads->dx, rows, grads->dx_row, width, 2), span("dw_gate", grads->dw_gate, inner, width, width, 2),
+                                span("dw_up", grads->dw_up, inner, width, width, 2), span("dw_down", grads->dw_down, out_width, inner, inner, 2),
+                                span("db_gate", grads->db_gate, 1, 0, inner, bs), span("db_up", grads->db_up, 1, 0, inner, bs), span("db_down", grads->db_down, 1, 0, out_width, bs)},
+                         {span("x", x, rows, width), span("dy", dy, rows, out_width), span("w_gate", w_gate, inner, width), span("w_up", w_up, inner, width),
+                          span("w_down", w_down, out_width, inner)})) return rc;
   const int64_t need_s = vtc_gated_ffn_saved(rows, inner);
   if (!saved || saved_bytes < need_s) return fail_handleless(VTC_ERR_CAPACITY, "%s: the saved buffer of the forward call holds %lld bytes, %lld needed", what, (long long)saved_bytes, (long long)need_s);
   const size_t need = ffn_backward(a, dy, nullptr, grads, nullptr, false, nullptr);
