@@ -465,55 +465,55 @@ constexpr int kGnMaxCvb = 8;
 constexpr int kGnSlabThreads = 512;
 
 // Block sums of NQ values per channel vector: v in every thread on entry, tot[vector * NQ + k] on exit.  Fixed order.
-template <int NQ> __device__ __forceinline__ void gn_block_sums(const float (&v)[NQ], int cvb, float* red, float* tot) {
-  const int row = threadIdx.x >> 4, in = threadIdx.x & 15, outs = cvb * NQ;
+template <int NQ, int THREADS> __device__ __forceinline__ void gn_block_sums(const float (&v)[NQ], int cvb, float* red, float* tot) {
+  const int row = threadIdx.x >> 4, in = threadIdx.x & 15, outs = cvb * NQ;   // rows of 16 lanes
 #pragma unroll
   for (int k = 0; k < NQ; ++k) {
     const float s = gn_row_sum(v[k], cvb);
-    if (in < cvb) red[row * outs + in * NQ + k] = s;   // 32 rows of 16 lanes
+    if (in < cvb) red[row * outs + in * NQ + k] = s;
   }
   __syncthreads();
-  const int o = threadIdx.x >> 2, part = threadIdx.x & 3;   // at most 128 sums, 4 threads each
+  constexpr int P = THREADS / 128;              // threads per sum (at most 128 sums), 8 rows each
+  const int o = threadIdx.x / P, part = threadIdx.x % P;
   float s = 0.f;
   if (o < outs)
 #pragma unroll
     for (int r = 0; r < 8; ++r) s += red[(part * 8 + r) * outs + o];
-  s += __shfl_xor(s, 1);
-  s += __shfl_xor(s, 2);
+#pragma unroll
+  for (int d = 1; d < P; d <<= 1) s += __shfl_xor(s, d);
   if (o < outs && part == 0) tot[o] = s;
   __syncthreads();
 }
 
-template <int DT, int NV, int ACT>
-__global__ __launch_bounds__(kGnSlabThreads, 4) void gn_slab_kernel(const GnParams p) {
+template <int DT, int NV, int ACT, int THREADS>
+__global__ __launch_bounds__(THREADS, 4) void gn_slab_kernel(const GnParams p) {
   typedef typename OpType<DT>::T T;
   constexpr int VEC = GnVec<DT>::VEC;
-  __shared__ float red[kGnSlabThreads / 16 * kGnMaxCvb * VEC], tot[kGnMaxCvb * VEC], gmean[kGnMaxCvb * VEC], grstd[kGnMaxCvb * VEC];
-  const int cvb = p.cvb, bc = cvb * VEC, bundles = p.C / bc, ngb = bc / p.cpg;
+  __shared__ float red[THREADS / 16 * kGnMaxCvb * VEC], tot[kGnMaxCvb * VEC], gmean[kGnMaxCvb * VEC], grstd[kGnMaxCvb * VEC];
+  const int cvb = p.cvb, bc = cvb * VEC, bundles = p.C / bc;
+  const int sh = 31 - __builtin_clz(p.cpg), ngb = bc >> sh;   // groups divide a power of two here: they are powers of two
   const unsigned blk = xcd_remap(blockIdx.x, gridDim.x);
   const long long n = blk / (unsigned)bundles;
   const int c_base = (int)(blk % (unsigned)bundles) * bc;
-  const int v = threadIdx.x & (cvb - 1), r0 = threadIdx.x / cvb, dr = kGnSlabThreads / cvb;
+  const int v = threadIdx.x & (cvb - 1), r0 = threadIdx.x / cvb, dr = THREADS / cvb;
   const long long len = gn_length(p, n);
   const int real = (int)len;
   const T* x = (const T*)p.x + n * p.xn + c_base + v * VEC;
   T* y = (T*)p.out + n * p.on + c_base + v * VEC;
   u16x8 data[NV];
+  {
+    const T* src = x + r0 * p.xl;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int r = r0 + i * dr;
-    if (r < real) data[i] = *(const u16x8*)(x + r * p.xl);
+    for (int i = 0; i < NV; ++i, src += dr * p.xl)
+      if (r0 + i * dr < real) data[i] = *(const u16x8*)src;
   }
   // One pass as the rows arrive: sums of x - f and (x - f)^2, f = the thread's own first value.  A set that holds its own shift
   // cancels at most a factor of its size (NV rows), whatever the data; the threads' means and M2 then merge by Chan's formula.
-  float s[VEC], q[VEC], first[VEC], base[VEC];
+  float s[VEC], q[VEC], first[VEC];
   const int cnt = r0 < real ? (real - r0 + dr - 1) / dr : 0;   // rows of this thread
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) s[k] = q[k] = first[k] = base[k] = 0.f;
-  if (cnt > 0) {
-    GnVec<DT>::unpack(*(const u16x8*)x, base);                 // the channels' values in row 0: the reference of every sum below
-    GnVec<DT>::unpack(data[0], first);
-  }
+  for (int k = 0; k < VEC; ++k) s[k] = q[k] = first[k] = 0.f;
+  if (cnt > 0) GnVec<DT>::unpack(data[0], first);
 #pragma unroll
   for (int i = 1; i < NV; ++i)
     if (r0 + i * dr < real) {
@@ -521,37 +521,46 @@ __global__ __launch_bounds__(kGnSlabThreads, 4) void gn_slab_kernel(const GnPara
       GnVec<DT>::unpack(data[i], f);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) { const float d = f[k] - first[k]; s[k] += d; q[k] = fmaf(d, d, q[k]); }
+      __builtin_amdgcn_sched_barrier(0);
     }
   const float fc = (float)cnt, ic = cnt > 0 ? 1.f / fc : 0.f;
   float v0[VEC];
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) v0[k] = fmaf(fc, first[k] - base[k], s[k]);
-  gn_block_sums<VEC>(v0, cvb, red, tot);
+  for (int k = 0; k < VEC; ++k) v0[k] = 0.f;
+  if (cnt > 0) {
+    asm volatile("" ::: "memory");   // (read here, not held over the loop)
+    GnVec<DT>::unpack(*(const u16x8*)x, v0);   // the channels' values in row 0: the reference of the sums between threads
+  }
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) v0[k] = fmaf(fc, first[k] - v0[k], s[k]);
+  gn_block_sums<VEC, THREADS>(v0, cvb, red, tot);
   const float inv = real > 0 ? 1.f / ((float)real * (float)p.cpg) : 0.f;
   if ((int)threadIdx.x < ngb) {
-    double t = 0.0;
-    if (real > 0)
-      for (int c = 0; c < p.cpg; ++c) {
-        const int ch = threadIdx.x * p.cpg + c;
-        t += (double)op_load<DT>(((const T*)p.x)[n * p.xn + c_base + ch]) + (double)tot[ch] / (double)real;
-      }
-    gmean[threadIdx.x] = (float)(t / (double)p.cpg);
+    // the group's mean from its first channel's value in row 0 on: fp32 loses nothing to a mean far from zero
+    float ref = 0.f, t = 0.f;
+    if (real > 0) {
+      const T* row0 = (const T*)p.x + n * p.xn + c_base + threadIdx.x * p.cpg;
+      const float ir = 1.f / (float)real;
+      ref = op_load<DT>(row0[0]);
+      for (int c = 0; c < p.cpg; ++c) t += fmaf(tot[threadIdx.x * p.cpg + c], ir, op_load<DT>(row0[c]) - ref);
+    }
+    gmean[threadIdx.x] = ref + t / (float)p.cpg;
   }
   __syncthreads();
   float mu[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) {
-    mu[k] = gmean[(v * VEC + k) / p.cpg];
+    mu[k] = gmean[(v * VEC + k) >> sh];
     const float d = fmaf(s[k], ic, first[k] - mu[k]);          // the thread's mean, from the group's
     v0[k] = cnt > 0 ? fmaf(fc * d, d, fmaf(-s[k], s[k] * ic, q[k])) : 0.f;
   }
-  gn_block_sums<VEC>(v0, cvb, red, tot);
+  gn_block_sums<VEC, THREADS>(v0, cvb, red, tot);
   if ((int)threadIdx.x < ngb) {
     float t = 0.f;
     for (int c = 0; c < p.cpg; ++c) t += tot[threadIdx.x * p.cpg + c];
-    const float rs = real > 0 ? (float)(1.0 / sqrt((double)t * (double)inv + (double)p.eps)) : 0.f;
+    const float rs = real > 0 ? 1.f / sqrtf(fmaf(t, inv, p.eps)) : 0.f;
     grstd[threadIdx.x] = rs;
-    const long long g = n * p.G + c_base / p.cpg + threadIdx.x;
+    const long long g = n * p.G + (c_base >> sh) + threadIdx.x;
     p.mean[g] = gmean[threadIdx.x];
     p.rstd[g] = rs;
   }
@@ -560,12 +569,13 @@ __global__ __launch_bounds__(kGnSlabThreads, 4) void gn_slab_kernel(const GnPara
 #pragma unroll
   for (int k = 0; k < VEC; ++k) {
     const int c = c_base + v * VEC + k;
-    a[k] = grstd[(v * VEC + k) / p.cpg] * gn_param<DT>(p.w, c, p.affine_f32, 1.f);
+    a[k] = grstd[(v * VEC + k) >> sh] * gn_param<DT>(p.w, c, p.affine_f32, 1.f);
     b[k] = gn_param<DT>(p.b, c, p.affine_f32, 0.f);
     if constexpr (DT != 0) b[k] = fmaf(-mu[k], a[k], b[k]);   // see gn_apply_kernel
   }
+  T* dst = y + r0 * p.ol;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  for (int i = 0; i < NV; ++i, dst += dr * p.ol) {
     const int r = r0 + i * dr;
     if (r >= p.L) break;
     float f[VEC];
@@ -577,7 +587,8 @@ __global__ __launch_bounds__(kGnSlabThreads, 4) void gn_slab_kernel(const GnPara
 #pragma unroll
       for (int k = 0; k < VEC; ++k) f[k] = 0.f;
     }
-    *(u16x8*)(y + r * p.ol) = GnVec<DT>::pack(f);
+    *(u16x8*)dst = GnVec<DT>::pack(f);
+    __builtin_amdgcn_sched_barrier(0);   // one vector at a time: interleaved, their temporaries would not fit beside the data
   }
 }
 
@@ -587,7 +598,8 @@ __global__ __launch_bounds__(kGnSlabThreads, NV <= 4 ? 4 : 2) void gn_bwd_slab_k
   typedef typename OpType<DT>::T T;
   constexpr int VEC = GnVec<DT>::VEC;
   __shared__ float red[kGnSlabThreads / 16 * kGnMaxCvb * 2 * VEC], tot[kGnMaxCvb * 2 * VEC], gA[kGnMaxCvb * VEC], gB[kGnMaxCvb * VEC];
-  const int cvb = p.cvb, bc = cvb * VEC, bundles = p.C / bc, ngb = bc / p.cpg;
+  const int cvb = p.cvb, bc = cvb * VEC, bundles = p.C / bc;
+  const int sh = 31 - __builtin_clz(p.cpg), ngb = bc >> sh;   // groups divide a power of two here: they are powers of two
   const unsigned blk = xcd_remap(blockIdx.x, gridDim.x);
   const long long n = blk / (unsigned)bundles;
   const int c_base = (int)(blk % (unsigned)bundles) * bc;
@@ -609,7 +621,7 @@ __global__ __launch_bounds__(kGnSlabThreads, NV <= 4 ? 4 : 2) void gn_bwd_slab_k
   float mu[VEC], rs[VEC], w[VEC], b[VEC], s[2 * VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) {
-    const int c = c_base + v * VEC + k, g = c / p.cpg;
+    const int c = c_base + v * VEC + k, g = c >> sh;
     mu[k] = p.mean[n * p.G + g];
     rs[k] = p.rstd[n * p.G + g];
     w[k] = gn_param<DT>(p.w, c, p.affine_f32, 1.f);
@@ -633,7 +645,7 @@ __global__ __launch_bounds__(kGnSlabThreads, NV <= 4 ? 4 : 2) void gn_bwd_slab_k
         s[VEC + k] = fmaf(dz, h, s[VEC + k]);
       }
     }
-  gn_block_sums<2 * VEC>(s, cvb, red, tot);
+  gn_block_sums<2 * VEC, kGnSlabThreads>(s, cvb, red, tot);
   if ((int)threadIdx.x < bc) {   // a channel's sums: for the affine's gradients, and into its group
     const int vv = threadIdx.x / VEC, k = threadIdx.x % VEC;
     double* o = p.sums + (n * p.C + c_base + threadIdx.x) * 2;
@@ -655,7 +667,7 @@ __global__ __launch_bounds__(kGnSlabThreads, NV <= 4 ? 4 : 2) void gn_bwd_slab_k
   __syncthreads();
   float A[VEC], B[VEC];
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) { A[k] = gA[(v * VEC + k) / p.cpg]; B[k] = gB[(v * VEC + k) / p.cpg]; }
+  for (int k = 0; k < VEC; ++k) { A[k] = gA[(v * VEC + k) >> sh]; B[k] = gB[(v * VEC + k) >> sh]; }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int r = r0 + i * dr;

@@ -223,17 +223,17 @@ void gn_shape(long long L, int* rows, int* chunks) {
   *rows = (int)r;
   *chunks = (int)std::max<long long>(1, (L + r - 1) / r);
 }
-// Most 16-byte vectors a thread keeps.  Measured, f16 + GELU, 512 channels, 32 groups, whole-sample blocks against the streaming
-// kernels: 64 x 499 rows 34 / 47 us forward, 68 / 76 backward; 64 x 1999 (8 vectors) 85 / 101 and 217 / 193; 24 x 1999 in 512
-// groups 35 / 57 and 67 / 101; 64 x 3999 (16 vectors) 243 / 203 and 444 / 327.
-constexpr int kGnSlabMost = 8;
+// Most 16-byte vectors of a block, in units of 512.  Measured, f16 + GELU, 512 channels in 32 groups, whole-sample blocks against
+// the streaming kernels (us): forward 64 x 499 rows 26 / 47, 64 x 1999 83 / 101, 64 x 3999 (16) 206 / 198, but 8 x 3999 26 / 42 and
+// 1 x 3999 18 / 23; backward 64 x 499 51 / 76, 64 x 1999 (8) 199 / 193, 24 x 1999 in 512 groups 61 / 101, 64 x 3999 444 / 302.
+constexpr int kGnSlabFwd = 16, kGnSlabBwd = 8;
 // Channel vectors of a whole-sample block (0: the sample does not fit, or its groups do not divide into such blocks).
 // 2 vectors are 32 bytes of a row, the least that a fetch of a 64-byte half line uses well; wider groups take 4 or 8.
-int gn_slab(int dtype, int vec, long long L, int C, int cpg) {
+int gn_slab(int dtype, int vec, long long L, int C, int cpg, int most) {
   const int v16 = 16 / esize(dtype);
   if (vec != v16) return 0;
   for (int cvb = 2; cvb <= kGnMaxCvb; cvb *= 2)
-    if ((cvb * v16) % cpg == 0 && C % (cvb * v16) == 0) return L * cvb <= (long long)kGnSlabThreads * kGnSlabMost ? cvb : 0;
+    if ((cvb * v16) % cpg == 0 && C % (cvb * v16) == 0) return L * cvb <= (long long)kGnSlabThreads * most ? cvb : 0;
   return 0;
 }
 
@@ -332,14 +332,15 @@ extern "C" int vtc_group_norm_act(int device, int dtype, const vtc_rows3* x, con
   const int vec = vec_of(dtype, {channels, eff(x->batch, batch), eff(x->row, length), eff(y->batch, batch), eff(y->row, length)}, {x->p, y->p});
   p.cv = channels / vec;
   hipStream_t s = (hipStream_t)stream;
-  if ((p.cvb = gn_slab(dtype, vec, length, channels, p.cpg))) {
+  if ((p.cvb = gn_slab(dtype, vec, length, channels, p.cpg, kGnSlabFwd))) {
     const unsigned n = (unsigned)(batch * (channels / (p.cvb * vec)));
-    const int nv = (int)((length * p.cvb + kGnSlabThreads - 1) / kGnSlabThreads);
+    const long long pieces = length * p.cvb;   // 16-byte vectors of a block: 256 threads of 4 or 16, 512 of 16
     by_type(dtype, [&](auto d) { by_act(act, [&](auto a) {
       constexpr int DT = decltype(d)::value, ACT = decltype(a)::value;
       if constexpr (ACT != ACT_SIGMOID) {
-        if (nv <= 2) hipLaunchKernelGGL((gn_slab_kernel<DT, 2, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
-        else hipLaunchKernelGGL((gn_slab_kernel<DT, 8, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
+        if (pieces <= 256 * 4) hipLaunchKernelGGL((gn_slab_kernel<DT, 4, ACT, 256>), dim3(n), dim3(256), 0, s, p);
+        else if (pieces <= 256 * 16) hipLaunchKernelGGL((gn_slab_kernel<DT, 16, ACT, 256>), dim3(n), dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((gn_slab_kernel<DT, 16, ACT, 512>), dim3(n), dim3(512), 0, s, p);
       }
     }); });
     return launched("group norm");
@@ -394,7 +395,7 @@ extern "C" int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows
   const int vec = vec_of(dtype, {channels, eff(x->batch, batch), eff(x->row, length), eff(dy->batch, batch), eff(dy->row, length),
                                  eff(dx->batch, batch), eff(dx->row, length)}, {x->p, dy->p, dx->p});
   p.cv = channels / vec;
-  if ((p.cvb = gn_slab(dtype, vec, length, channels, p.cpg))) {
+  if ((p.cvb = gn_slab(dtype, vec, length, channels, p.cpg, kGnSlabBwd))) {
     const unsigned n = (unsigned)(batch * (channels / (p.cvb * vec)));
     const int nv = (int)((length * p.cvb + kGnSlabThreads - 1) / kGnSlabThreads);
     by_type(dtype, [&](auto d) { by_act(act, [&](auto a) {
