@@ -87,6 +87,12 @@ __device__ __forceinline__ void gelu2(float& a, float& b) {
   a = r[0]; b = r[1];
 }
 
+// Sums over the 16 lanes of a DPP row on the VALU (rotations; a shuffle is an LDS access)
+template <int CTRL> __device__ __forceinline__ float ror_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float row16_sum(float v) { return ror_add<0x121>(ror_add<0x122>(ror_add<0x124>(ror_add<0x128>(v)))); }
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);

@@ -451,14 +451,11 @@ template <int DT> struct GnVec {
 };
 
 // sum over the lanes of a row of 16 that hold the same channel vector (lane % cvb), on the VALU (DPP rotations)
-template <int CTRL> __device__ __forceinline__ float gn_ror_add(float v) {
-  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
 __device__ __forceinline__ float gn_row_sum(float v, int cvb) {
-  if (cvb <= 1) v = gn_ror_add<0x121>(v);
-  if (cvb <= 2) v = gn_ror_add<0x122>(v);
-  if (cvb <= 4) v = gn_ror_add<0x124>(v);
-  if (cvb <= 8) v = gn_ror_add<0x128>(v);
+  if (cvb <= 1) v = ror_add<0x121>(v);
+  if (cvb <= 2) v = ror_add<0x122>(v);
+  if (cvb <= 4) v = ror_add<0x124>(v);
+  if (cvb <= 8) v = ror_add<0x128>(v);
   return v;
 }
 constexpr int kGnMaxCvb = 8;

@@ -213,10 +213,7 @@ template <bool F16> struct OgDgate {
   template <int N> __device__ __forceinline__ void finish(int c, int fr, long long part, long long parts) {
     if (!p.colsum) return;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) { sg[k] += __shfl_xor(sg[k], o); su[k] += __shfl_xor(su[k], o); }
-    }
+    for (int k = 0; k < N; ++k) { sg[k] = row16_sum(sg[k]); su[k] = row16_sum(su[k]); }
     if (fr == 0 && c < t.cols) {
       float* dst = p.colsum + part * p.ldg + t.n0 + c;
 #pragma unroll

@@ -555,10 +555,10 @@ OgPlan og_plan(const OgCost& o, int nk, int splits_big, int splits_small, double
 }
 int div_up(long long a, int b) { return (int)((a + b - 1) / b); }
 
-void finish_prob(OpProb& q, bool small, int bm, int bn, int K, int tile0) {
+void finish_prob(OpProb& q, bool small, int bm, int bn, int K, int tile0, int w_rows = 0) {   // w_rows: rows of B behind a tile, if not bn
   q.tiles_m = div_up(q.M, bm);
   q.tiles_n = div_up(q.N, bn);
-  q.group_n = small ? q.tiles_n : group_of(q.tiles_m, q.tiles_n, 2.0 * q.M * K, 2.0 * q.N * K, 2.0 * bn * K);
+  q.group_n = small ? q.tiles_n : group_of(q.tiles_m, q.tiles_n, 2.0 * q.M * K, 2.0 * q.N * K, 2.0 * (w_rows ? w_rows : bn) * K);
   q.tile0 = tile0;
 }
 void set_k(OpGemmParams& p, const OgPlan& plan, int k0, int k1 = 0) {
@@ -608,7 +608,7 @@ template <bool F16> void gate_up(int64_t M, int K, int F, OpMat x, OpMat wg, OpM
   p.nprob = 1;
   OpProb& q = p.prob[0];
   q.a[0] = x; q.b[0] = wg; q.b[1] = wu; q.c = o.h; q.ldc = F8; q.M = (int)M; q.N = F8; q.Nb = F; q.cvec = 1;
-  finish_prob(q, plan.small, plan.small ? 128 : 256, plan.small ? 32 : 128, K, 0);
+  finish_prob(q, plan.small, plan.small ? 128 : 256, plan.small ? 32 : 128, K, 0, 256);
   p.ntiles = q.tiles_m * q.tiles_n;
   set_k(p, plan, K);
   p.bias = bg; p.bias2 = bu; p.bias_f32 = bias_f32; p.act = act; p.s = o.s; p.a = o.a; p.ldg = F8;
