@@ -497,18 +497,24 @@ Span span(const char* name, const vtc_mat* m, long long rows, long long cols) { 
 
 bool pieces_ok(const vtc_mat* m, int cols) { return cols % 8 == 0 && m->row % 8 == 0 && (uintptr_t)m->p % 16 == 0; }
 
-// An operand made of aligned 16-byte pieces: the caller's memory where it is, a padded copy in the workspace where it is not.
-OpMat operand(Arena& ar, const vtc_mat* m, int64_t rows, int cols, bool force, hipStream_t s, bool launch) {
-  if (!force && pieces_ok(m, cols)) return OpMat{(const h16*)m->p, m->row};
-  const int d = up8(cols);
-  h16* c = ar.take<h16>((size_t)rows * d);
-  if (launch && rows > 0) {
-    const long long n = rows * (d / 8);
-    hipLaunchKernelGGL(pad_copy_kernel, dim3((unsigned)std::min<long long>((n + 255) / 256, 65536)), dim3(256), 0, s, (const h16*)m->p, (long long)m->row, c,
-                       (long long)rows, cols, d);
+// Operands made of aligned 16-byte pieces: the caller's memory where it is, padded copies in the workspace where it is not.
+struct Operands {
+  Arena& ar;
+  PadParams p{};
+  int n = 0;
+  long long most = 0;   // pieces of the largest copy
+  OpMat get(const vtc_mat* m, int64_t rows, int cols, bool force = false) {
+    if (!force && pieces_ok(m, cols)) return OpMat{(const h16*)m->p, m->row};
+    const int d = up8(cols);
+    h16* c = ar.take<h16>((size_t)rows * d);
+    p.j[n++] = PadJob{(const h16*)m->p, c, m->row, rows, cols, d};
+    most = std::max<long long>(most, rows * (d / 8));
+    return OpMat{c, d};
   }
-  return OpMat{c, d};
-}
+  void copy(hipStream_t s) const {
+    if (most) hipLaunchKernelGGL(pad_copy_kernel, dim3((unsigned)std::min<long long>((most + 255) / 256, 65536), (unsigned)n), dim3(256), 0, s, p);
+  }
+};
 
 // Column-group width of a product's tile order: see launch_gemm256
 int group_of(int tiles_m, int tiles_n, double a_bytes, double w_bytes, double w_group_bytes) {
@@ -659,17 +665,19 @@ FfnSaved ffn_saved(void* base, int64_t rows, int inner) {
 size_t ffn_forward(const FfnArgs& a, const vtc_mat* y, void* saved, char* ws, bool launch, hipStream_t s) {
   Arena ar{ws};
   const int F8 = up8(a.F);
-  const OpMat x = operand(ar, a.x, a.M, a.K, false, s, launch);
+  Operands in{ar};
+  const OpMat x = in.get(a.x, a.M, a.K);
   // gate and up share one pitch in the kernel
   const bool copy_w = a.wg->row != a.wu->row || !pieces_ok(a.wg, a.K) || !pieces_ok(a.wu, a.K);
-  const OpMat wg = operand(ar, a.wg, a.F, a.K, copy_w, s, launch), wu = operand(ar, a.wu, a.F, a.K, copy_w, s, launch);
-  const OpMat wd = operand(ar, a.wd, a.N, a.F, false, s, launch);
+  const OpMat wg = in.get(a.wg, a.F, a.K, copy_w), wu = in.get(a.wu, a.F, a.K, copy_w);
+  const OpMat wd = in.get(a.wd, a.N, a.F);
   const FfnSaved sv = ffn_saved(saved, a.M, a.F);
   h16* h = saved ? sv.h : ar.take<h16>((size_t)a.M * F8);
   const bool skinny = a.M <= kSkinnyRows;
   OutPlan out{};
   if (!skinny) out = plan_out(ar, a.M, a.N, div_up(a.F, 64));
   if (!launch) return ar.used;
+  in.copy(s);
   by_f16(a.dtype, [&](auto f) {
     constexpr bool F16 = decltype(f)::value;
     gate_up<F16>(a.M, a.K, a.F, x, wg, wu, a.bg, a.bu, a.bias_f32, a.act, GateOut{h, sv.s, sv.a}, skinny, s);
@@ -690,10 +698,11 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, cons
   Arena ar{ws};
   const int K8 = up8(a.K), F8 = up8(a.F), N8 = up8(a.N);
   const int M = (int)a.M;
-  const OpMat x = operand(ar, a.x, a.M, a.K, false, s, launch), y = operand(ar, dy, a.M, a.N, false, s, launch);
+  Operands in{ar};
+  const OpMat x = in.get(a.x, a.M, a.K), y = in.get(dy, a.M, a.N);
   const bool copy_w = a.wg->row != a.wu->row || !pieces_ok(a.wg, a.K) || !pieces_ok(a.wu, a.K);
-  const OpMat wg = operand(ar, a.wg, a.F, a.K, copy_w, s, launch), wu = operand(ar, a.wu, a.F, a.K, copy_w, s, launch);
-  const OpMat wd = operand(ar, a.wd, a.N, a.F, false, s, launch);
+  const OpMat wg = in.get(a.wg, a.F, a.K, copy_w), wu = in.get(a.wu, a.F, a.K, copy_w);
+  const OpMat wd = in.get(a.wd, a.N, a.F);
   h16 *dg = ar.take<h16>((size_t)a.M * F8), *du = ar.take<h16>((size_t)a.M * F8);
   // dh and what it turns into
   const OgPlan dplan = og_plan({(long long)div_up(M, 256) * div_up(F8, 192), (long long)div_up(M, 128) * div_up(F8, 64), 0.75, 20.0, 7.0}, div_up(a.N, 64), 1, 1, 0);
@@ -727,6 +736,7 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, cons
   set_k(w, wplan, M);
   float* part = o->dw_gate || !launch ? ar.take<float>((size_t)w.splits * w.split_stride) : nullptr;
   if (!launch) return ar.used;
+  in.copy(s);
   for (int i = 0; i < 3; ++i) w.prob[i].c = part + i * one;
 
   const FfnSaved sv = ffn_saved((void*)saved, a.M, a.F);
