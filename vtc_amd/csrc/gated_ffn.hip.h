@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const SplitReducePara
 
 // ---- few rows: C[M <= 16 MT][N] = A W^T.  A block owns 16 columns, its 8 waves take every 8th K step of 32 straight from global
 // memory (the weights are read once, by nobody else), their partial tiles meet in LDS.  MFMA computes C^T: lane (fr, fq) holds
-// row fr of A and columns 4 fq .. + 4.
+// row fr of A and columns 4 fq .. + 4.  Bound: latency; one row, 768 x 2048: 4.8 us for gate and up (6.3 MB), 4.8 us for down.
 struct SkinnyParams {
   const h16 *x, *w0, *w1;     // w1: W_up (GATE)
   long long ldx, ldw;

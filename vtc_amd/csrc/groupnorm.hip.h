@@ -6,6 +6,13 @@
 //   dx = rstd (w_c dz - (A + xhat B) / M),  A = sum w_c dz,  B = sum w_c dz xhat over the group, M = its element count.
 // Rows at and behind length[n] are not read; y and dx are zero there.  A sample of length 0 has mean = rstd = 0.
 //
+// Two forms.  Samples that fit a block's registers are read once (gn_slab_kernel, gn_bwd_slab_kernel); everything else - long or odd
+// samples, wide groups, strides that are no whole vectors - streams: statistics per row block, merge, elementwise pass, in which x (and
+// dy) are read a second time, last rows first, since those are still in the last-level cache.  Bound: memory and the activation's
+// vector instructions (about 25 issue slots of an element for GELU, 83 us of 131 M elements), which add up: 64 x 3999 x 512 f16 with
+// GELU takes 206 us on chip where its 524 MB alone take 105, and 198 streaming.  Figures of both forms: kGnSlabFwd in vtc_ops.hip.
+// 5 x 1531 x 201 fp32 (streaming, 4-byte accesses): statistics 5, elementwise 12, backward sums 7, merges 4 + 3, dx 7 us.
+//
 // Statistics: every partial is (mean, M2 = sum of squared distances from it) and partials merge by Chan's formula, so a mean
 // that is large against the spread does not cancel; inside a thread the sums are of x - x_first (the row block's first row, per
 // channel), in fp32 over at most a few hundred rows; merges across row blocks are fp64.  All orders are fixed, no atomics:
