@@ -3,8 +3,10 @@
 Tolerances: a result rounded to type t is off by at most eps(t) / 2 of its value; the fp32 arithmetic in front of it is bounded term
 by term beside each check.  Refusals run without a GPU (the library checks its arguments before it looks for a device)."""
 
+import copy
 import ctypes as C
 import math
+import pickle
 
 import numpy as np
 import pytest
@@ -179,6 +181,16 @@ def test_rotary_refusals_of_the_wrapper():
                 dict(rotary_dim=8, base=1.0), dict(rotary_dim=8, scaling="linear", factor=0.0), dict(rotary_dim=8, scaling="by_parts", factor=2.0)):
         with pytest.raises(ValueError):
             ops.Rotary(**bad)
+
+
+def test_rotary_description_is_copied_and_pickled_without_addresses():
+    spec = ops.Rotary(48, layout="interleaved", scaling="by_parts", factor=8.0, original_length=500)
+    first = spec._struct(64)
+    for other in (copy.deepcopy(spec), copy.copy(spec), pickle.loads(pickle.dumps(spec))):
+        assert np.array_equal(other.frequency, spec.frequency) and not other.frequency.flags.writeable
+        s = other._struct(64)
+        assert (s.rotary_dim, s.layout, s.amplitude) == (first.rotary_dim, first.layout, first.amplitude)
+        assert C.cast(s.frequency, C.c_void_p).value == other.frequency.ctypes.data != spec.frequency.ctypes.data
 
 
 @gpu
@@ -615,6 +627,42 @@ def test_gated_ffn_activations_and_fp32_biases(act, m):
     y, saved = ops.gated_ffn_forward(x, *w, *b, act=act, save=True)
     grads = ops.gated_ffn_backward(dy, x, *w, saved, act=act, bias_dtype=torch.float32)
     check_ffn(torch.float16, x, w, b, act, dy, y, grads)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [0x7FFFFFFF, -1, 0x7F800001, 0x7F800000])   # NaN of both signs with every bit set, the least one, inf
+@pytest.mark.parametrize("m,k,f", [(5, 64, 136), (300, 64, 136), (9000, 768, 2048)])
+def test_gated_ffn_gradients_of_bias_values_that_are_no_numbers(bits, m, k, f):
+    for which in (0, 1):
+        x, w, b, dy = make_ffn(torch.bfloat16, m, k, f, k, True, bias_kind=torch.float32)
+        b[which].view(torch.int32)[77] = bits
+        y, saved = ops.gated_ffn_forward(x, *w, *b, act="sigmoid", save=True)
+        dx, dwg, dwu, dwd, dbg, dbu, _ = ops.gated_ffn_backward(dy, x, *w, saved, act="sigmoid", bias_dtype=torch.float32)
+        clean = torch.arange(f, device="cuda") != 77
+        for t in (dwg[clean], dwu[clean], dwd[:, clean], dbg[clean], dbu[clean]):
+            assert torch.isfinite(t).all()
+        nan = bits != 0x7F800000
+        if which == 0:     # sigmoid(inf) = 1 with slope 0
+            assert torch.isnan(y).all() == nan and torch.isfinite(y).all() != nan
+            assert torch.isnan(dx).all() == nan and torch.isfinite(dx).all() != nan
+            assert torch.isnan(dwg[77]).all() == nan and torch.isnan(dbg[77]) == nan and torch.isnan(dwu[77]).all() == nan
+        else:              # u = inf: h and dg are infinite, so sums over them are inf or NaN; du does not depend on u
+            assert not torch.isfinite(y).any() and not torch.isfinite(dx).any() and not torch.isfinite(dwg[77]).any()
+            assert torch.isfinite(dwu[77]).all() and torch.isfinite(dbu[77]) and not torch.isfinite(dwd[:, 77]).any()
+
+
+@gpu
+@pytest.mark.parametrize("bits", [0x7FFF, -1])   # NaN of both signs with every bit set
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("m,k,f", [(5, 64, 136), (300, 64, 136), (9000, 768, 2048)])
+def test_gated_ffn_gradients_of_a_row_that_is_no_number(kind, bits, m, k, f):
+    x, w, b, dy = make_ffn(TYPES[kind], m, k, f, k, True)
+    x.view(torch.int16)[2, 11] = bits
+    y, saved = ops.gated_ffn_forward(x, *w, *b, save=True)
+    dx, dwg, dwu, dwd, dbg, dbu, dbd = ops.gated_ffn_backward(dy, x, *w, saved)
+    clean = torch.arange(m, device="cuda") != 2
+    assert torch.isnan(y[2]).all() and torch.isnan(dx[2]).all() and torch.isfinite(y[clean]).all() and torch.isfinite(dx[clean]).all()
+    assert all(torch.isnan(t).all() for t in (dwg, dwu, dwd, dbg, dbu)) and torch.isfinite(dbd).all()
 
 
 @gpu

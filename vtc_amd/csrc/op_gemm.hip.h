@@ -67,7 +67,10 @@ struct OpGemmParams {
 
 __device__ __forceinline__ float op_bias(const void* b, int i, int f32, bool f16) {
   if (!b) return 0.f;
-  if (f32) return ((const float*)b)[i];
+  if (f32) {
+    const unsigned v = ((const unsigned*)b)[i];
+    return __uint_as_float((v & 0x7fffffffu) > 0x7f800000u ? 0x7fc00000u : v);   // a NaN whose low bits survive store24's rounding
+  }
   const h16 v = ((const h16*)b)[i];
   return f16 ? from_h16<true>(v) : from_h16<false>(v);
 }
@@ -106,7 +109,8 @@ template <bool F16> struct OpTile {
       __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3])},
                                              rs, off(ld, r, c + 4 * h, 4), 0, 0);
   }
-  // 8 values in 24 bits (round half away; inf and NaN keep their upper bits)
+  // 8 values in 24 bits (round half away; inf stays, and so does a NaN whose low bits are clear: those of 16-bit values, of the matrix
+  // instructions and of op_bias)
   __device__ __forceinline__ void store24(__amdgpu_buffer_rsrc_t hi, __amdgpu_buffer_rsrc_t lo, long long ld, int r, int c, const float* v) const {
     unsigned b[8];
 #pragma unroll

@@ -122,6 +122,13 @@ class Rotary:
         self.frequency = f
         self._structs = {}
 
+    def __getstate__(self):   # copies and pickles leave the C descriptions, which hold addresses, behind
+        return {"rotary_dim": self.rotary_dim, "layout": self.layout, "amplitude": self.amplitude, "frequency": self.frequency}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state, frequency=np.array(state["frequency"]), _structs={})
+        self.frequency.setflags(write=False)
+
     def _struct(self, head_dim: int) -> L.VtcRotary:
         """The C description for heads of this size (it points into self.frequency)."""
         s = self._structs.get(head_dim)
