@@ -34,57 +34,74 @@ __global__ __launch_bounds__(256) void pad_copy_kernel(PadParams p) {
   }
 }
 
-// column sums of kColRows rows (dy -> partial sums of d b_down); part [blocks of rows][pitch]
+// column sums of kColRows rows (dy -> partial sums of d b_down); part [blocks of rows][pitch].  red: 4 x 512 floats
 constexpr int kColRows = 64;
+struct ColSumParams { const h16* x; long long ld, rows; float* part; int pitch, cols, row_blocks, blocks; };   // blocks: row_blocks x 512 columns each
 template <bool F16>
-__global__ __launch_bounds__(256) void colsum_kernel(const h16* x, long long ld, float* part, int pitch, long long rows, int cols) {
-  __shared__ float red[4][64 * 8];
-  const int v = blockIdx.y * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-  const long long r0 = (long long)blockIdx.x * kColRows, r1 = min(rows, r0 + kColRows);
+__device__ __forceinline__ void colsum_tile(const ColSumParams& p, unsigned block, float (*red)[512]) {
+  const int rb = (int)(block % (unsigned)p.row_blocks), cb = (int)(block / (unsigned)p.row_blocks);
+  const int v = cb * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const long long r0 = (long long)rb * kColRows, r1 = min(p.rows, r0 + kColRows);
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (v * 8 < cols)
+  if (v * 8 < p.cols)
 #pragma unroll 8
     for (long long r = r0 + w; r < r1; r += 4) {
-      const u16x8 f = *(const u16x8*)(x + r * ld + v * 8);
+      const u16x8 f = *(const u16x8*)(p.x + r * p.ld + v * 8);
 #pragma unroll
       for (int k = 0; k < 8; ++k) s[k] += from_h16<F16>(f[k]);
     }
 #pragma unroll
   for (int k = 0; k < 8; ++k) red[w][(threadIdx.x & 63) * 8 + k] = s[k];
   __syncthreads();
-  if (w == 0 && v * 8 < pitch)
+  if (w == 0 && v * 8 < p.pitch)
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int i = threadIdx.x * 8 + k;
-      part[(long long)blockIdx.x * pitch + v * 8 + k] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+      p.part[(long long)rb * p.pitch + v * 8 + k] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
     }
 }
+template <bool F16>
+__global__ __launch_bounds__(256) void colsum_kernel(const ColSumParams p) {
+  __shared__ float red[4][512];
+  colsum_tile<F16>(p, blockIdx.x, red);
+}
 
+// The rest of a small backward pass behind dg and du in one launch: the weights' gradients (the longest first), dx, dy's column sums.
+// They do not depend on each other; each alone leaves CUs idle and costs a launch.  Backward with biases, launched apart / together:
+// 512 rows, 768 x 2048, 59 / 44 us; 2048 rows 100 / 77; 1237 x 389 x 1031 with its forward 72 / 63.
+struct SmallGradsParams { OpGemmParams w, dx; ColSumParams c; unsigned w_blocks, dx_blocks; };
+template <bool F16, int DX_EPI>
+__global__ __launch_bounds__(256, 2) void small_grads_kernel(const SmallGradsParams p) {
+  __shared__ __attribute__((aligned(16))) char smem[3 * kOsStage];
+  if (blockIdx.x < p.w_blocks) op_small_tile<F16, true, true, OG_PART>(p.w, blockIdx.x, p.w_blocks, smem);
+  else if (blockIdx.x - p.w_blocks < p.dx_blocks) op_small_tile<F16, false, true, DX_EPI>(p.dx, blockIdx.x - p.w_blocks, p.dx_blocks, smem);
+  else colsum_tile<F16>(p.c, blockIdx.x - p.w_blocks - p.dx_blocks, (float (*)[512])smem);
+}
+
+// What is left of a pass once its products are there, in one launch (blockIdx.y): K-split partials (+ bias) -> 16-bit results, and
+// partial column sums -> bias gradients, out[c] = sum over n partial rows, in order, fp64 (16 slices of rows by 16 columns a block).
 struct ColReduce { const float* part; void* out; long long n; int pitch, cols; };
-// bias gradients: out[c] = sum over n partial rows, in order, fp64; up to three of them in one launch (blockIdx.y)
-struct ColReduceParams { ColReduce r[3]; int f16, out_f32; };
-__global__ __launch_bounds__(1024) void col_reduce_kernel(const ColReduceParams p) {
-  __shared__ double red[16][64];
-  const ColReduce& q = p.r[blockIdx.y];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+struct SplitReduce { const float* part; h16* out; long long ldo, pitch, rows, stride; int splits, cols, vec; const void* bias; };
+struct ReduceParams { SplitReduce r[4]; ColReduce c[3]; int nr, nc, bias_f32; };   // bias_f32: biases and their gradients are fp32
+template <bool F16> __device__ __forceinline__ void col_reduce(const ColReduce& q, int out_f32) {
+  __shared__ double red[16][16];
+  const int c = blockIdx.x * 16 + (threadIdx.x & 15), w = threadIdx.x >> 4;
+  if ((int)blockIdx.x * 16 >= q.cols) return;
   double s = 0.0;
   if (c < q.cols)
 #pragma unroll 8
     for (long long i = w; i < q.n; i += 16) s += (double)q.part[i * q.pitch + c];
-  red[w][threadIdx.x & 63] = s;
+  red[w][threadIdx.x & 15] = s;
   __syncthreads();
   if (w || c >= q.cols) return;
   for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
   const float v = (float)s;
-  if (p.out_f32) ((float*)q.out)[c] = v;
-  else ((h16*)q.out)[c] = p.f16 ? to_h16<true>(v) : to_h16<false>(v);
+  if (out_f32) ((float*)q.out)[c] = v;
+  else ((h16*)q.out)[c] = to_h16<F16>(v);
 }
-
-// K-split partials (+ bias) -> 16-bit result; up to three matrices in one launch
-struct SplitReduce { const float* part; h16* out; long long ldo, pitch, rows; int cols, vec; const void* bias; };
-struct SplitReduceParams { SplitReduce r[3]; int n, splits, bias_f32; long long stride; };
 template <bool F16>
-__global__ __launch_bounds__(256) void split_reduce_kernel(const SplitReduceParams p) {
+__global__ __launch_bounds__(256) void reduce_kernel(const ReduceParams p) {
+  if ((int)blockIdx.y >= p.nr) { col_reduce<F16>(p.c[blockIdx.y - p.nr], p.bias_f32); return; }
   const SplitReduce& q = p.r[blockIdx.y];
   const long long pieces = q.pitch / 4;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < q.rows * pieces; i += (long long)gridDim.x * 256) {
@@ -93,8 +110,8 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const SplitReducePara
     if (c >= q.cols) continue;
     const float* src = q.part + r * q.pitch + c;
     float4 s = *(const float4*)src;
-    for (int k = 1; k < p.splits; ++k) {
-      const float4 t = *(const float4*)(src + k * p.stride);
+    for (int k = 1; k < q.splits; ++k) {
+      const float4 t = *(const float4*)(src + k * q.stride);
       s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
     }
     if (q.bias) {

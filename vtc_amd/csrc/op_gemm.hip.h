@@ -627,15 +627,14 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
 // buffers (A 16 KB, B 8 KB each), two in flight, one barrier per K-tile.  The contraction runs in the same order as in the kernel
 // above, so an unsplit product has the same bits in either.  Measured against the 256-wide tiles: the table at og_plan.
 constexpr int kOsA = 16384, kOsStage = 24576;
-template <bool F16, bool AKS, bool BKS, int EPI>
-__global__ __launch_bounds__(256, 2) void op_small_kernel(const OpGemmParams p) {
-  __shared__ __attribute__((aligned(16))) char smem[3 * kOsStage];
+template <bool F16, bool AKS, bool BKS, int EPI>   // smem: 3 kOsStage bytes
+__device__ __forceinline__ void op_small_tile(const OpGemmParams& p, unsigned block, unsigned blocks, char* smem) {
   constexpr bool MULTI = AKS;
   constexpr int NSEG = (EPI == OG_PLAIN || EPI == OG_PART) && BKS && !AKS ? 2 : 1;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fq = lane >> 4, lr = lane >> 3, lc = lane & 7;
-  const unsigned u = xcd_remap(blockIdx.x, gridDim.x);
+  const unsigned u = xcd_remap(block, blocks);
   const unsigned ti = u / (unsigned)p.splits;
   const int split = (int)(u - ti * (unsigned)p.splits);
   int pi = 0;
@@ -823,6 +822,12 @@ __global__ __launch_bounds__(256, 2) void op_small_kernel(const OpGemmParams p) 
       grad.template finish<8>(half ? c1 : c0, fr, (long long)tile_m * 4 + wave, q.tiles_m * 4ll);
     }
   }
+}
+
+template <bool F16, bool AKS, bool BKS, int EPI>
+__global__ __launch_bounds__(256, 2) void op_small_kernel(const OpGemmParams p) {
+  __shared__ __attribute__((aligned(16))) char smem[3 * kOsStage];
+  op_small_tile<F16, AKS, BKS, EPI>(p, blockIdx.x, gridDim.x, smem);
 }
 
 }  // namespace vtc

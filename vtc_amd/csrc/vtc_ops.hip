@@ -549,7 +549,8 @@ OgPlan og_plan(const OgCost& o, int nk, int splits_big, int splits_small, double
     for (int sp = 1; sp <= (small ? splits_small : splits_big); ++sp) {
       int k = (nk + sp - 1) / sp;
       if (!small) k = (k + 1) & ~1;
-      if ((nk + k - 1) / k != sp || (sp > 1 && k < 4)) continue;
+      if (sp > 1 && k < 4) break;
+      if ((nk + k - 1) / k != sp) continue;
       const double cap = small ? 512.0 : 256.0, units = (double)(small ? o.tiles_small : o.tiles_big) * sp;
       auto round = [&](double fill) { return small ? k * (0.42 + 0.38 * fill) + o.end_small : k * o.width * (1.35 + 0.75 * fill) + o.end_big; };
       const double full = std::floor(units / cap), rest = units / cap - full;
@@ -579,10 +580,12 @@ template <bool F16, bool AKS, bool BKS, int EPI, int BN> void launch_og(const Op
   else if constexpr (EPI != OG_PART || AKS)   // 256-wide tiles are split over K for the weights' gradients only
     hipLaunchKernelGGL((op_gemm_kernel<F16, AKS, BKS, EPI, BN>), dim3((unsigned)std::min(units, 256)), dim3(512), 0, s, p);
 }
-template <bool F16> void launch_reduce(const SplitReduceParams& r, hipStream_t s) {
-  long long most = 1;
-  for (int i = 0; i < r.n; ++i) most = std::max(most, r.r[i].rows * (r.r[i].pitch / 4));
-  hipLaunchKernelGGL((split_reduce_kernel<F16>), dim3((unsigned)std::min<long long>((most + 255) / 256, 16384), (unsigned)r.n), dim3(256), 0, s, r);
+template <bool F16> void launch_reduce(const ReduceParams& r, hipStream_t s) {
+  if (r.nr + r.nc == 0) return;
+  long long most = 1;   // blocks in x
+  for (int i = 0; i < r.nr; ++i) most = std::max(most, std::min<long long>((r.r[i].rows * (r.r[i].pitch / 4) + 255) / 256, 16384));
+  for (int i = 0; i < r.nc; ++i) most = std::max<long long>(most, (r.c[i].cols + 15) / 16);
+  hipLaunchKernelGGL((reduce_kernel<F16>), dim3((unsigned)most, (unsigned)(r.nr + r.nc)), dim3(256), 0, s, r);
 }
 template <bool F16, bool GATE> void launch_skinny(const SkinnyParams& p, hipStream_t s) {
   const dim3 grid((unsigned)((p.N + 15) / 16)), block(512);
@@ -629,28 +632,28 @@ OutPlan plan_out(Arena& ar, int64_t M, int N, int nk) {
   if (o.plan.splits > 1) o.part = ar.take<float>((size_t)o.plan.splits * M * o.N8);
   return o;
 }
-template <bool F16, bool BKS> void product_out(const OutPlan& o, int64_t M, int N, const OpMat* a, const OpMat* b, const int* k, int segs, const void* bias,
-                                               int bias_f32, void* c, long long ldc, hipStream_t s) {
+struct OutProduct { const OpMat *a, *b; const int* k; int segs; const void* bias; int bias_f32; void* c; long long ldc; };
+OpGemmParams out_params(const OutPlan& o, int64_t M, int N, const OutProduct& x) {
   const bool small = o.plan.small;
-  const int cvec = N % 8 == 0 && ldc % 8 == 0 && (uintptr_t)c % 16 == 0;
   OpGemmParams p{};
   p.nprob = 1;
   OpProb& q = p.prob[0];
-  for (int i = 0; i < segs; ++i) { q.a[i] = a[i]; q.b[i] = b[i]; }
-  q.M = (int)M; q.Nb = N; q.cvec = cvec;
-  if (o.part) { q.c = o.part; q.ldc = o.N8; q.N = o.N8; }
-  else { q.c = c; q.ldc = ldc; q.N = N; }
-  finish_prob(q, small, small ? 128 : 256, small ? 64 : 192, k[0] + (segs > 1 ? k[1] : 0), 0);
+  for (int i = 0; i < x.segs; ++i) { q.a[i] = x.a[i]; q.b[i] = x.b[i]; }
+  q.M = (int)M; q.Nb = N; q.cvec = N % 8 == 0 && x.ldc % 8 == 0 && (uintptr_t)x.c % 16 == 0;
+  if (o.part) { q.c = o.part; q.ldc = o.N8; q.N = o.N8; p.split_stride = M * o.N8; }
+  else { q.c = x.c; q.ldc = x.ldc; q.N = N; }
+  finish_prob(q, small, small ? 128 : 256, small ? 64 : 192, x.k[0] + (x.segs > 1 ? x.k[1] : 0), 0);
   p.ntiles = q.tiles_m * q.tiles_n;
-  set_k(p, o.plan, k[0], segs > 1 ? k[1] : 0);
-  p.bias = bias; p.bias_f32 = bias_f32;
-  if (!o.part) { launch_og<F16, false, BKS, OG_PLAIN, 192>(p, small, s); return; }
-  p.split_stride = M * o.N8;
-  launch_og<F16, false, BKS, OG_PART, 192>(p, true, s);
-  SplitReduceParams r{};
-  r.r[0] = SplitReduce{o.part, (h16*)c, ldc, o.N8, M, N, cvec, bias};
-  r.n = 1; r.splits = p.splits; r.stride = p.split_stride; r.bias_f32 = bias_f32;
-  launch_reduce<F16>(r, s);
+  set_k(p, o.plan, x.k[0], x.segs > 1 ? x.k[1] : 0);
+  p.bias = x.bias; p.bias_f32 = x.bias_f32;
+  return p;
+}
+void add_out_reduce(ReduceParams& r, const OutPlan& o, const OpGemmParams& p, int64_t M, int N, const OutProduct& x) {
+  if (o.part) r.r[r.nr++] = SplitReduce{o.part, (h16*)x.c, x.ldc, o.N8, M, p.split_stride, p.splits, N, p.prob[0].cvec, x.bias};
+}
+template <bool F16, bool BKS> void launch_out(const OutPlan& o, const OpGemmParams& p, hipStream_t s) {
+  if (o.part) launch_og<F16, false, BKS, OG_PART, 192>(p, true, s);
+  else launch_og<F16, false, BKS, OG_PLAIN, 192>(p, o.plan.small, s);
 }
 
 // Layout of what the forward call keeps: h, then the upper 16 bits of s and of a, then their next 8 bits
@@ -688,7 +691,13 @@ size_t ffn_forward(const FfnArgs& a, const vtc_mat* y, void* saved, char* ws, bo
       launch_skinny<F16, false>(p, s);
     } else {
       const OpMat hm{h, F8};
-      product_out<F16, false>(out, a.M, a.N, &hm, &wd, &a.F, 1, a.bd, a.bias_f32, (void*)y->p, y->row, s);
+      const OutProduct x{&hm, &wd, &a.F, 1, a.bd, a.bias_f32, (void*)y->p, y->row};
+      const OpGemmParams p = out_params(out, a.M, a.N, x);
+      launch_out<F16, false>(out, p, s);
+      ReduceParams r{};
+      r.bias_f32 = a.bias_f32;
+      add_out_reduce(r, out, p, a.M, a.N, x);
+      launch_reduce<F16>(r, s);
     }
   });
   return ar.used;
@@ -751,36 +760,36 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, cons
     set_k(d, dplan, a.N);
     d.s = sv.s; d.a = sv.a; d.dg = dg; d.du = du; d.ldg = F8; d.colsum = cs_f;
     launch_og<F16, false, true, OG_DGATE, 192>(d, dplan.small, s);
-    if (o->dx) {
-      const OpMat xa[2] = {{dg, F8}, {du, F8}}, xb[2] = {wg, wu};
-      const int xk[2] = {a.F, a.F};
-      product_out<F16, true>(xplan, M, a.K, xa, xb, xk, 2, nullptr, 0, o->dx, o->dx_row, s);
+    ReduceParams r{};
+    r.bias_f32 = a.bias_f32;
+    const OpMat xa[2] = {{dg, F8}, {du, F8}}, xb[2] = {wg, wu};
+    const int xk[2] = {a.F, a.F};
+    const OutProduct xp{xa, xb, xk, 2, nullptr, 0, o->dx, o->dx_row};
+    const OpGemmParams dx = out_params(xplan, M, a.K, xp);
+    const int col_blocks = (N8 / 8 + 63) / 64;
+    const ColSumParams cs{y.p, y.ld, M, cs_n, N8, a.N, row_blocks, cs_n ? row_blocks * col_blocks : 0};
+    if (o->dx && part && xplan.plan.small && wplan.small) {
+      const SmallGradsParams g{w, dx, cs, (unsigned)(w.ntiles * w.splits), (unsigned)(dx.ntiles * dx.splits)};
+      const dim3 grid(g.w_blocks + g.dx_blocks + (unsigned)cs.blocks);
+      if (xplan.part) hipLaunchKernelGGL((small_grads_kernel<F16, OG_PART>), grid, dim3(256), 0, s, g);
+      else hipLaunchKernelGGL((small_grads_kernel<F16, OG_PLAIN>), grid, dim3(256), 0, s, g);
+    } else {
+      if (o->dx) launch_out<F16, true>(xplan, dx, s);
+      if (part) launch_og<F16, true, true, OG_PART, 256>(w, wplan.small, s);
+      if (cs_n) hipLaunchKernelGGL((colsum_kernel<F16>), dim3((unsigned)cs.blocks), dim3(256), 0, s, cs);
     }
-    if (part) {
-      launch_og<F16, true, true, OG_PART, 256>(w, wplan.small, s);
-      SplitReduceParams r{};
-      void* outs[3] = {o->dw_gate, o->dw_up, o->dw_down};
-      for (int i = 0; i < 3; ++i)
-        r.r[i] = SplitReduce{part + i * one, (h16*)outs[i], cols[i], pitch[i], rows[i], cols[i], cols[i] % 8 == 0 && (uintptr_t)outs[i] % 16 == 0, nullptr};
-      r.n = 3; r.splits = w.splits; r.stride = w.split_stride;
-      launch_reduce<F16>(r, s);
-    }
-    if (cs_n) hipLaunchKernelGGL((colsum_kernel<F16>), dim3((unsigned)row_blocks, (unsigned)((N8 / 8 + 63) / 64)), dim3(256), 0, s, y.p, y.ld, cs_n, N8,
-                                 (long long)M, a.N);
-    if (cs_f || cs_n) {
-      ColReduceParams r{};
-      int n = 0, widest = 1;
-      auto add = [&](float* src, void* out, long long count, int pitch_, int c) {
-        if (!out) return;
-        r.r[n++] = ColReduce{src, out, count, pitch_, c};
-        widest = std::max(widest, c);
-      };
-      add(cs_f, o->db_gate, parts, F8, a.F);
-      add(cs_f ? cs_f + (size_t)parts * F8 : nullptr, o->db_up, parts, F8, a.F);
-      add(cs_n, o->db_down, row_blocks, N8, a.N);
-      r.f16 = F16; r.out_f32 = a.bias_f32;
-      hipLaunchKernelGGL(col_reduce_kernel, dim3((unsigned)((widest + 63) / 64), (unsigned)n), dim3(1024), 0, s, r);
-    }
+    if (o->dx) add_out_reduce(r, xplan, dx, M, a.K, xp);
+    void* outs[3] = {o->dw_gate, o->dw_up, o->dw_down};
+    for (int i = 0; i < 3 && part; ++i)
+      r.r[r.nr++] = SplitReduce{part + i * one, (h16*)outs[i], cols[i], pitch[i], rows[i], w.split_stride, w.splits, cols[i],
+                                cols[i] % 8 == 0 && (uintptr_t)outs[i] % 16 == 0, nullptr};
+    auto add = [&](const float* src, void* out, long long count, int pitch_, int c) {
+      if (out) r.c[r.nc++] = ColReduce{src, out, count, pitch_, c};
+    };
+    add(cs_f, o->db_gate, parts, F8, a.F);
+    add(cs_f ? cs_f + (size_t)parts * F8 : nullptr, o->db_up, parts, F8, a.F);
+    add(cs_n, o->db_down, row_blocks, N8, a.N);
+    launch_reduce<F16>(r, s);
   });
   return ar.used;
 }

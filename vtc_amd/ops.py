@@ -12,6 +12,7 @@ a training step into a graph uses the explicit ones, or makes the differentiable
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import numpy as np
@@ -63,6 +64,20 @@ _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurr
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _bytes(entry: str, *sizes) -> int:
+    """What a size query of the library answers; it depends on nothing but the sizes."""
+    n = getattr(_library(), entry)(*sizes)
+    if n < 0:
+        L.check(int(n))
+    return n
+
+
+def _empty(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor like t (empty_like without a format is the cheapest way to one)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _workspace(n: int, x: torch.Tensor) -> torch.Tensor:
@@ -287,7 +302,7 @@ def _rows3(t):
 
 def _gn_out(what, x, out):
     if out is None:
-        return torch.empty_like(x, memory_format=torch.contiguous_format)
+        return _empty(x)
     _same(what, x, "out", out)
     if out.shape != x.shape or (out.numel() and out.stride(2) != 1):
         raise ValueError(f"{what}: out must have shape {tuple(x.shape)} with contiguous channels")
@@ -309,9 +324,7 @@ def group_norm_act_forward(x: torch.Tensor, groups: int, weight=None, bias=None,
         rstd.zero_()
         return out, mean, rstd
     so = _library()
-    size = so.vtc_group_norm_act_workspace(n, t, c, groups, 0)
-    if size < 0:
-        L.check(int(size))
+    size = _bytes("vtc_group_norm_act_workspace", n, t, c, groups, 0)
     ws = _workspace(size, x)
     rc = so.vtc_group_norm_act(index, dt, _rows3(x), _rows3(out), n, t, c, groups, _ptr(weight), _ptr(bias), f32, eps, ACTS[act], _ptr(lengths),
                                mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), size, _stream(index))
@@ -336,9 +349,7 @@ def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, groups: int, mean
     dw = None if weight is None else torch.empty_like(weight)
     db = None if bias is None else torch.empty_like(bias)
     so = _library()
-    size = so.vtc_group_norm_act_workspace(n, t, c, groups, 1)
-    if size < 0:
-        L.check(int(size))
+    size = _bytes("vtc_group_norm_act_workspace", n, t, c, groups, 1)
     ws = _workspace(size, x)
     rc = so.vtc_group_norm_act_backward(index, dt, _rows3(dy), _rows3(x), _rows3(out), n, t, c, groups, _ptr(weight), _ptr(bias), f32, ACTS[act],
                                         _ptr(lengths), mean.data_ptr(), rstd.data_ptr(), _ptr(dw), _ptr(db), ws.data_ptr(), size, _stream(index))
@@ -429,14 +440,12 @@ def gated_ffn_forward(x: torch.Tensor, w_gate, w_up, w_down, b_gate=None, b_up=N
     index, dt, f32, k, f, n = _ffn_args(what, x, w_gate, w_up, w_down, (b_gate, b_up, b_down), act)
     rows = _rows2(x)
     m = rows.shape[0]
-    y = torch.empty_like(x, memory_format=torch.contiguous_format) if n == k else torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    y = _empty(x) if n == k else torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
     so = _library()
-    size = so.vtc_gated_ffn_workspace(m, k, f, n, 0)
-    if size < 0:
-        L.check(int(size))
+    size = _bytes("vtc_gated_ffn_workspace", m, k, f, n, 0)
     saved, saved_size = None, 0
     if save:
-        saved_size = so.vtc_gated_ffn_saved(m, f)
+        saved_size = _bytes("vtc_gated_ffn_saved", m, f)
         saved = _workspace(saved_size, x)
     if m == 0:
         return y, saved
@@ -463,20 +472,17 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate, w_up, w_down, 
         raise ValueError(f"{what}: bias_dtype must be {x.dtype} or float32")
     rows, drows = _rows2(x), _rows2(dy)
     m = rows.shape[0]
-    new = lambda shape, kind: torch.empty(shape, dtype=kind, device=x.device)  # noqa: E731
-    dx = new(x.shape, x.dtype) if need_dx else None
-    dw = tuple(new(w.shape, x.dtype) if need_dw else None for w in (w_gate, w_up, w_down))
-    db = tuple(new((c,), bias_dtype) if biases else None for c in (f, f, n))
+    dx = _empty(x) if need_dx else None
+    dw = (_empty(w_gate), _empty(w_up), _empty(w_down)) if need_dw else (None, None, None)
+    db = tuple(x.new_empty((c,)) if bias_dtype is x.dtype else x.new_empty((c,), dtype=bias_dtype) for c in (f, f, n)) if biases else (None, None, None)
     if m == 0:
         for t in dw + db:
             if t is not None:
                 t.zero_()
         return (dx,) + dw + db
     so = _library()
-    size = so.vtc_gated_ffn_workspace(m, k, f, n, 1)
-    if size < 0:
-        L.check(int(size))
-    if saved is None or not saved.is_cuda or saved.get_device() != index or saved.dtype is not torch.uint8 or saved.numel() < so.vtc_gated_ffn_saved(m, f):
+    size = _bytes("vtc_gated_ffn_workspace", m, k, f, n, 1)
+    if saved is None or not saved.is_cuda or saved.get_device() != index or saved.dtype is not torch.uint8 or saved.numel() < _bytes("vtc_gated_ffn_saved", m, f):
         raise ValueError(f"{what}: saved is the forward call's (with save=True)")
     ws = _workspace(size, x)
     grads = L.VtcFfnGrads(_ptr(dx), k, *(_ptr(t) for t in dw + db))
