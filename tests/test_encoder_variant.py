@@ -46,7 +46,10 @@ def test_every_stage_of_a_variant_against_the_oracle(name, dtype):
     """The bars of the base encoder's stage test (f16 storage: 1e-2 / 1.5e-2 on conv and hidden rows of unit scale, 2e-2 on logits;
     bf16 storage: 8 times the rounding)."""
     variant = VARIANTS[name]
-    conv_tol, hid_tol, logit_tol = (1e-2, 1.5e-2, 2e-2) if dtype == "f16" else (6e-2, 1.2e-1, 1.5e-1)
+    # Everything between two stores is fp32, so a stage's error is, to first order, linear in the stores' half step, 2^-11 (f16) and 2^-8
+    # (bf16) of a value: 8 x 1e-2 on conv rows.  (The base encoder's bf16 bar of 6e-2 holds for one store per conv layer; a layer with
+    # its own norm stores twice, the conv's rows and the normed ones: up to 2 x 6e-2.)
+    conv_tol, hid_tol, logit_tol = (1e-2, 1.5e-2, 2e-2) if dtype == "f16" else (8e-2, 1.2e-1, 1.5e-1)
     w = variant_state(variant)
     B, W = 3, 16000
     T = O.conv_out_len(W)

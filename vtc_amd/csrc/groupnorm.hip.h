@@ -9,11 +9,11 @@
 // Two forms.  Samples that fit a block's registers are read once (gn_slab_kernel, gn_bwd_slab_kernel); everything else - long or odd
 // samples, wide groups, strides that are no whole vectors - streams: statistics per row block, merge, elementwise pass, in which x (and
 // dy) are read a second time, last rows first, since those are still in the last-level cache.  Bound: memory and the activation's
-// vector instructions (about 25 issue slots of an element for GELU, 83 us of 131 M elements), which add up: 64 x 3999 x 512 f16 with
-// GELU takes 206 us on chip where its 524 MB alone take 105, and 198 streaming.  Figures of both forms: kGnSlabFwd in vtc_ops.hip.
-// 5 x 1531 x 201 fp32 (streaming, 4-byte accesses): statistics 5, elementwise 12, backward sums 7, merges 4 + 3, dx 7 us.
+// vector instructions (about 25 issue slots of an element for GELU, 83 us of 131 M elements).  64 x 3999 x 512 f16 with GELU (524 MB,
+// 105 us at a copy's rate) streams in 64 (statistics) + 5 + 104 us.  Figures of both forms: kGnSlabVectors in vtc_ops.hip.
+// 5 x 1531 x 201 fp32 (streaming, 4-byte accesses): statistics 5, elementwise 11, backward sums 7, merges 4 + 3, dx 7 us.
 //
-// Statistics: every partial is (mean, M2 = sum of squared distances from it) and partials merge by Chan's formula, so a mean
+// Statistics: every partial is (mean, M2 = sum of squared distances from it) and partials merge about their common mean, so a mean
 // that is large against the spread does not cancel; inside a thread the sums are of x - x_first (the row block's first row, per
 // channel), in fp32 over at most a few hundred rows; merges across row blocks are fp64.  All orders are fixed, no atomics:
 // results are bit-reproducible.
@@ -133,38 +133,43 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const GnParams p) {
   }
 }
 
-// ---- merge the row blocks of a sample: 16 groups x 16 threads, thread i takes row blocks i, i + 16, .., their results merge in order
-struct GnMoment { double mean, m2, cnt; };
-__device__ __forceinline__ void gn_merge(GnMoment& a, double mean, double m2, double cnt) {   // Chan's formula
-  if (cnt == 0.0) return;
-  const double d = mean - a.mean, tot = a.cnt + cnt;
-  a.mean += d * (cnt / tot);
-  a.m2 += m2 + d * d * (a.cnt * cnt / tot);
-  a.cnt = tot;
+// ---- merge the row blocks of a sample: 16 groups x 16 threads, thread i takes row blocks i, i + 16, ..  First the mean, then the squared
+// distances from it, in fp64: one division per group (Chan's formula pairwise takes two per partial: 21 us instead of 5 for 64 x 3999 rows in
+// 32 groups).
+__device__ __forceinline__ double gn_slices(double v, double (*sh)[16], int slice, int in) {   // sum over the 16 threads of a group, in a tree
+  __syncthreads();
+  sh[slice][in] = v;
+  __syncthreads();
+  for (int h = 8; h > 0; h >>= 1) {
+    if (slice < h) sh[slice][in] += sh[slice + h][in];
+    __syncthreads();
+  }
+  return sh[0][in];
 }
 // mean and rstd of 16 groups from g0 on, by a block of 256; stat: [16] results for the block
-__device__ __forceinline__ void gn_finalize(const GnParams& p, long long n, int g0, GnMoment (*sh)[16], float2* stat) {
+__device__ __forceinline__ void gn_finalize(const GnParams& p, long long n, int g0, double (*sh)[16], float2* stat) {
   const int in = threadIdx.x & 15, g = g0 + in, slice = threadIdx.x >> 4;
   const long long len = gn_length(p, n);
-  GnMoment a{0.0, 0.0, 0.0};
-  if (g < p.G) {
-    const float2* part = (const float2*)p.part + n * p.chunks * p.G + g;
-    const int live = (int)min((long long)p.chunks, (len + p.rows - 1) / p.rows);
-    for (int k = slice; k < live; k += 16) {
-      const float2 t = part[(long long)k * p.G];
-      gn_merge(a, t.x, t.y, (double)min((long long)p.rows, len - (long long)k * p.rows) * p.cpg);
-    }
+  const float2* part = (const float2*)p.part + n * p.chunks * p.G + g;
+  const int live = g < p.G ? (int)min((long long)p.chunks, (len + p.rows - 1) / p.rows) : 0;
+  auto rows = [&](int k) { return (double)min((long long)p.rows, len - (long long)k * p.rows); };
+  double s = 0.0;
+#pragma unroll 4
+  for (int k = slice; k < live; k += 16) s += rows(k) * part[(long long)k * p.G].x;
+  const double mean = len > 0 ? gn_slices(s, sh, slice, in) / (double)len : 0.0;
+  s = 0.0;
+#pragma unroll 4
+  for (int k = slice; k < live; k += 16) {
+    const float2 t = part[(long long)k * p.G];
+    const double d = t.x - mean;
+    s += t.y + rows(k) * p.cpg * d * d;
   }
-  sh[slice][in] = a;
-  __syncthreads();
-  if (slice == 0 && g < p.G) {
-    for (int i = 1; i < 16; ++i) { const GnMoment& o = sh[i][in]; gn_merge(a, o.mean, o.m2, o.cnt); }
-    stat[in] = make_float2((float)a.mean, a.cnt > 0.0 ? (float)(1.0 / sqrt(a.m2 / a.cnt + (double)p.eps)) : 0.f);
-  }
+  s = gn_slices(s, sh, slice, in);
+  if (slice == 0 && g < p.G) stat[in] = make_float2((float)mean, len > 0 ? (float)(1.0 / sqrt(s / ((double)len * p.cpg) + (double)p.eps)) : 0.f);
   __syncthreads();
 }
 __global__ __launch_bounds__(256) void gn_finalize_kernel(const GnParams p) {
-  __shared__ GnMoment sh[16][16];
+  __shared__ double sh[16][16];
   __shared__ float2 stat[16];
   const unsigned per = (unsigned)(p.G + 15) / 16;
   const long long n = blockIdx.x / per;
@@ -184,7 +189,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
   const long long n = blk / (unsigned)p.achunks;
   const long long len = gn_length(p, n), r0 = (long long)(blk % (unsigned)p.achunks) * p.arows;
   const int rows = (int)min((long long)p.arows, p.L - r0);
-  __shared__ GnMoment sh[16][16];
+  __shared__ double sh[16][16];
   __shared__ float2 stat[kGnMergeHere];
   if (p.merge_here) {
     for (int g0 = 0; g0 < p.G; g0 += 16) gn_finalize(p, n, g0, sh, stat + g0);
@@ -431,8 +436,8 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnParams p) {
 }
 
 // ---- whole samples on chip: one block owns `bc` channels (whole groups, at least 32 B of a row) of one sample and keeps its rows in
-// registers, so x (and dy) are read once.  512 threads, NV 16-byte vectors each: vector i of thread t is piece (t + 512 i), piece
-// = row * cvb + channel vector.  Bound: HBM and the activation's VALU work, about equal.  Neighbouring
+// registers, so x (and dy) are read once.  256 threads (backward 512), NV 16-byte vectors each: vector i of thread t is piece
+// t + threads * i, piece = row * cvb + channel vector.  Bound: HBM and the activation's VALU work, about equal.  Neighbouring
 // blocks share 128-byte lines and run on one XCD (xcd_remap), so the L2 serves the other parts of a line.
 template <int DT> struct GnVec {
   static constexpr int VEC = 16 / (int)sizeof(typename OpType<DT>::T);
@@ -466,7 +471,7 @@ __device__ __forceinline__ float gn_row_sum(float v, int cvb) {
   return v;
 }
 constexpr int kGnMaxCvb = 8;
-constexpr int kGnSlabThreads = 512;
+constexpr int kGnSlabThreads = 256, kGnSlabBwdThreads = 512;
 
 // Block sums of NQ values per channel vector: v in every thread on entry, tot[vector * NQ + k] on exit.  Fixed order.
 template <int NQ, int THREADS> __device__ __forceinline__ void gn_block_sums(const float (&v)[NQ], int cvb, float* red, float* tot) {
@@ -489,17 +494,17 @@ template <int NQ, int THREADS> __device__ __forceinline__ void gn_block_sums(con
   __syncthreads();
 }
 
-template <int DT, int NV, int ACT, int THREADS>
-__global__ __launch_bounds__(THREADS, 4) void gn_slab_kernel(const GnParams p) {
+template <int DT, int NV, int ACT>
+__global__ __launch_bounds__(kGnSlabThreads, 4) void gn_slab_kernel(const GnParams p) {
   typedef typename OpType<DT>::T T;
   constexpr int VEC = GnVec<DT>::VEC;
-  __shared__ float red[THREADS / 16 * kGnMaxCvb * VEC], tot[kGnMaxCvb * VEC], gmean[kGnMaxCvb * VEC], grstd[kGnMaxCvb * VEC];
+  __shared__ float red[kGnSlabThreads / 16 * kGnMaxCvb * VEC], tot[kGnMaxCvb * VEC], gmean[kGnMaxCvb * VEC], grstd[kGnMaxCvb * VEC];
   const int cvb = p.cvb, bc = cvb * VEC, bundles = p.C / bc;
   const int sh = 31 - __builtin_clz(p.cpg), ngb = bc >> sh;   // groups divide a power of two here: they are powers of two
   const unsigned blk = xcd_remap(blockIdx.x, gridDim.x);
   const long long n = blk / (unsigned)bundles;
   const int c_base = (int)(blk % (unsigned)bundles) * bc;
-  const int v = threadIdx.x & (cvb - 1), r0 = threadIdx.x / cvb, dr = THREADS / cvb;
+  const int v = threadIdx.x & (cvb - 1), r0 = threadIdx.x / cvb, dr = kGnSlabThreads / cvb;
   const long long len = gn_length(p, n);
   const int real = (int)len;
   const T* x = (const T*)p.x + n * p.xn + c_base + v * VEC;
@@ -537,7 +542,7 @@ __global__ __launch_bounds__(THREADS, 4) void gn_slab_kernel(const GnParams p) {
   }
 #pragma unroll
   for (int k = 0; k < VEC; ++k) v0[k] = fmaf(fc, first[k] - v0[k], s[k]);
-  gn_block_sums<VEC, THREADS>(v0, cvb, red, tot);
+  gn_block_sums<VEC, kGnSlabThreads>(v0, cvb, red, tot);
   const float inv = real > 0 ? 1.f / ((float)real * (float)p.cpg) : 0.f;
   if ((int)threadIdx.x < ngb) {
     // the group's mean from its first channel's value in row 0 on: fp32 loses nothing to a mean far from zero
@@ -558,7 +563,7 @@ __global__ __launch_bounds__(THREADS, 4) void gn_slab_kernel(const GnParams p) {
     const float d = fmaf(s[k], ic, first[k] - mu[k]);          // the thread's mean, from the group's
     v0[k] = cnt > 0 ? fmaf(fc * d, d, fmaf(-s[k], s[k] * ic, q[k])) : 0.f;
   }
-  gn_block_sums<VEC, THREADS>(v0, cvb, red, tot);
+  gn_block_sums<VEC, kGnSlabThreads>(v0, cvb, red, tot);
   if ((int)threadIdx.x < ngb) {
     float t = 0.f;
     for (int c = 0; c < p.cpg; ++c) t += tot[threadIdx.x * p.cpg + c];
@@ -598,16 +603,16 @@ __global__ __launch_bounds__(THREADS, 4) void gn_slab_kernel(const GnParams p) {
 
 // backward of the same: x stays in registers, and dz in fp32, so the slope is computed once
 template <int DT, int NV, int ACT>
-__global__ __launch_bounds__(kGnSlabThreads, NV <= 4 ? 4 : 2) void gn_bwd_slab_kernel(const GnParams p) {
+__global__ __launch_bounds__(kGnSlabBwdThreads, NV <= 4 ? 4 : 2) void gn_bwd_slab_kernel(const GnParams p) {
   typedef typename OpType<DT>::T T;
   constexpr int VEC = GnVec<DT>::VEC;
-  __shared__ float red[kGnSlabThreads / 16 * kGnMaxCvb * 2 * VEC], tot[kGnMaxCvb * 2 * VEC], gA[kGnMaxCvb * VEC], gB[kGnMaxCvb * VEC];
+  __shared__ float red[kGnSlabBwdThreads / 16 * kGnMaxCvb * 2 * VEC], tot[kGnMaxCvb * 2 * VEC], gA[kGnMaxCvb * VEC], gB[kGnMaxCvb * VEC];
   const int cvb = p.cvb, bc = cvb * VEC, bundles = p.C / bc;
   const int sh = 31 - __builtin_clz(p.cpg), ngb = bc >> sh;   // groups divide a power of two here: they are powers of two
   const unsigned blk = xcd_remap(blockIdx.x, gridDim.x);
   const long long n = blk / (unsigned)bundles;
   const int c_base = (int)(blk % (unsigned)bundles) * bc;
-  const int v = threadIdx.x & (cvb - 1), r0 = threadIdx.x / cvb, dr = kGnSlabThreads / cvb;
+  const int v = threadIdx.x & (cvb - 1), r0 = threadIdx.x / cvb, dr = kGnSlabBwdThreads / cvb;
   const int real = (int)gn_length(p, n);
   const T* x = (const T*)p.x + n * p.xn + c_base + v * VEC;
   const T* dy = (const T*)p.dy + n * p.dn + c_base + v * VEC;
@@ -649,7 +654,7 @@ __global__ __launch_bounds__(kGnSlabThreads, NV <= 4 ? 4 : 2) void gn_bwd_slab_k
         s[VEC + k] = fmaf(dz, h, s[VEC + k]);
       }
     }
-  gn_block_sums<2 * VEC, kGnSlabThreads>(s, cvb, red, tot);
+  gn_block_sums<2 * VEC, kGnSlabBwdThreads>(s, cvb, red, tot);
   if ((int)threadIdx.x < bc) {   // a channel's sums: for the affine's gradients, and into its group
     const int vv = threadIdx.x / VEC, k = threadIdx.x % VEC;
     double* o = p.sums + (n * p.C + c_base + threadIdx.x) * 2;

@@ -215,25 +215,28 @@ namespace {
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Rows of a block, by the length alone: a sample's result must not depend on how many samples share the call.
-void gn_shape(long long L, int* rows, int* chunks) {
-  long long r = (L + 63) / 64;
-  r = std::max<long long>(r, 16);
-  r = std::min<long long>(r, 256);
+// Rows of a block, by the length and the channels alone: a sample's result must not depend on how many samples share the call.  Blocks of
+// many rows pay their joins less often, blocks of few fill the chip with few samples: 64 x 3999 x 512 f16 + GELU forward takes 213 us
+// with 128 blocks of a sample, 194 with 64, 178 with 32, 178 with 16; one such sample 21, 21, 23, 29; 64 x 7999 340, 312, 323, 326.
+// Channels that are no whole vectors go one per thread, with fewer rows side by side.
+void gn_shape(long long L, int C, int* rows, int* chunks) {
+  const int split = C % 8 == 0 ? 32 : 64;
+  const long long r = std::min<long long>(std::max<long long>((L + split - 1) / split, 16), 128);
   *rows = (int)r;
   *chunks = (int)std::max<long long>(1, (L + r - 1) / r);
 }
-// Most 16-byte vectors of a block, in units of 512.  Measured, f16 + GELU, 512 channels in 32 groups, whole-sample blocks against
-// the streaming kernels (us): forward 64 x 499 rows 26 / 47, 64 x 1999 83 / 101, 64 x 3999 (16) 206 / 198, but 8 x 3999 26 / 42 and
-// 1 x 3999 18 / 23; backward 64 x 499 51 / 76, 64 x 1999 (8) 199 / 193, 24 x 1999 in 512 groups 61 / 101, 64 x 3999 444 / 302.
-constexpr int kGnSlabFwd = 16, kGnSlabBwd = 8;
+// Most 16-byte vectors of a whole-sample block.  Measured, f16 + GELU, 512 channels in 32 groups, whole-sample blocks against the
+// streaming kernels (us): forward 64 x 499 rows 26 / 46, 64 x 999 43 / 59, 64 x 1999 83 / 89; 64 x 3999 (blocks of twice this size)
+// 206 / 182, where 8 x 3999 would take 26 / 42 and 1 x 3999 19 / 24 (the large batch decides: the choice must not look at it).  Backward 64 x 499 51 / 64, 64 x 999 70 / 87, 24 x 1999 in 512
+// groups 62 / 99, 64 x 1999 199 / 162 (beyond the last-level cache), 64 x 3999 444 / 305.
+constexpr long long kGnSlabVectors = 4096;
 // Channel vectors of a whole-sample block (0: the sample does not fit, or its groups do not divide into such blocks).
 // 2 vectors are 32 bytes of a row, the least that a fetch of a 64-byte half line uses well; wider groups take 4 or 8.
-int gn_slab(int dtype, int vec, long long L, int C, int cpg, int most) {
+int gn_slab(int dtype, int vec, long long L, int C, int cpg) {
   const int v16 = 16 / esize(dtype);
   if (vec != v16) return 0;
   for (int cvb = 2; cvb <= kGnMaxCvb; cvb *= 2)
-    if ((cvb * v16) % cpg == 0 && C % (cvb * v16) == 0) return L * cvb <= (long long)kGnSlabThreads * most ? cvb : 0;
+    if ((cvb * v16) % cpg == 0 && C % (cvb * v16) == 0) return L * cvb <= kGnSlabVectors ? cvb : 0;
   return 0;
 }
 
@@ -248,7 +251,7 @@ int gn_check(const char* what, int dtype, int affine_f32, const vtc_rows3* const
   if (L > (1ll << 40) || N > (1ll << 40) / L) return fail_handleless(VTC_ERR_ARG, "%s: too many rows", what);
   int rows, chunks;
   if (L > (long long)256 * 0x7ffffff) return fail_handleless(VTC_ERR_ARG, "%s: too many rows", what);
-  gn_shape(L, &rows, &chunks);
+  gn_shape(L, C, &rows, &chunks);
   if (N * ((L + 3) / 4) > 0x7fff0000 || N * (long long)chunks > 0x7fffffff || N * (long long)((C + 7) / 8) > 0x7fffffff) return fail_handleless(VTC_ERR_ARG, "%s: too many rows", what);
   for (int i = 0; i < n_t; ++i) {
     const vtc_rows3& t = *ts[i];
@@ -276,14 +279,14 @@ int gn_check(const char* what, int dtype, int affine_f32, const vtc_rows3* const
   return VTC_OK;
 }
 
-size_t gn_forward_bytes(int64_t N, int64_t L, int G) {
+size_t gn_forward_bytes(int64_t N, int64_t L, int C, int G) {
   int rows, chunks;
-  gn_shape(L, &rows, &chunks);
+  gn_shape(L, C, &rows, &chunks);
   return align256((size_t)N * chunks * G * 8);
 }
 size_t gn_backward_bytes(int64_t N, int64_t L, int C, int G) {
   int rows, chunks;
-  gn_shape(L, &rows, &chunks);
+  gn_shape(L, C, &rows, &chunks);
   return align256((size_t)N * chunks * C * 8) + align256((size_t)N * (C + G) * 16);
 }
 
@@ -291,7 +294,7 @@ GnParams gn_params(int64_t N, int64_t L, int C, int G, const void* w, const void
   GnParams p{};
   p.N = N; p.L = L; p.C = C; p.G = G; p.cpg = C / G;
   p.w = w; p.b = b; p.affine_f32 = affine_f32; p.length = lengths;
-  gn_shape(L, &p.rows, &p.chunks);
+  gn_shape(L, C, &p.rows, &p.chunks);
   // the elementwise pass: ~2000 blocks where there are rows for it, at least 4 rows and at most 64
   p.arows = (int)std::min<long long>(64, std::max<long long>(4, N * L / 2048));
   p.achunks = (int)((L + p.arows - 1) / p.arows);
@@ -307,7 +310,7 @@ extern "C" int64_t vtc_group_norm_act_workspace(int64_t batch, int64_t length, i
     return VTC_ERR_ARG;
   }
   if (batch == 0 || length == 0) return 0;
-  return (int64_t)(backward ? gn_backward_bytes(batch, length, channels, groups) : gn_forward_bytes(batch, length, groups));
+  return (int64_t)(backward ? gn_backward_bytes(batch, length, channels, groups) : gn_forward_bytes(batch, length, channels, groups));
 }
 
 extern "C" int vtc_group_norm_act(int device, int dtype, const vtc_rows3* x, const vtc_rows3* y, int64_t batch, int64_t length,
@@ -320,7 +323,7 @@ extern "C" int vtc_group_norm_act(int device, int dtype, const vtc_rows3* x, con
   if (!(eps >= 0.0) || !std::isfinite(eps)) return fail_handleless(VTC_ERR_ARG, "group norm: eps must be finite and not negative");
   if (batch == 0 || length == 0) return VTC_OK;
   if (!mean || !rstd) return fail_handleless(VTC_ERR_ARG, "group norm: mean and rstd are needed");
-  const size_t need = gn_forward_bytes(batch, length, groups);
+  const size_t need = gn_forward_bytes(batch, length, channels, groups);
   if (!workspace || workspace_bytes < (int64_t)need) return fail_handleless(VTC_ERR_CAPACITY, "group norm: the workspace holds %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   if ((uintptr_t)workspace % 256) return fail_handleless(VTC_ERR_ARG, "group norm: the workspace is not aligned to 256 bytes");
   DeviceGuard guard(device);
@@ -332,15 +335,13 @@ extern "C" int vtc_group_norm_act(int device, int dtype, const vtc_rows3* x, con
   const int vec = vec_of(dtype, {channels, eff(x->batch, batch), eff(x->row, length), eff(y->batch, batch), eff(y->row, length)}, {x->p, y->p});
   p.cv = channels / vec;
   hipStream_t s = (hipStream_t)stream;
-  if ((p.cvb = gn_slab(dtype, vec, length, channels, p.cpg, kGnSlabFwd))) {
+  if ((p.cvb = gn_slab(dtype, vec, length, channels, p.cpg))) {
     const unsigned n = (unsigned)(batch * (channels / (p.cvb * vec)));
-    const long long pieces = length * p.cvb;   // 16-byte vectors of a block: 256 threads of 4 or 16, 512 of 16
     by_type(dtype, [&](auto d) { by_act(act, [&](auto a) {
       constexpr int DT = decltype(d)::value, ACT = decltype(a)::value;
       if constexpr (ACT != ACT_SIGMOID) {
-        if (pieces <= 256 * 4) hipLaunchKernelGGL((gn_slab_kernel<DT, 4, ACT, 256>), dim3(n), dim3(256), 0, s, p);
-        else if (pieces <= 256 * 16) hipLaunchKernelGGL((gn_slab_kernel<DT, 16, ACT, 256>), dim3(n), dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((gn_slab_kernel<DT, 16, ACT, 512>), dim3(n), dim3(512), 0, s, p);
+        if (length * p.cvb <= 256 * 4) hipLaunchKernelGGL((gn_slab_kernel<DT, 4, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
+        else hipLaunchKernelGGL((gn_slab_kernel<DT, 16, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
       }
     }); });
     return launched("group norm");
@@ -395,15 +396,15 @@ extern "C" int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows
   const int vec = vec_of(dtype, {channels, eff(x->batch, batch), eff(x->row, length), eff(dy->batch, batch), eff(dy->row, length),
                                  eff(dx->batch, batch), eff(dx->row, length)}, {x->p, dy->p, dx->p});
   p.cv = channels / vec;
-  if ((p.cvb = gn_slab(dtype, vec, length, channels, p.cpg, kGnSlabBwd))) {
+  if ((p.cvb = gn_slab(dtype, vec, length, channels, p.cpg))) {
     const unsigned n = (unsigned)(batch * (channels / (p.cvb * vec)));
-    const int nv = (int)((length * p.cvb + kGnSlabThreads - 1) / kGnSlabThreads);
+    const int nv = (int)((length * p.cvb + kGnSlabBwdThreads - 1) / kGnSlabBwdThreads);
     by_type(dtype, [&](auto d) { by_act(act, [&](auto a) {
       constexpr int DT = decltype(d)::value, ACT = decltype(a)::value;
       if constexpr (ACT != ACT_SIGMOID) {
-        if (nv <= 2) hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 2, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
-        else if (nv <= 4) hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 4, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
-        else hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 8, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
+        if (nv <= 2) hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 2, ACT>), dim3(n), dim3(kGnSlabBwdThreads), 0, s, p);
+        else if (nv <= 4) hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 4, ACT>), dim3(n), dim3(kGnSlabBwdThreads), 0, s, p);
+        else hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 8, ACT>), dim3(n), dim3(kGnSlabBwdThreads), 0, s, p);
       }
       if (dweight || dbias) hipLaunchKernelGGL((gn_affine_grads_kernel<DT>), dim3(grad_blocks), dim3(256), 0, s, p);
     }); });
