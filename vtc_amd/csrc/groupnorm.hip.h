@@ -10,7 +10,7 @@
 // samples, wide groups, strides that are no whole vectors - streams: statistics per row block, merge, elementwise pass, in which x (and
 // dy) are read a second time, last rows first, since those are still in the last-level cache.  Bound: memory and the activation's
 // vector instructions (about 25 issue slots of an element for GELU, 83 us of 131 M elements).  64 x 3999 x 512 f16 with GELU (524 MB,
-// 105 us at a copy's rate) streams in 64 (statistics) + 5 + 104 us.  Figures of both forms: kGnSlabVectors in vtc_ops.hip.
+// 105 us at a copy's rate) streams in 64 (statistics) + 5 + 104 us, 186 with its launches.  Figures of both forms: kGnSlabVectors in vtc_ops.hip.
 // 5 x 1531 x 201 fp32 (streaming, 4-byte accesses): statistics 5, elementwise 11, backward sums 7, merges 4 + 3, dx 7 us.
 //
 // Statistics: every partial is (mean, M2 = sum of squared distances from it) and partials merge about their common mean, so a mean
