@@ -1,0 +1,50 @@
+"""Host-side arithmetic of the feed-forward operators' matrix products, in C++ programs built from the library's own headers."""
+
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+def build(tmp_path, source):
+    if shutil.which("g++") is None:
+        pytest.skip("no g++")
+    exe = tmp_path / Path(source).stem
+    b = subprocess.run(["g++", "-O1", "-std=c++17", "-I", str(ROOT / "vtc_amd" / "csrc"), str(ROOT / "tests" / source), "-o", str(exe)],
+                       capture_output=True, text=True, timeout=300)
+    assert b.returncode == 0, b.stderr[-2000:]
+    return exe
+
+
+def halves(columns, tile, most=128):
+    """First columns of the half-tiles of a product's last tile."""
+    last = (columns - 1) // tile * tile
+    return [last] if tile <= most else [last, last + 128]
+
+
+def test_operand_windows_stay_inside_the_operand(tmp_path):
+    """Every K-tile of dx (two segments, 192-wide tiles) and of the weights' gradients (256-wide tiles, long contractions), also where
+    the second half of the last tile lies wholly behind the matrix and at K-tiles whose row offsets pass 2^31 bytes."""
+    lines = []
+    # dx: contraction over `inner`, columns of the width; K-tiles of both segments run on a half that has no columns
+    for width, inner in ((16384, 53248), (768, 2048), (389, 1031), (8, 8), (1, 1), (100, 262144), (262144, 262144), (200000, 100000), (4096 + 64, 262144)):
+        pitch = (width + 7) // 8 * 8
+        for ld in (pitch, 1 << 20):
+            for c0 in halves(width, 192):
+                tiles = 2 * ((inner + 63) // 64)
+                lines.append((inner, ld, width, c0, 128, (tiles + 1) & ~1, 2))
+            lines.append((inner, ld, width, (width - 1) // 64 * 64, 64, 2 * ((inner + 63) // 64), 2))
+    # the weights' gradients: contraction over the rows, columns of `inner`, of the width or of the output
+    for rows, columns in ((78400, 13696), (200000, 13696), (2 ** 31 - 256, 8), (1_000_003, 4104), (31936, 2048), (1237, 389), (1, 1), (2 ** 24 + 1, 65)):
+        pitch = (columns + 7) // 8 * 8
+        for ld in (pitch, 1 << 20):
+            for c0 in halves(columns, 256):
+                lines.append((rows, ld, columns, c0, 128, ((rows + 63) // 64 + 1) & ~1, 1))
+            lines.append((rows, ld, columns, (columns - 1) // 64 * 64, 64, (rows + 63) // 64, 1))
+    exe = build(tmp_path, "op_extent_walk.cpp")
+    r = subprocess.run([str(exe)], input="\n".join(" ".join(map(str, x)) for x in lines), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout
+    assert f"{len(lines)} products walked" in r.stdout

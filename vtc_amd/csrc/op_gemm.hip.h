@@ -20,6 +20,7 @@
 #include "common.hip.h"
 #include "gemm256.hip.h"
 #include "op_act.hip.h"
+#include "op_extent.h"
 
 namespace vtc {
 
@@ -76,8 +77,6 @@ __device__ __forceinline__ float op_bias(const void* b, int i, int f32, bool f16
 }
 
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-// k-rows a descriptor of a K-strided half-tile spans: 64, and the most that 128 columns can run over at the least pitch of 8
-constexpr int kRowsAhead = 192;
 constexpr unsigned kOob = 0x80000000u;   // a buffer offset that is out of range of every descriptor used here
 
 // The output side of a tile: descriptors of [rows x cols left] windows, stores that drop what lies outside.
@@ -294,8 +293,8 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
   };
   auto half_ks = [&](Stream& d, const h16* base, long long ld, int col0, int cols, int k0, int K) {   // cols: left from col0
     d.p = (const char*)(base + (long long)k0 * ld + col0);
-    d.end = __builtin_amdgcn_readfirstlane(((max(min(cols, 128), 0) + 7) & ~7) * 2 - (int)ld * 2);   // (clamps are vector instructions)
-    d.left = cols > 0 ? K - k0 : 0;
+    d.end = __builtin_amdgcn_readfirstlane(ks_end(cols, 128, (int)ld));   // (clamps are vector instructions)
+    d.left = ks_left(cols, K, k0);
   };
   int cur_tm = 0, cur_tn = 0;   // tile being staged
   // operand A (half h) / B (half h) of segment s from contraction index k0 on
@@ -348,7 +347,7 @@ __global__ __launch_bounds__(512, 2) void op_gemm_kernel(const OpGemmParams p) {
   // N copies of 16 bytes per lane to LDS (everything that does not exist arrives as zero), then one K-tile on
   auto copies = [&](auto ks, auto count, Stream& d, int ld2, const unsigned* vo, const int* piece, char* lds) {
     constexpr bool KS = decltype(ks)::value;
-    const int end = KS ? __builtin_amdgcn_readfirstlane(max(min(d.left, kRowsAhead) * ld2 + d.end, 0)) : d.end;
+    const int end = KS ? __builtin_amdgcn_readfirstlane(ks_bytes(d.left, ld2, d.end)) : d.end;
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)d.p, 0, end, 0x00020000);
 #pragma unroll
     for (int i = 0; i < decltype(count)::value; ++i)
@@ -682,7 +681,7 @@ __device__ __forceinline__ void op_small_tile(const OpGemmParams& p, unsigned bl
   auto stream = [&](auto ks, const OpMat& A, int at, int exist, int most, int kk, int K) {
     const int ld2 = (int)A.ld * 2, K8 = (K + 7) & ~7;
     if constexpr (decltype(ks)::value)
-      return Stream{(const char*)(A.p + (long long)kk * A.ld + at), ((max(min(exist, most), 0) + 7) & ~7) * 2 - ld2, exist > 0 ? K - kk : 0};
+      return Stream{(const char*)(A.p + (long long)kk * A.ld + at), ks_end(exist, most, (int)A.ld), ks_left(exist, K, kk)};
     else
       return Stream{(const char*)(A.p + (long long)at * A.ld + kk), exist > 0 ? (min(exist, most) - 1) * ld2 + K8 * 2 : 0, K8 - kk};
   };
@@ -703,7 +702,7 @@ __device__ __forceinline__ void op_small_tile(const OpGemmParams& p, unsigned bl
       if (sa.left <= 0 && seg == 0) set_seg(1, 0);
     }
     char* l = smem + stage * kOsStage;
-    auto end = [](bool ks, const Stream& d, int ld2) { return ks ? __builtin_amdgcn_readfirstlane(max(min(d.left, kRowsAhead) * ld2 + d.end, 0)) : d.end; };
+    auto end = [](bool ks, const Stream& d, int ld2) { return ks ? __builtin_amdgcn_readfirstlane(ks_bytes(d.left, ld2, d.end)) : d.end; };
     const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)sa.p, 0, end(AKS, sa, lda2), 0x00020000);
     const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)sb.p, 0, end(BKS, sb, ldb2), 0x00020000);
 #pragma unroll
