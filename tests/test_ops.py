@@ -92,6 +92,41 @@ def test_rotary_scalings_far_and_negative_positions(scaling, factor):
     check_rotary(ops.rotary(x, spec, positions=pos), x, spec, pos)
 
 
+@pytest.mark.parametrize("rotary_dim", [2, 4, 6, 32, 64, 128])
+@pytest.mark.parametrize("base", [100.0, 10000.0, 500000.0])
+@pytest.mark.parametrize("length", [1, 3, 6, 7, 30, 200, 201, 202, 2048, 47_000, 48_000, 100_000, 3_000_000])
+def test_rotary_by_parts_frequencies_by_counting_turns(rotary_dim, base, length):
+    """The ramp's ends found by counting turns over the original length, pair by pair, on an index that runs on past the last pair."""
+    r, s = rotary_dim, 8.0
+    spec = ops.Rotary(r, base=base, scaling="by_parts", factor=s, original_length=length)
+    turns = [length * base ** (-2.0 * j / r) / (2.0 * math.pi) for j in range(r)]
+    if any(abs(t - e) < 1e-9 * e for t in turns for e in (1.0, 32.0)):
+        pytest.skip("a pair on the border itself")
+    low = max([j for j in range(r) if turns[j] > 32.0], default=0)
+    high = min([j for j in range(r) if turns[j] < 1.0], default=r - 1)
+    for j in range(r // 2):
+        f = base ** (-2.0 * j / r)
+        share = 1.0 if j >= high else 0.0 if j <= low else (j - low) / (high - low)   # of the division by the factor
+        assert spec.frequency[j] == pytest.approx(f * (1.0 - share) + f / s * share, rel=1e-12), j
+        if turns[j] < 1.0:
+            assert spec.frequency[j] == pytest.approx(f / s, rel=1e-12), j
+        if turns[j] > 32.0:
+            assert spec.frequency[j] == pytest.approx(f, rel=1e-12), j
+    assert spec.amplitude == pytest.approx(1.0 + 0.1 * math.log(s))
+
+
+@pytest.mark.parametrize("rotary_dim", [4, 64, 128])
+def test_rotary_ntk_and_linear_frequencies(rotary_dim):
+    """ntk leaves the first pair alone, divides the last one by the factor and spaces the others evenly in the logarithm between."""
+    r, s = rotary_dim, 8.0
+    plain, ntk, linear = (ops.Rotary(r, scaling=k, factor=s) for k in ("none", "ntk", "linear"))
+    j = np.arange(r // 2)
+    assert np.allclose(plain.frequency, 10000.0 ** (-j / (r / 2)), rtol=1e-13, atol=0)
+    assert np.allclose(ntk.frequency, plain.frequency * s ** (-j / (r / 2 - 1)), rtol=1e-12, atol=0)
+    assert np.allclose(linear.frequency * s, plain.frequency, rtol=1e-13, atol=0)
+    assert plain.amplitude == ntk.amplitude == linear.amplitude == 1.0
+
+
 @gpu
 def test_rotary_strides_in_place_and_broadcast():
     g = torch.Generator(device="cuda").manual_seed(6)

@@ -94,8 +94,8 @@ class Rotary:
     "linear":   frequency / factor
     "ntk":      base * factor ** (rotary_dim / (rotary_dim - 2)) in place of base
     "by_parts": pairs that turn more than 32 times over `original_length` positions keep their frequency, those that turn less
-                than once are divided by `factor`, between them a ramp linear in the pair's index; the result is multiplied by
-                1 + 0.1 ln(factor)
+                than once are divided by `factor`, between them (from pair 0 on, if none turns that often) a ramp linear in the
+                pair's index; the result is multiplied by 1 + 0.1 ln(factor)
 
     Frequencies are 64-bit; frequency= and amplitude= give the caller's own instead.  The object does not change once it is made."""
 
@@ -123,8 +123,11 @@ class Rotary:
         elif scaling == "by_parts":
             def index(turns):   # the pair that turns this often over the original length
                 return r * math.log(original_length / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
-            low, high = max(math.floor(index(32.0)), 0), min(math.ceil(index(1.0)), r // 2 - 1)
-            ramp = np.clip((j - low) / max(high - low, 1e-3), 0.0, 1.0)
+            # the ramp may end behind the last pair (index(1) counts on): clamped to it, a pair that still turns twice would be slowed
+            # by the whole factor.  Where not even pair 0 turns once, the ramp lies in front of it
+            high = min(math.ceil(index(1.0)), r - 1)
+            low = min(max(math.floor(index(32.0)), 0), high - 1)
+            ramp = np.clip((j - low) / (high - low), 0.0, 1.0)
             f = f / s * ramp + f * (1.0 - ramp)
             self.amplitude = 0.1 * math.log(s) + 1.0 if s > 1.0 else 1.0
         if frequency is not None:
