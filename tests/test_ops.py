@@ -929,3 +929,36 @@ def test_gated_ffn_refusals_with_tensors():
                 lambda: ops.gated_ffn_backward(dy, x, *w, saved, bias_dtype=torch.bfloat16)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_gated_ffn_pitch_of_a_single_row_is_not_looked_at(backward):
+    """x[:, -1] of a long recording.  No such device: what the argument checks let pass goes no further."""
+    so, far = L.load(), 1_536_000
+    mat = lambda at, row: C.byref(L.VtcMat(at, row))  # noqa: E731
+    for rows, pitch, ok in ((1, far, True), (1, 0, True), (1, -5, True), (2, far, False), (2, 767, False)):
+        x, w = mat(1 << 20, pitch), (mat(4 << 20, 768), mat(8 << 20, 768), mat(12 << 20, 256))
+        if backward:
+            grads = L.VtcFfnGrads(1 << 28, pitch, None, None, None)
+            rc = so.vtc_gated_ffn_backward(-1, 1, rows, 768, 256, 768, mat(16 << 20, pitch), x, *w, 32 << 20, 1 << 20, 0, C.byref(grads), 64 << 20, 1 << 27, None)
+        else:
+            rc = so.vtc_gated_ffn(-1, 1, rows, 768, 256, 768, x, *w, None, None, None, 0, 2, mat(16 << 20, pitch), None, 0, 64 << 20, 1 << 27, None)
+        msg = L.last_error(None)
+        assert rc != 0 and ("device" in msg if ok else "pitch" in msg), (rows, pitch, msg)
+
+
+@gpu
+@pytest.mark.parametrize("batch", [1, 2, 8, 70])
+def test_gated_ffn_on_the_last_frames_of_long_recordings(batch):
+    t, k, f = 2000, 768, 256
+    x, w, b, dy = make_ffn(torch.float16, batch, k, f, k, True)
+    wide, wide_dy = (torch.zeros((batch, t, k), dtype=torch.float16, device="cuda") for _ in range(2))
+    wide[:, -1], wide_dy[:, -1] = x, dy
+    want, saved = ops.gated_ffn_forward(x, *w, *b, save=True)
+    grads = ops.gated_ffn_backward(dy, x, *w, saved)
+    for view, dview in ((wide[:, -1], wide_dy[:, -1]), (wide[:, -1:], wide_dy[:, -1:])):
+        y, s = ops.gated_ffn_forward(view, *w, *b, save=True)
+        assert y.shape == view.shape and torch.equal(y.view(batch, k), want)
+        got = ops.gated_ffn_backward(dview, view, *w, s)
+        assert got[0].shape == view.shape and torch.equal(got[0].reshape(batch, k), grads[0])
+        assert all(torch.equal(a, c) for a, c in zip(got[1:], grads[1:]))

@@ -433,7 +433,7 @@ namespace {
 
 constexpr int64_t kFfnMaxDim = 1 << 18;   // width, inner width: tile offsets stay far below 2^31 bytes
 constexpr int kSkinnyRows = 64;
-constexpr long long kMaxPitch = 1 << 20;  // elements between rows of a matrix
+constexpr long long kMaxPitch = 1 << 20;  // elements between rows of a matrix (of more than one row)
 
 // Carves a workspace; with base == null it only measures.
 struct Arena {
@@ -457,11 +457,21 @@ struct FfnArgs {
 
 int ffn_check_mat(const char* what, const char* name, const vtc_mat* m, int64_t rows, int cols) {
   if (!m || !m->p) return fail_handleless(VTC_ERR_ARG, "%s: %s is null", what, name);
-  if (m->row < cols || m->row > kMaxPitch) return fail_handleless(VTC_ERR_ARG, "%s: %s has a row pitch of %lld for %d columns (at most %lld)", what, name, (long long)m->row, cols, kMaxPitch);
+  if (rows > 1 && (m->row < cols || m->row > kMaxPitch))
+    return fail_handleless(VTC_ERR_ARG, "%s: %s has a row pitch of %lld for %d columns (at most %lld)", what, name, (long long)m->row, cols, kMaxPitch);
   if ((uintptr_t)m->p % 2) return fail_handleless(VTC_ERR_ARG, "%s: %s is not aligned to its type", what, name);
-  (void)rows;
   return VTC_OK;
 }
+// A single row has no pitch: whatever the caller's says (the newest frame of a recording lies a whole recording from the next one's),
+// what follows sees its width.
+struct OneRow {
+  vtc_mat m{};
+  void narrow(const vtc_mat*& at, int64_t rows, int cols) {
+    if (!at || rows > 1) return;
+    m = vtc_mat{at->p, cols};
+    at = &m;
+  }
+};
 int ffn_check(const char* what, const FfnArgs& a) {
   if (a.dtype != OP_F16 && a.dtype != OP_BF16) return fail_handleless(VTC_ERR_ARG, "%s: operands are f16 or bf16 (matrix instructions with fp32 sums), got type %d", what, a.dtype);
   if (a.act < ACT_NONE || a.act > ACT_SIGMOID) return fail_handleless(VTC_ERR_ARG, "%s: unknown activation %d", what, a.act);
@@ -827,6 +837,9 @@ extern "C" int vtc_gated_ffn(int device, int dtype, int64_t rows, int32_t width,
                              const void* b_down, int32_t bias_f32, int32_t act, const vtc_mat* y, void* saved, int64_t saved_bytes,
                              void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "gated ffn";
+  OneRow one[5];
+  one[0].narrow(x, rows, width); one[1].narrow(w_gate, inner, width); one[2].narrow(w_up, inner, width); one[3].narrow(w_down, out_width, inner);
+  one[4].narrow(y, rows, out_width);
   FfnArgs a{dtype, act, bias_f32, rows, width, inner, out_width, x, w_gate, w_up, w_down, b_gate, b_up, b_down};
   if (int rc = ffn_check(what, a)) return rc;
   if (int rc = ffn_check_mat(what, "y", y, rows, out_width)) return rc;
@@ -851,10 +864,16 @@ extern "C" int vtc_gated_ffn_backward(int device, int dtype, int64_t rows, int32
                                       int64_t saved_bytes, int32_t bias_f32, const vtc_ffn_grads* grads, void* workspace,
                                       int64_t workspace_bytes, void* stream) {
   const char* what = "gated ffn backward";
+  OneRow one[5];
+  one[0].narrow(x, rows, width); one[1].narrow(w_gate, inner, width); one[2].narrow(w_up, inner, width); one[3].narrow(w_down, out_width, inner);
+  one[4].narrow(dy, rows, out_width);
   FfnArgs a{dtype, ACT_NONE, bias_f32, rows, width, inner, out_width, x, w_gate, w_up, w_down, nullptr, nullptr, nullptr};
   if (int rc = ffn_check(what, a)) return rc;
   if (int rc = ffn_check_mat(what, "dy", dy, rows, out_width)) return rc;
   if (!grads) return fail_handleless(VTC_ERR_ARG, "%s: null argument", what);
+  vtc_ffn_grads flat = *grads;
+  if (rows == 1) flat.dx_row = width;
+  grads = &flat;
   if (rows == 0) return fail_handleless(VTC_ERR_ARG, "%s: no rows (the gradients of nothing are zeros, which the caller has)", what);
   if ((grads->dw_gate || grads->dw_up || grads->dw_down) && !(grads->dw_gate && grads->dw_up && grads->dw_down))
     return fail_handleless(VTC_ERR_ARG, "%s: the three weight gradients go together", what);

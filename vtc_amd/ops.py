@@ -391,6 +391,9 @@ def group_norm_act(x: torch.Tensor, groups: int, weight=None, bias=None, eps: fl
 _FFN_TYPES = {torch.float16: 1, torch.bfloat16: 2}
 
 
+_MAX_PITCH = 1 << 20   # the library's limit for matrices of more than one row
+
+
 def _mat(t, cols):
     row = t.stride(0)
     return L.VtcMat(t.data_ptr(), row if row > cols else cols)   # a single row may have any stride
@@ -427,10 +430,11 @@ def _ffn_args(what, x, w_gate, w_up, w_down, biases, act):
 
 
 def _rows2(t):
-    """t (.., n) as rows (m, n) whose elements are contiguous; a view where the strides allow it."""
+    """t (.., n) as rows (m, n) whose elements are contiguous; a view where the strides allow it, else a copy (also of rows that are
+    further apart than the library takes, such as the last frames of several long recordings: those are few)."""
     r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     row, col = r.stride()
-    if (col != 1 or (row < r.shape[1] and r.shape[0] > 1)) and r.numel():
+    if (col != 1 or (not r.shape[1] <= row <= _MAX_PITCH and r.shape[0] > 1)) and r.numel():
         r = r.contiguous()
     return r
 
