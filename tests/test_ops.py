@@ -962,3 +962,52 @@ def test_gated_ffn_on_the_last_frames_of_long_recordings(batch):
         got = ops.gated_ffn_backward(dview, view, *w, s)
         assert got[0].shape == view.shape and torch.equal(got[0].reshape(batch, k), grads[0])
         assert all(torch.equal(a, c) for a, c in zip(got[1:], grads[1:]))
+
+
+@gpu
+@pytest.mark.parametrize("call", ["rotary", "rotary_qk", "group_norm_act", "gated_ffn"])
+def test_forward_mode_tangents_are_refused(call):
+    forward_ad = torch.autograd.forward_ad
+    x, w, b, _ = make_ffn(torch.float16, 6, 16, 24, 16, True)
+    h = x.view(1, 6, 1, 16)
+    calls = {"rotary": lambda t: ops.rotary(t.view(1, 6, 1, 16), ops.Rotary(16)), "rotary_qk": lambda t: ops.rotary_qk(h, t.view(1, 6, 1, 16), ops.Rotary(16)),
+             "group_norm_act": lambda t: ops.group_norm_act(t.view(1, 6, 16), 2), "gated_ffn": lambda t: ops.gated_ffn(t, *w, *b)}
+    plain = calls[call](x)
+    with forward_ad.dual_level():
+        again = calls[call](x)
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError):
+            calls[call](dual)
+        with pytest.raises(ValueError, match="no gradient"):
+            ops.rotary(dual.view(1, 6, 1, 16), ops.Rotary(16), out=torch.empty_like(h))
+    for a, c in zip(plain if isinstance(plain, tuple) else (plain,), again if isinstance(again, tuple) else (again,)):
+        assert torch.equal(a, c)
+
+
+@gpu
+@pytest.mark.parametrize("call", ["rotary", "rotary_qk", "group_norm", "group_norm_backward"])
+def test_writing_through_out_is_seen_by_autograd(call):
+    """A value that an earlier operation keeps for its gradient is overwritten: the gradient refuses, as for torch's own operations."""
+    leaf = torch.randn((2, 5, 24), device="cuda", requires_grad=True)
+    y = leaf * 2
+    z = (y * y).sum()
+    d = y.detach()
+    heads = d.view(2, 5, 3, 8)
+    spec = ops.Rotary(8)
+    if call == "rotary":
+        assert ops.rotary(heads, spec, out=heads) is heads
+    elif call == "rotary_qk":
+        ops.rotary_qk(torch.zeros_like(heads), heads, spec, out=(torch.empty_like(heads), heads))
+    else:
+        x = torch.randn_like(d)
+        _, mean, rstd = ops.group_norm_act_forward(x, 3, out=d if call == "group_norm" else None)
+        if call == "group_norm_backward":
+            ops.group_norm_act_backward(x, x, 3, mean, rstd, out=d)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    # a tensor that itself requires a gradient is not written to while gradients are recorded
+    for bad in (lambda: ops.rotary(heads, spec, out=y.view(2, 5, 3, 8)), lambda: ops.group_norm_act_forward(d, 3, out=y)):
+        with pytest.raises(ValueError, match="no gradient"):
+            bad()
+    with torch.no_grad():
+        assert ops.group_norm_act_forward(d, 3, out=y)[0] is y

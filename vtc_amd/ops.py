@@ -5,8 +5,9 @@ Rotary positions, group norm with an activation on channel-last rows and the gat
 Every function launches on the current stream of its tensors' device and neither synchronises nor copies to the host.
 
 Each operator has explicit forward and backward calls (`*_forward`, `*_backward`, `inverse=True`) and, where that is handier, a
-differentiable one (`rotary`, `rotary_qk`, `group_norm_act`, `gated_ffn`) whose gradient is those calls.  A program that captures
-a training step into a graph uses the explicit ones, or makes the differentiable call inside the capture as well.
+differentiable one (`rotary`, `rotary_qk`, `group_norm_act`, `gated_ffn`) whose gradient is those calls (reverse mode; a
+forward-mode tangent is refused).  The explicit calls and what is written through out= carry no gradient.  A program that captures a
+training step into a graph uses the explicit ones, or makes the differentiable call inside the capture as well.
 """
 
 from __future__ import annotations
@@ -17,6 +18,8 @@ import math
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as forward_ad
+from torch.autograd.graph import increment_version
 
 from . import lib as L
 
@@ -83,6 +86,21 @@ def _empty(t: torch.Tensor) -> torch.Tensor:
 def _workspace(n: int, x: torch.Tensor) -> torch.Tensor:
     # the allocator's blocks start at multiples of 512 bytes; inside a graph capture they come from the graph's own pool
     return torch.empty(n if n > 0 else 1, dtype=torch.uint8, device=x.device)
+
+
+def _tracked(*tensors) -> bool:
+    """Whether autograd has to hear of a call on these tensors.  A forward-mode tangent counts: the operators have none of their own, and
+    the autograd functions below say so, where the plain call would drop it."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _check_out(what: str, out) -> None:
+    if torch.is_grad_enabled() and out.requires_grad:
+        raise ValueError(f"{what}: out= has no gradient, and the tensor given requires one; detach it")
 
 
 # ------------------------------------------------------------------------------------------------ rotary positions
@@ -191,6 +209,7 @@ def _rotary_call(tensors, spec: Rotary, positions, offset: int, inverse: bool, o
         else:
             y = outs[i]
             _same("rotary", x0, "out", y)
+            _check_out("rotary", y)
             if y.shape != shape or (y.stride(-1) != 1 and not empty):
                 raise ValueError(f"rotary: out must have shape {tuple(shape)} with contiguous heads, got {tuple(y.shape)}")
         results.append(y)
@@ -215,6 +234,8 @@ def _rotary_call(tensors, spec: Rotary, positions, offset: int, inverse: bool, o
                                      pb, pt, offset, 1 if inverse else 0, _stream(index))
     if rc:
         L.check(rc)
+    if outs is not None:
+        increment_version(results)   # a gradient that has kept what was there before has to notice
     return results
 
 
@@ -243,10 +264,10 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor, spec: Rotary, positions: torch.T
     _need_gpu(q, "rotary")
     _need_gpu(k, "rotary")
     if out is not None:
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        if _tracked(q, k):
             raise ValueError("rotary: out= has no gradient; detach the inputs")
         return tuple(_rotary_call((q, k), spec, positions, offset, inverse, tuple(out)))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+    if _tracked(q, k):
         return _RotaryFunction.apply(spec, positions, offset, inverse, q, k)
     return tuple(_rotary_call((q, k), spec, positions, offset, inverse, None))
 
@@ -255,10 +276,10 @@ def rotary(x: torch.Tensor, spec: Rotary, positions: torch.Tensor | None = None,
     """rotary_qk for one tensor."""
     _need_gpu(x, "rotary")
     if out is not None:
-        if torch.is_grad_enabled() and x.requires_grad:
+        if _tracked(x):
             raise ValueError("rotary: out= has no gradient; detach the input")
         return _rotary_call((x,), spec, positions, offset, inverse, (out,))[0]
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _tracked(x):
         return _RotaryFunction.apply(spec, positions, offset, inverse, x)[0]
     return _rotary_call((x,), spec, positions, offset, inverse, None)[0]
 
@@ -307,6 +328,7 @@ def _gn_out(what, x, out):
     if out is None:
         return _empty(x)
     _same(what, x, "out", out)
+    _check_out(what, out)
     if out.shape != x.shape or (out.numel() and out.stride(2) != 1):
         raise ValueError(f"{what}: out must have shape {tuple(x.shape)} with contiguous channels")
     return out
@@ -320,7 +342,7 @@ def group_norm_act_forward(x: torch.Tensor, groups: int, weight=None, bias=None,
     (batch, groups, float32) are what the backward call needs.  A sample's result does not depend on the rest of its batch."""
     what = "group_norm_act"
     index, dt, f32, n, t, c = _gn_args(what, x, groups, weight, bias, lengths, act)
-    out = _gn_out(what, x, out)
+    given, out = out, _gn_out(what, x, out)
     mean, rstd = torch.empty((2, n, groups), dtype=torch.float32, device=x.device).unbind(0)
     if n == 0 or t == 0:
         mean.zero_()
@@ -333,6 +355,8 @@ def group_norm_act_forward(x: torch.Tensor, groups: int, weight=None, bias=None,
                                mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), size, _stream(index))
     if rc:
         L.check(rc)
+    if given is not None:
+        increment_version(given)
     return out, mean, rstd
 
 
@@ -348,7 +372,7 @@ def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, groups: int, mean
     for s in (mean, rstd):
         if not s.is_cuda or s.get_device() != index or s.dtype is not torch.float32 or s.shape != (n, groups) or not s.is_contiguous():
             raise ValueError(f"{what}: mean and rstd are the forward call's, float32 of shape ({n}, {groups})")
-    out = _gn_out(what, x, out)
+    given, out = out, _gn_out(what, x, out)
     dw = None if weight is None else torch.empty_like(weight)
     db = None if bias is None else torch.empty_like(bias)
     so = _library()
@@ -358,6 +382,8 @@ def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, groups: int, mean
                                         _ptr(lengths), mean.data_ptr(), rstd.data_ptr(), _ptr(dw), _ptr(db), ws.data_ptr(), size, _stream(index))
     if rc:
         L.check(rc)
+    if given is not None:
+        increment_version(given)
     return out, dw, db
 
 
@@ -382,7 +408,7 @@ class _GroupNormActFunction(torch.autograd.Function):
 def group_norm_act(x: torch.Tensor, groups: int, weight=None, bias=None, eps: float = 1e-5, act: str = "none", lengths=None) -> torch.Tensor:
     """act(group_norm(x)) with a gradient for x, weight and bias; see group_norm_act_forward."""
     _need_gpu(x, "group_norm_act")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _tracked(x, weight, bias):
         return _GroupNormActFunction.apply(x, groups, weight, bias, eps, act, lengths)
     return group_norm_act_forward(x, groups, weight, bias, eps, act, lengths)[0]
 
@@ -523,6 +549,6 @@ class _GatedFfnFunction(torch.autograd.Function):
 def gated_ffn(x: torch.Tensor, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu") -> torch.Tensor:
     """The block with a gradient for x, the weights and the biases; see gated_ffn_forward."""
     _need_gpu(x, "gated_ffn")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_gate, w_up, w_down, b_gate, b_up, b_down)):
+    if _tracked(x, w_gate, w_up, w_down, b_gate, b_up, b_down):
         return _GatedFfnFunction.apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
     return gated_ffn_forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)[0]
