@@ -1011,3 +1011,49 @@ def test_writing_through_out_is_seen_by_autograd(call):
             bad()
     with torch.no_grad():
         assert ops.group_norm_act_forward(d, 3, out=y)[0] is y
+
+
+@gpu
+@pytest.mark.parametrize("n,c,groups", [((1 << 18) + 3, 512, 32), ((1 << 19) + 5, 512, 32), ((1 << 24) + 9, 8, 1), ((1 << 22) + 1, 24, 12)])
+def test_group_norm_of_more_samples_than_a_launch_holds(n, c, groups):
+    """Single frames, more of them than 2^32 threads take: the kernels go in several launches each.  The borders of 512-, 256- and 1024-thread
+    kernels; a sample's bits are those of a call on a few samples alone, and the affine's gradients are sums over all."""
+    g = torch.Generator(device="cuda").manual_seed(c)
+    x, dy = (torch.randn((n, 1, c), generator=g, device="cuda").half() for _ in range(2))
+    w, b = (1 + 0.3 * torch.randn(c, generator=g, device="cuda")).half(), (0.3 * torch.randn(c, generator=g, device="cuda")).half()
+    lengths = torch.ones(n, dtype=torch.int32, device="cuda")
+    lengths[-2] = 0
+    y, mean, rstd = ops.group_norm_act_forward(x, groups, w, b, lengths=lengths)
+    dx, dw, db = ops.group_norm_act_backward(dy, x, groups, mean, rstd, w, b, lengths=lengths)
+    for at in (0, (1 << 22) - 2, (1 << 23) // (c // 16 or 1) - 2, (1 << 24) // (c // 16 or 1) - 2, n // 2, n - 4):
+        part = slice(at, at + 4)
+        if at + 4 > n:
+            continue
+        y1, m1, r1 = ops.group_norm_act_forward(x[part], groups, w, b, lengths=lengths[part])
+        dx1, _, _ = ops.group_norm_act_backward(dy[part], x[part], groups, m1, r1, w, b, lengths=lengths[part])
+        assert torch.equal(y[part], y1) and torch.equal(mean[part], m1) and torch.equal(rstd[part], r1) and torch.equal(dx[part], dx1), at
+    assert not y[-2].any() and not dx[-2].any()
+    want_w, want_b = (torch.zeros(c, dtype=torch.float64, device="cuda") for _ in range(2))
+    room_w, room_b = (torch.zeros(c, dtype=torch.float64, device="cuda") for _ in range(2))
+    for rows in torch.arange(n, device="cuda").split(1 << 20):
+        v, d = x[rows, 0].double().view(-1, groups, c // groups), dy[rows, 0].double() * lengths[rows, None]
+        m = v.mean(2, keepdim=True)
+        r = 1 / torch.sqrt(((v - m) ** 2).mean(2, keepdim=True) + 1e-5)
+        h = ((v - m) * r).reshape(-1, c)
+        # of a term: rstd 2^-18, the mean 2^-20 of the spread and 2^-24 of itself, the product 2^-24; the sums are 64-bit
+        err = h.abs() * 2.0 ** -17 + 2.0 ** -20 + (m.abs() * r).expand(-1, -1, c // groups).reshape(-1, c) * 2.0 ** -23
+        want_w, want_b = want_w + (d * h).sum(0), want_b + d.sum(0)
+        room_w, room_b = room_w + (d.abs() * err).sum(0), room_b + d.abs().sum(0) * 2.0 ** -40
+    for got, want, room in ((dw, want_w, room_w), (db, want_b, room_b)):
+        close(got, want.cpu(), half_step(got.dtype, want).cpu() + room.cpu())
+
+
+def test_group_norm_sample_counts_are_not_limited_by_the_grid():
+    """No such device: what the argument checks let pass goes no further."""
+    so = L.load()
+    for n, l, ok in ((1 << 32, 1, True), (1 << 20, 1 << 16, True), (1, (1 << 30) - (1 << 17), True), (1, 1 << 30, False), (1 << 39, 4, False)):
+        t = lambda at: C.byref(L.VtcRows3(at, 8 * l, 8))  # noqa: E731
+        size = so.vtc_group_norm_act_workspace(n, min(l, 1 << 30), 8, 1, 0)
+        rc = so.vtc_group_norm_act(-1, 1, t(1 << 20), t(1 << 50), n, l, 8, 1, None, None, 0, 1e-5, 0, None, 1 << 60, 1 << 60, 1 << 61, size, None)
+        msg = L.last_error(None)
+        assert rc != 0 and ("device" in msg if ok else "too many rows" in msg), (n, l, msg)

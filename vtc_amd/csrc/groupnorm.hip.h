@@ -34,7 +34,8 @@ struct GnParams {
   const int* length;            // [N] or null
   float *mean, *rstd;           // [N][G]
   float* part;                  // statistics: [N][chunks][G][2] (mean, M2); backward sums: [N][chunks][C][2]
-  double* sums;                 // backward: [N][C][2] sums over rows, then [N][G][2] (A / M, B / M)
+  double* sums;                 // backward: [N][C][2] sums over rows
+  double* gsums;                // backward, streaming: [N][G][2] (A / M, B / M)
   void *dw, *db;                // gradients of the affine, may be null
   long long N, L;
   int C, G, cpg, cv, rows, chunks;   // cv = C / VEC; rows per row block (chunk) of the sums, row blocks per sample
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(256) void gn_bwd_groups_kernel(const GnParams p) {
   b = wave_sum_d(b);
   const double m = (double)gn_length(p, n) * p.cpg;
   if (lane == 0) {
-    double* o = p.sums + p.N * p.C * 2 + i * 2;
+    double* o = p.gsums + i * 2;
     o[0] = m > 0 ? a / m : 0.0;
     o[1] = m > 0 ? b / m : 0.0;
   }
@@ -398,7 +399,7 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnParams p) {
   const int lanes = min(p.cv, 256), rp = 256 / lanes;
   const int tc = threadIdx.x % lanes, tr = threadIdx.x / lanes;
   if (tr >= rp) return;
-  const double* grp = p.sums + p.N * p.C * 2 + n * p.G * 2;
+  const double* grp = p.gsums + n * p.G * 2;
   for (int v = tc; v < p.cv; v += 256) {
     float mu[VEC], rs[VEC], w[VEC], b[VEC], A[VEC], B[VEC];
 #pragma unroll

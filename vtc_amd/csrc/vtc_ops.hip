@@ -240,6 +240,23 @@ int gn_slab(int dtype, int vec, long long L, int C, int cpg) {
   return 0;
 }
 
+// A launch holds fewer than 2^32 threads, so many samples go in several launches of each kernel, one after the other (a sample's result does
+// not depend on them).  threads: the most that one sample takes in any kernel of the call; the rest of 2^32 is room for blocks that are
+// not a sample's (the affine's gradients) and for counts rounded up.
+constexpr long long kLaunchThreads = (1ll << 32) - (1 << 17);
+constexpr long long kGnMaxLength = (1 << 30) - (1 << 17);   // 64 rows in a block of 256 where there are that many: one sample fits a launch
+long long gn_slice(long long N, long long threads) { return std::min(N, std::max(1ll, kLaunchThreads / threads)); }
+GnParams gn_from(GnParams p, int dtype, long long n0, long long count) {   // the same call on `count` samples from n0 on
+  const long long es = esize(dtype);
+  auto on = [&](const void* t, long long stride) -> const void* { return t ? (const char*)t + n0 * stride * es : nullptr; };
+  p.N = count;
+  p.x = on(p.x, p.xn); p.dy = on(p.dy, p.dn); p.out = (void*)on(p.out, p.on);
+  p.mean += n0 * p.G; p.rstd += n0 * p.G;
+  if (p.length) p.length += n0;
+  if (p.sums) { p.sums += n0 * p.C * 2; p.gsums += n0 * p.G * 2; }
+  return p;
+}
+
 int gn_check(const char* what, int dtype, int affine_f32, const vtc_rows3* const* ts, int n_t, int64_t N, int64_t L, int C, int G, int act) {
   if (!dtype_ok(dtype)) return fail_handleless(VTC_ERR_ARG, "%s: unknown type %d", what, dtype);
   if (affine_f32 != 0 && affine_f32 != 1) return fail_handleless(VTC_ERR_ARG, "%s: affine_f32 must be 0 or 1", what);
@@ -249,10 +266,7 @@ int gn_check(const char* what, int dtype, int affine_f32, const vtc_rows3* const
   if (G < 1 || C % G) return fail_handleless(VTC_ERR_ARG, "%s: %d channels do not divide into %d groups", what, C, G);
   if (N == 0 || L == 0) return VTC_OK;
   if (L > (1ll << 40) || N > (1ll << 40) / L) return fail_handleless(VTC_ERR_ARG, "%s: too many rows", what);
-  int rows, chunks;
-  if (L > (long long)256 * 0x7ffffff) return fail_handleless(VTC_ERR_ARG, "%s: too many rows", what);
-  gn_shape(L, C, &rows, &chunks);
-  if (N * ((L + 3) / 4) > 0x7fff0000 || N * (long long)chunks > 0x7fffffff || N * (long long)((C + 7) / 8) > 0x7fffffff) return fail_handleless(VTC_ERR_ARG, "%s: too many rows", what);
+  if (L > kGnMaxLength) return fail_handleless(VTC_ERR_ARG, "%s: too many rows", what);
   for (int i = 0; i < n_t; ++i) {
     const vtc_rows3& t = *ts[i];
     if (!t.p) return fail_handleless(VTC_ERR_ARG, "%s: null tensor", what);
@@ -336,30 +350,39 @@ extern "C" int vtc_group_norm_act(int device, int dtype, const vtc_rows3* x, con
   p.cv = channels / vec;
   hipStream_t s = (hipStream_t)stream;
   if ((p.cvb = gn_slab(dtype, vec, length, channels, p.cpg))) {
-    const unsigned n = (unsigned)(batch * (channels / (p.cvb * vec)));
-    by_type(dtype, [&](auto d) { by_act(act, [&](auto a) {
-      constexpr int DT = decltype(d)::value, ACT = decltype(a)::value;
-      if constexpr (ACT != ACT_SIGMOID) {
-        if (length * p.cvb <= 256 * 4) hipLaunchKernelGGL((gn_slab_kernel<DT, 4, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
-        else hipLaunchKernelGGL((gn_slab_kernel<DT, 16, ACT>), dim3(n), dim3(kGnSlabThreads), 0, s, p);
-      }
-    }); });
+    const int per = channels / (p.cvb * vec);   // blocks of a sample
+    const long long slice = gn_slice(batch, (long long)per * kGnSlabThreads);
+    for (long long n0 = 0; n0 < batch; n0 += slice) {
+      const GnParams q = gn_from(p, dtype, n0, std::min(slice, batch - n0));
+      const dim3 grid((unsigned)(q.N * per));
+      by_type(dtype, [&](auto d) { by_act(act, [&](auto a) {
+        constexpr int DT = decltype(d)::value, ACT = decltype(a)::value;
+        if constexpr (ACT != ACT_SIGMOID) {
+          if (length * p.cvb <= 256 * 4) hipLaunchKernelGGL((gn_slab_kernel<DT, 4, ACT>), grid, dim3(kGnSlabThreads), 0, s, q);
+          else hipLaunchKernelGGL((gn_slab_kernel<DT, 16, ACT>), grid, dim3(kGnSlabThreads), 0, s, q);
+        }
+      }); });
+    }
     return launched("group norm");
   }
-  const unsigned blocks = (unsigned)(batch * p.chunks);
   // few partials and few blocks to repeat it in: the elementwise pass merges them itself, a launch less (5 x 1531 rows, 3 groups:
   // 12 us instead of 6 + 9; with 63 row blocks of 32 groups it would cost 64 x 3999 rows 20 us)
   p.merge_here = groups <= kGnMergeHere && p.chunks * groups <= 256 && batch * p.achunks <= 4096;
-  by_vec(dtype, vec, [&](auto d, auto v) {
-    constexpr int DT = decltype(d)::value, VEC = decltype(v)::value;
-    const size_t lds = ((size_t)2 * channels + 256 * 2 * VEC) * 4;
-    hipLaunchKernelGGL((gn_stats_kernel<DT, VEC>), dim3(blocks), dim3(256), lds, s, p);
-    if (!p.merge_here) hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(batch * ((groups + 15) / 16))), dim3(256), 0, s, p);
-    by_act(act, [&](auto a) {
-      if constexpr (decltype(a)::value != ACT_SIGMOID)
-        hipLaunchKernelGGL((gn_apply_kernel<DT, VEC, decltype(a)::value>), dim3((unsigned)(batch * p.achunks)), dim3(256), 0, s, p);
+  const int per16 = (groups + 15) / 16;
+  const long long slice = gn_slice(batch, 256ll * std::max({p.chunks, p.achunks, per16}));
+  for (long long n0 = 0; n0 < batch; n0 += slice) {
+    const GnParams q = gn_from(p, dtype, n0, std::min(slice, batch - n0));
+    by_vec(dtype, vec, [&](auto d, auto v) {
+      constexpr int DT = decltype(d)::value, VEC = decltype(v)::value;
+      const size_t lds = ((size_t)2 * channels + 256 * 2 * VEC) * 4;
+      hipLaunchKernelGGL((gn_stats_kernel<DT, VEC>), dim3((unsigned)(q.N * q.chunks)), dim3(256), lds, s, q);
+      if (!q.merge_here) hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(q.N * per16)), dim3(256), 0, s, q);
+      by_act(act, [&](auto a) {
+        if constexpr (decltype(a)::value != ACT_SIGMOID)
+          hipLaunchKernelGGL((gn_apply_kernel<DT, VEC, decltype(a)::value>), dim3((unsigned)(q.N * q.achunks)), dim3(256), 0, s, q);
+      });
     });
-  });
+  }
   return launched("group norm");
 }
 
@@ -393,35 +416,45 @@ extern "C" int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows
   p.mean = (float*)mean; p.rstd = (float*)rstd;
   p.part = (float*)workspace;
   p.sums = (double*)((char*)workspace + align256((size_t)batch * p.chunks * channels * 8));
+  p.gsums = p.sums + batch * channels * 2;
   const int vec = vec_of(dtype, {channels, eff(x->batch, batch), eff(x->row, length), eff(dy->batch, batch), eff(dy->row, length),
                                  eff(dx->batch, batch), eff(dx->row, length)}, {x->p, dy->p, dx->p});
   p.cv = channels / vec;
   if ((p.cvb = gn_slab(dtype, vec, length, channels, p.cpg))) {
-    const unsigned n = (unsigned)(batch * (channels / (p.cvb * vec)));
+    const int per = channels / (p.cvb * vec);   // blocks of a sample
     const int nv = (int)((length * p.cvb + kGnSlabBwdThreads - 1) / kGnSlabBwdThreads);
+    const long long slice = gn_slice(batch, (long long)per * kGnSlabBwdThreads);
     by_type(dtype, [&](auto d) { by_act(act, [&](auto a) {
       constexpr int DT = decltype(d)::value, ACT = decltype(a)::value;
-      if constexpr (ACT != ACT_SIGMOID) {
-        if (nv <= 2) hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 2, ACT>), dim3(n), dim3(kGnSlabBwdThreads), 0, s, p);
-        else if (nv <= 4) hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 4, ACT>), dim3(n), dim3(kGnSlabBwdThreads), 0, s, p);
-        else hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 8, ACT>), dim3(n), dim3(kGnSlabBwdThreads), 0, s, p);
+      for (long long n0 = 0; n0 < batch; n0 += slice) {
+        const GnParams q = gn_from(p, dtype, n0, std::min(slice, batch - n0));
+        const dim3 grid((unsigned)(q.N * per)), block(kGnSlabBwdThreads);
+        if constexpr (ACT != ACT_SIGMOID) {
+          if (nv <= 2) hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 2, ACT>), grid, block, 0, s, q);
+          else if (nv <= 4) hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 4, ACT>), grid, block, 0, s, q);
+          else hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, 8, ACT>), grid, block, 0, s, q);
+        }
       }
       if (dweight || dbias) hipLaunchKernelGGL((gn_affine_grads_kernel<DT>), dim3(grad_blocks), dim3(256), 0, s, p);
     }); });
     return launched("group norm backward");
   }
-  const unsigned blocks = (unsigned)(batch * p.chunks);
-  const long long group_blocks = ((long long)batch * groups + 3) / 4;
+  const long long slice = gn_slice(batch, std::max({256ll * p.chunks, 256ll * p.achunks, 1024ll, 64ll * groups}));
+  const bool sliced = slice < batch, affine = dweight || dbias;
   by_vec(dtype, vec, [&](auto d, auto v) {
     constexpr int DT = decltype(d)::value, VEC = decltype(v)::value;
     by_act(act, [&](auto a) {
       constexpr int ACT = decltype(a)::value;
       if constexpr (ACT != ACT_SIGMOID) {
-        hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, VEC, ACT>), dim3(blocks), dim3(256), 0, s, p);
-        hipLaunchKernelGGL(gn_bwd_merge_kernel, dim3((unsigned)batch), dim3(1024), 0, s, p);
-        hipLaunchKernelGGL((gn_bwd_groups_kernel<DT>), dim3((unsigned)group_blocks), dim3(256), 0, s, p);
-        // the blocks behind the rows' sum the affine's gradients
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, VEC, ACT>), dim3((unsigned)(batch * p.achunks + (dweight || dbias ? grad_blocks : 0))), dim3(256), 0, s, p);
+        for (long long n0 = 0; n0 < batch; n0 += slice) {
+          const GnParams q = gn_from(p, dtype, n0, std::min(slice, batch - n0));
+          hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, VEC, ACT>), dim3((unsigned)(q.N * q.chunks)), dim3(256), 0, s, q);
+          hipLaunchKernelGGL(gn_bwd_merge_kernel, dim3((unsigned)q.N), dim3(1024), 0, s, q);
+          hipLaunchKernelGGL((gn_bwd_groups_kernel<DT>), dim3((unsigned)((q.N * groups + 3) / 4)), dim3(256), 0, s, q);
+          // the blocks behind the rows' sum the affine's gradients
+          hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, VEC, ACT>), dim3((unsigned)(q.N * q.achunks + (affine && !sliced ? grad_blocks : 0))), dim3(256), 0, s, q);
+        }
+        if (affine && sliced) hipLaunchKernelGGL((gn_affine_grads_kernel<DT>), dim3(grad_blocks), dim3(256), 0, s, p);
       }
     });
   });
