@@ -48,3 +48,28 @@ def test_operand_windows_stay_inside_the_operand(tmp_path):
     r = subprocess.run([str(exe)], input="\n".join(" ".join(map(str, x)) for x in lines), capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout
     assert f"{len(lines)} products walked" in r.stdout
+
+
+def plans(tmp_path, questions):
+    exe = build(tmp_path, "op_plan_table.cpp")
+    r = subprocess.run([str(exe)], input="\n".join(" ".join(map(str, q)) for q in questions), capture_output=True, text=True, timeout=300)
+    lines = r.stdout.splitlines()
+    assert r.returncode == 0 and len(lines) == len(questions), r.stdout[-500:] + r.stderr[-500:]
+    return [line.split() for line in lines]
+
+
+def test_no_launch_takes_2_to_the_32_threads(tmp_path):
+    most = 2 ** 24 - 1   # blocks of 256 threads
+    widths = (1, 8, 64, 65, 100, 128, 129, 192, 2048, 262144)
+    ask = []
+    for m in (65, 10 ** 6, 2 ** 30 + 1, 2 ** 31 - 256):
+        for n in widths:
+            if (m // 128 + 1) * (n // 32 + 1) > 2 ** 30:   # refused as too many
+                continue
+            for k in (1, 64, 2048):
+                ask += [("gate", m, k, n, 0), ("gate", m, k, n, 1), ("rows", m, n, k), ("dgate", m, k, n), ("weights", m, k, n, n)]
+    for q, (_, _, _, blocks) in zip(ask, plans(tmp_path, ask)):
+        assert 1 <= int(blocks) <= most, q
+    ask = [("rotary", t, per, table) for t in (1, 7, 5000, 2 ** 24 - 1, 2 ** 24, 2 ** 25 + 3, 2 ** 26) for per, table in ((1, 2048), (24 * 4, 64), (1000, 8), (5000, 8))]
+    for q, (n, blocks) in zip(ask, plans(tmp_path, ask)):
+        assert 1 <= int(n) <= q[3] and int(blocks) <= most, q

@@ -9,6 +9,7 @@
 #include "../../include/vtc_amd.h"
 #include "gated_ffn.hip.h"
 #include "groupnorm.hip.h"
+#include "op_plan.h"
 #include "ops.h"
 #include "rotary.hip.h"
 
@@ -192,14 +193,10 @@ extern "C" int vtc_rotary_heads(int device, int dtype, const vtc_rotary* r, int6
   p.amp = (float)r->amplitude; p.inverse = inverse ? 1 : 0;
   p.vec_half = half / vec;
   p.items = p.vec_half + (p.tail + 2 * vec - 1) / (2 * vec);
-  // tokens of a block: ~4 items per thread, the angle table within its LDS, and at least ~1000 blocks where there are rows for it
   const long long per_tok = (long long)p.heads * p.items;
-  long long tpb = std::max<long long>(1, 1024 / per_tok);
-  tpb = std::min<long long>(tpb, kRotTableEntries / half);
-  tpb = std::min<long long>(tpb, std::max<long long>(1, p.tokens / 1024));
-  p.tpb = (int)tpb;
-  const long long blocks = (p.tokens + tpb - 1) / tpb;
-  if (blocks > 0x7fffffff || per_tok * tpb > 0x7fffffff) return fail_handleless(VTC_ERR_ARG, "rotary: too many rows");
+  p.tpb = rotary_tokens_per_block(p.tokens, per_tok, kRotTableEntries / half);
+  const long long blocks = (p.tokens + p.tpb - 1) / p.tpb;
+  if (blocks > kMaxBlocks || per_tok * p.tpb > 0x7fffffff) return fail_handleless(VTC_ERR_ARG, "rotary: too many rows");
   by_vec(dtype, vec, [&](auto d, auto v) {
     constexpr int DT = decltype(d)::value, VEC = decltype(v)::value;
     if (r->layout == VTC_ROTARY_HALF)
@@ -240,10 +237,9 @@ int gn_slab(int dtype, int vec, long long L, int C, int cpg) {
   return 0;
 }
 
-// A launch holds fewer than 2^32 threads, so many samples go in several launches of each kernel, one after the other (a sample's result does
-// not depend on them).  threads: the most that one sample takes in any kernel of the call; the rest of 2^32 is room for blocks that are
-// not a sample's (the affine's gradients) and for counts rounded up.
-constexpr long long kLaunchThreads = (1ll << 32) - (1 << 17);
+// Many samples go in several launches of each kernel, one after the other (a sample's result does not depend on them).  threads: the
+// most that one sample takes in any kernel of the call; what kLaunchThreads leaves of 2^32 is room for blocks that are not a sample's (the
+// affine's gradients) and for counts rounded up.
 constexpr long long kGnMaxLength = (1 << 30) - (1 << 17);   // 64 rows in a block of 256 where there are that many: one sample fits a launch
 long long gn_slice(long long N, long long threads) { return std::min(N, std::max(1ll, kLaunchThreads / threads)); }
 GnParams gn_from(GnParams p, int dtype, long long n0, long long count) {   // the same call on `count` samples from n0 on
@@ -574,37 +570,6 @@ int group_of(int tiles_m, int tiles_n, double a_bytes, double w_bytes, double w_
   return r;
 }
 
-// How a product runs: tile size and K splits, by a model of its time (us) fitted to kernel times measured at 768 x 2048.  A round is
-// as many tiles as the chip holds at once (256 of 256 rows, one per CU; 512 of 128 x 64, two per CU); `fill` is its share in use,
-// since K-tiles slow down as more CUs fetch.  Per K-tile: 1.35 + 0.75 fill for 256 x 256 (x 3/4 for 192 columns), 0.42 + 0.38 fill
-// for 128 x 64; per tile the epilogue's share.  Partials cross memory twice at 4 TB/s and cost a launch.  Measured, 256-wide / small:
-//   gate and up      512 rows 22 / 10   2048 26 / 24   4096 30 / 43   16384 109 / 183
-//   ..., slopes kept 512 rows 29 / 13   2048 33 / 31   4096 38 / 54   16384 147 / 236
-//   down             512 rows 36 / 12   2048 37 / 18   8192 43 / 39   16384  59 / 81
-//   dx               512 rows 72 / 16   2048 74 / 30   8192 86 / 82   16384 109 / 173
-//   dg and du        512 rows 36 / 13   2048 37 / 20   8192 88 / 73   16384 149 / 162
-//   weights          512 rows 31 / 22   2048 46 / 44   8192 91 / 137  16384 165 / 290
-struct OgPlan { bool small; int splits, kps; };
-struct OgCost { long long tiles_big, tiles_small; double width, end_big, end_small; };   // tiles; epilogue of a tile
-OgPlan og_plan(const OgCost& o, int nk, int splits_big, int splits_small, double out_elems) {
-  OgPlan best{false, 1, (nk + 1) & ~1};
-  double cost = 1e300;
-  for (int small = 0; small < 2; ++small)
-    for (int sp = 1; sp <= (small ? splits_small : splits_big); ++sp) {
-      int k = (nk + sp - 1) / sp;
-      if (!small) k = (k + 1) & ~1;
-      if (sp > 1 && k < 4) break;
-      if ((nk + k - 1) / k != sp) continue;
-      const double cap = small ? 512.0 : 256.0, units = (double)(small ? o.tiles_small : o.tiles_big) * sp;
-      auto round = [&](double fill) { return small ? k * (0.42 + 0.38 * fill) + o.end_small : k * o.width * (1.35 + 0.75 * fill) + o.end_big; };
-      const double full = std::floor(units / cap), rest = units / cap - full;
-      double c = full * round(1.0) + (rest > 0.0 ? round(rest) : 0.0);
-      if (sp > 1) c += 4.0 + sp * out_elems * 8.0 / 4.0e6;
-      if (c < cost) { cost = c; best = OgPlan{small != 0, sp, k}; }
-    }
-  return best;
-}
-int div_up(long long a, int b) { return (int)((a + b - 1) / b); }
 
 void finish_prob(OpProb& q, bool small, int bm, int bn, int K, int tile0, int w_rows = 0) {   // w_rows: rows of B behind a tile, if not bn
   q.tiles_m = div_up(q.M, bm);
@@ -655,8 +620,7 @@ template <bool F16> void gate_up(int64_t M, int K, int F, OpMat x, OpMat wg, OpM
     return;
   }
   const bool save = o.s.hi != nullptr;
-  const OgPlan plan = og_plan({(long long)div_up(M, 256) * div_up(F8, 128), (long long)div_up(M, 128) * div_up(F8, 32), 1.0, save ? 12.0 : 5.0, save ? 6.0 : 4.0},
-                              div_up(K, 64), 1, 1, 0);
+  const OgPlan plan = plan_gate(M, K, F8, save);
   OpGemmParams p{};
   p.nprob = 1;
   OpProb& q = p.prob[0];
@@ -672,7 +636,7 @@ template <bool F16> void gate_up(int64_t M, int K, int F, OpMat x, OpMat wg, OpM
 // C = A B^T (+ bias) in 16 bits for one or two operand pairs; with few tiles in K splits whose partials lie in the workspace
 struct OutPlan { OgPlan plan; int N8; float* part; };
 OutPlan plan_out(Arena& ar, int64_t M, int N, int nk) {
-  OutPlan o{og_plan({(long long)div_up(M, 256) * div_up(N, 192), (long long)div_up(M, 128) * div_up(N, 64), 0.75, 4.0, 2.0}, nk, 1, 32, (double)M * N), up8(N), nullptr};
+  OutPlan o{plan_rows(M, N, nk), up8(N), nullptr};
   if (o.plan.splits > 1) o.part = ar.take<float>((size_t)o.plan.splits * M * o.N8);
   return o;
 }
@@ -758,7 +722,7 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, cons
   const OpMat wd = in.get(a.wd, a.N, a.F);
   h16 *dg = ar.take<h16>((size_t)a.M * F8), *du = ar.take<h16>((size_t)a.M * F8);
   // dh and what it turns into
-  const OgPlan dplan = og_plan({(long long)div_up(M, 256) * div_up(F8, 192), (long long)div_up(M, 128) * div_up(F8, 64), 0.75, 20.0, 7.0}, div_up(a.N, 64), 1, 1, 0);
+  const OgPlan dplan = plan_dgate(M, a.N, F8);
   const long long parts = dplan.small ? 4ll * div_up(M, 128) : 2ll * div_up(M, 256);
   const int row_blocks = div_up(M, kColRows);
   float* cs_f = (o->db_gate || o->db_up) || !launch ? ar.take<float>((size_t)2 * parts * F8) : nullptr;
@@ -772,11 +736,9 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, cons
   const h16* bs[3] = {x.p, x.p, launch ? ffn_saved((void*)saved, a.M, a.F).h : nullptr};
   const long long ldb[3] = {x.ld, x.ld, F8};
   const int rows[3] = {a.F, a.F, a.N}, cols[3] = {a.K, a.K, a.F}, pitch[3] = {K8, K8, F8};
-  long long tb = 0, ts = 0;
-  for (int i = 0; i < 3; ++i) { tb += (long long)div_up(rows[i], 256) * div_up(pitch[i], 256); ts += (long long)div_up(rows[i], 128) * div_up(pitch[i], 64); }
   const long long one = (long long)a.F * K8;
   w.split_stride = 2 * one + (long long)a.N * F8;
-  const OgPlan wplan = og_plan({tb, ts, 1.0, 6.0, 3.0}, div_up(M, 64), 32, 32, (double)w.split_stride);
+  const OgPlan wplan = plan_weights(M, a.K, a.F, a.N);
   int tiles = 0;
   for (int i = 0; i < 3; ++i) {
     OpProb& q = w.prob[i];
@@ -812,9 +774,10 @@ size_t ffn_backward(const FfnArgs& a, const vtc_mat* dy, const void* saved, cons
     const OpGemmParams dx = out_params(xplan, M, a.K, xp);
     const int col_blocks = (N8 / 8 + 63) / 64;
     const ColSumParams cs{y.p, y.ld, M, cs_n, N8, a.N, row_blocks, cs_n ? row_blocks * col_blocks : 0};
-    if (o->dx && part && xplan.plan.small && wplan.small) {
+    const long long joint = (long long)w.ntiles * w.splits + (long long)dx.ntiles * dx.splits + cs.blocks;
+    if (o->dx && part && xplan.plan.small && wplan.small && joint <= kMaxBlocks) {
       const SmallGradsParams g{w, dx, cs, (unsigned)(w.ntiles * w.splits), (unsigned)(dx.ntiles * dx.splits)};
-      const dim3 grid(g.w_blocks + g.dx_blocks + (unsigned)cs.blocks);
+      const dim3 grid((unsigned)joint);
       if (xplan.part) hipLaunchKernelGGL((small_grads_kernel<F16, OG_PART>), grid, dim3(256), 0, s, g);
       else hipLaunchKernelGGL((small_grads_kernel<F16, OG_PLAIN>), grid, dim3(256), 0, s, g);
     } else {
@@ -903,6 +866,8 @@ extern "C" int vtc_gated_ffn_backward(int device, int dtype, int64_t rows, int32
   FfnArgs a{dtype, ACT_NONE, bias_f32, rows, width, inner, out_width, x, w_gate, w_up, w_down, nullptr, nullptr, nullptr};
   if (int rc = ffn_check(what, a)) return rc;
   if (int rc = ffn_check_mat(what, "dy", dy, rows, out_width)) return rc;
+  if (grads && grads->db_down && (rows / kColRows + 1) * (out_width / 512 + 1) > kMaxBlocks)
+    return fail_handleless(VTC_ERR_ARG, "%s: %lld rows of width %d are too many", what, (long long)rows, out_width);
   if (!grads) return fail_handleless(VTC_ERR_ARG, "%s: null argument", what);
   vtc_ffn_grads flat = *grads;
   if (rows == 1) flat.dx_row = width;
