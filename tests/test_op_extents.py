@@ -73,3 +73,23 @@ def test_no_launch_takes_2_to_the_32_threads(tmp_path):
     ask = [("rotary", t, per, table) for t in (1, 7, 5000, 2 ** 24 - 1, 2 ** 24, 2 ** 25 + 3, 2 ** 26) for per, table in ((1, 2048), (24 * 4, 64), (1000, 8), (5000, 8))]
     for q, (n, blocks) in zip(ask, plans(tmp_path, ask)):
         assert 1 <= int(n) <= q[3] and int(blocks) <= most, q
+
+
+def test_feed_forward_sizes_of_the_gpu_tests_cover_both_tilings(tmp_path):
+    """The sizes that tests/test_ops.py checks against 64 bits: all products on small tiles, and all products on 256-wide ones.  A change of
+    the cost model that moves them has to bring other sizes."""
+    from test_ops import FFN_SIZES, FFN_SPLIT_SIZES, FFN_WIDE_SIZES
+
+    def ask(m, k, f, n):
+        both = 2 * 64 * ((f + 63) // 64)   # dx: the K-tiles of two segments
+        return [("gate", m, k, f, 0), ("gate", m, k, f, 1), ("rows", m, n, f), ("dgate", m, n, f), ("rows", m, k, both), ("weights", m, k, f, n)]
+
+    wide = [plans(tmp_path, ask(*s)) for s in FFN_WIDE_SIZES]
+    assert all(p[0] == "wide" for s in wide for p in s)
+    assert any(int(p[1]) > 256 for s in wide for p in s) and any(int(p[1]) < 256 for s in wide for p in s)
+    assert any(int(s[5][2]) > 1 for s in wide)                    # weights' gradients in K splits
+    tiled = [plans(tmp_path, ask(*s)) for s in FFN_SIZES + FFN_SPLIT_SIZES if s[0] > 64]
+    assert all(p[0] == "small" for s in tiled for p in s)
+    assert all(any(int(s[i][2]) > 1 for s in tiled) and any(int(s[i][2]) == 1 for s in tiled) for i in (2, 4, 5))   # K splits of down, dx, weights
+    long = plans(tmp_path, ask(4100, 4160, 131080, 200))
+    assert long[4][0] == "wide" and long[5][0] == "wide" and 4160 % 192 in range(1, 129) and 4160 * 131080 > 2 ** 29

@@ -1057,3 +1057,69 @@ def test_group_norm_sample_counts_are_not_limited_by_the_grid():
         rc = so.vtc_group_norm_act(-1, 1, t(1 << 20), t(1 << 50), n, l, 8, 1, None, None, 0, 1e-5, 0, None, 1 << 60, 1 << 60, 1 << 61, size, None)
         msg = L.last_error(None)
         assert rc != 0 and ("device" in msg if ok else "too many rows" in msg), (n, l, msg)
+
+
+# Every product of these runs on 256-wide tiles (tests/test_op_extents.py asks the library's plan): several tiles of a block one after the
+# other and fewer tiles than blocks, halves of a tile behind the matrix, K splits of the weights' gradients, rows that are copied first and rows that are not
+FFN_WIDE_SIZES = [(9001, 773, 2051, 757), (24601, 1100, 700, 1300), (12013, 1096, 712, 1288)]
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("m,k,f,n", FFN_WIDE_SIZES)
+def test_gated_ffn_on_256_wide_tiles(kind, m, k, f, n):
+    act = {9001: "silu", 24601: "gelu", 12013: "sigmoid"}[m]
+    kind = TYPES[kind]
+    x, w, b, dy = make_ffn(kind, m, k, f, n, True, bias_kind=torch.float32 if m == 24601 else None)
+    y, saved = ops.gated_ffn_forward(x, *w, *b, act=act, save=True)
+    assert torch.equal(y, ops.gated_ffn_forward(x, *w, *b, act=act)[0])
+    grads = ops.gated_ffn_backward(dy, x, *w, saved, act=act, bias_dtype=b[0].dtype)
+    check_ffn(kind, x, w, b, act, dy, y, grads)
+    # the bounds above grow with the contraction; in the 2-norm, at most four half steps lie on the way to a result (h or dg / du, the other
+    # factor of a product of two of them, the result, and Phi's fit), and n terms in fp32 add n 2^-24
+    want = ffn_64(x, *w, *b, act, dy)
+    for name, got in (("y", y),) + tuple(zip(NAMES, grads)):
+        room = 2 * torch.finfo(kind).eps + m * 2.0 ** -24
+        assert float((got.double() - want[name]).norm() / want[name].norm()) <= room, name
+
+
+# Small tiles with the down product, dx and the weights' gradients in K splits, alone or together
+FFN_SPLIT_SIZES = [(499, 768, 2048, 768), (301, 389, 2051, 261), (70, 100, 4100, 52), (1237, 389, 1031, 389)]
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("m,k,f,n", FFN_SPLIT_SIZES)
+def test_gated_ffn_in_k_splits(kind, m, k, f, n):
+    x, w, b, dy = make_ffn(TYPES[kind], m, k, f, n, True)
+    y, saved = ops.gated_ffn_forward(x, *w, *b, act="gelu", save=True)
+    grads = ops.gated_ffn_backward(dy, x, *w, saved, act="gelu")
+    check_ffn(TYPES[kind], x, w, b, "gelu", dy, y, grads)
+    want = ffn_64(x, *w, *b, "gelu", dy)   # the 2-norm as in test_gated_ffn_on_256_wide_tiles
+    for name, got in (("y", y),) + tuple(zip(NAMES, grads)):
+        room = 2 * torch.finfo(TYPES[kind]).eps + max(m, f) * 2.0 ** -24
+        assert float((got.double() - want[name]).norm() / want[name].norm()) <= room, name
+
+
+@gpu
+def test_gated_ffn_weights_of_more_than_2_to_the_29_elements():
+    """K-tiles of dx whose k-rows lie more than 2^31 bytes behind the first, with a half-tile of columns behind the matrix; a sample of rows
+    and columns of every result against the 64-bit definition."""
+    m, k, f, n = 4100, 4160, 131080, 200
+    kind = torch.bfloat16
+    x, w, b, dy = make_ffn(kind, m, k, f, n, False)
+    y, saved = ops.gated_ffn_forward(x, *w, save=True)
+    dx, dwg, dwu, dwd = ops.gated_ffn_backward(dy, x, *w, saved, biases=False)[:4]
+    del saved
+    rows = torch.tensor([0, 1, 255, 256, 2047, 4095, 4096, 4099], device="cuda")
+    want = ffn_64(x[rows], *w, *b, "silu", dy[rows])
+    tol = ffn_tolerances(x[rows], *w, *b, "silu", dy[rows], kind)
+    for name, got in (("y", y[rows]), ("dx", dx[rows])):
+        close(got, want[name].cpu(), half_step(kind, want[name]).cpu() + tol[name].cpu() * 1.001, name)
+    del want, tol
+    cols = torch.tensor([0, 127, 128, 65535, 65536, 131071, 131072, 131079], device="cuda")
+    part = (w[0][cols], w[1][cols], w[2][:, cols].contiguous())   # these inner columns alone: their weights' gradients do not depend on the others
+    want = ffn_64(x, *part, *b, "silu", dy)
+    tol = ffn_tolerances(x, *part, *b, "silu", dy, kind)
+    for name, got in (("dw_gate", dwg[cols]), ("dw_up", dwu[cols]), ("dw_down", dwd[:, cols])):
+        close(got, want[name].cpu(), half_step(kind, want[name]).cpu() + tol[name].cpu() * 1.001, name)
