@@ -1123,3 +1123,83 @@ def test_gated_ffn_weights_of_more_than_2_to_the_29_elements():
     tol = ffn_tolerances(x, *part, *b, "silu", dy, kind)
     for name, got in (("dw_gate", dwg[cols]), ("dw_up", dwu[cols]), ("dw_down", dwd[:, cols])):
         close(got, want[name].cpu(), half_step(kind, want[name]).cpu() + tol[name].cpu() * 1.001, name)
+
+
+def fused_layouts(batch, length, heads, dim):
+    """(shape, axis of the 3 projections, order that brings (batch, length, heads, dim)) of fused projections, by the order of their dimensions."""
+    return {
+        "rows": ((batch, length, 3, heads, dim), 2, (0, 1, 2, 3)),
+        "sequence first": ((length, batch, 3, heads, dim), 2, (1, 0, 2, 3)),
+        "heads first": ((batch, 3, heads, length, dim), 1, (0, 2, 1, 3)),
+        "projection first": ((3, batch, length, heads, dim), 0, (0, 1, 2, 3)),
+        "projections of a head together": ((batch, length, heads, 3, dim), 3, (0, 1, 2, 3)),
+        "length last": ((heads, batch, 3, length, dim), 2, (1, 2, 0, 3)),
+    }
+
+
+LAYOUT_NAMES = list(fused_layouts(1, 1, 1, 2))
+
+
+@gpu
+@pytest.mark.parametrize("name", LAYOUT_NAMES)
+@pytest.mark.parametrize("batch", [1, 4])
+def test_rotary_in_place_in_fused_projections_of_any_order(name, batch):
+    length, heads, dim = 33, 5, 24
+    shape, axis, order = fused_layouts(batch, length, heads, dim)[name]
+    g = torch.Generator(device="cuda").manual_seed(41)
+    qkv = torch.randn(shape, generator=g, device="cuda").half()
+    before = qkv.clone()
+    spec = ops.Rotary(16, layout="interleaved")
+    q, k = (qkv.select(axis, i).permute(order) for i in (0, 1))
+    ops.rotary_qk(q, k, spec, out=(q, k))
+    pos = torch.arange(length).expand(batch, length)
+    for i, t in ((0, q), (1, k)):
+        check_rotary(t, before.select(axis, i).permute(order), spec, pos)
+    assert torch.equal(qkv.select(axis, 2), before.select(axis, 2))
+    q2 = before.select(axis, 2).permute(order)   # and from one projection into another's place
+    ops.rotary(q2, spec, out=before.select(axis, 0).permute(order))
+    check_rotary(before.select(axis, 0).permute(order), q2, spec, pos)
+
+
+def test_rotary_takes_what_is_apart_and_refuses_what_is_shared():
+    """In place on two tensors of one buffer, by brute force over their elements.  No such device: what passes the checks goes no further."""
+    f = (C.c_double * 32)(*([0.5] * 32))
+    rng = np.random.default_rng(17)
+    so = L.load()
+
+    def accepted(base, strides, counts, heads, dim):
+        spec = L.VtcRotary(dim, 2, 0, 0, 1.0, C.cast(f, L._f64p))
+        arr = (L.VtcHeads * 2)(*(L.VtcHeads(1 << 20 if i == 0 else (1 << 20) + 2 * base, 1 << 20 if i == 0 else (1 << 20) + 2 * base, *strides, *strides, heads[i])
+                                 for i in (0, 1)))
+        rc = so.vtc_rotary_heads(-1, 1, C.byref(spec), counts[0], counts[1], arr, 2, None, 0, 0, 0, 0, 0, None)
+        msg = L.last_error(None)
+        assert rc != 0 and ("device" in msg or "shares memory" in msg or "overlaps itself" in msg), msg
+        return None if "overlaps itself" in msg else "device" in msg
+
+    def elements(base, strides, counts, heads, dim):
+        n = [np.arange(c) for c in (counts[0], counts[1], heads, dim)]
+        return set((base + n[0][:, None, None, None] * strides[0] + n[1][:, None, None] * strides[1] + n[2][:, None] * strides[2] + n[3]).ravel().tolist())
+
+    for name in LAYOUT_NAMES:                    # whole projections: always apart
+        shape, axis, order = fused_layouts(3, 4, 2, 6)[name]
+        t = torch.empty(shape)
+        a, b = (t.select(axis, i).permute(order) for i in (0, 1))
+        for base in (b.storage_offset(), -b.storage_offset()):
+            assert accepted(base, a.stride()[:3], (3, 4), (2, 2), 6), name
+        assert accepted(b.storage_offset() - 1, a.stride()[:3], (3, 4), (2, 2), 6) is False, name   # the last element of the first one
+    seen = {True: 0, False: 0}
+    for _ in range(3000):
+        counts, heads, dim = rng.integers(1, 4, 2).tolist(), rng.integers(1, 4, 2).tolist(), int(rng.choice([2, 4, 6]))
+        sizes = [*counts, max(heads)]
+        strides, span = [0, 0, 0], dim
+        for i in rng.permutation(3).tolist():    # nested, with room between
+            strides[i] = span + int(rng.choice([0, 0, 2, dim, 3 * dim]))
+            span = strides[i] * (sizes[i] - 1) + span
+        base = int(rng.integers(-span - 4, span + 4))
+        got = accepted(base, strides, counts, heads, dim)
+        if got is None:
+            continue
+        shared = bool(elements(0, strides, counts, heads[0], dim) & elements(base, strides, counts, heads[1], dim))
+        assert got == (not shared), (base, strides, counts, heads, dim)
+        seen[got] += 1
+    assert min(seen.values()) > 300, seen

@@ -122,15 +122,48 @@ int rotary_check_tensor(const char* name, const vtc_heads& t, const vtc_rotary& 
   return VTC_OK;
 }
 
-// No element in common: ranges that do not meet, or columns apart in rows of one pitch (q and k inside a fused projection's rows).
-bool apart(const void* a, const char* a_end, long long a_batch, long long a_row, long long a_width, const void* b, const char* b_end,
-           long long b_batch, long long b_row, long long b_width, long long batch, int es) {
-  if (!overlap(a, a_end, b, b_end)) return true;
-  if (a_row != b_row || a_row < 1 || (batch > 1 && (a_batch % a_row || b_batch % a_row))) return false;
-  const long long bytes = (const char*)b - (const char*)a;
+// One side of a tensor: (batch, length, heads) blocks of `width` contiguous elements
+struct Blocks {
+  const void* p;
+  long long stride[3], count[3];
+  int width;
+  const char* end(int es) const { return end_of(p, {{count[0], stride[0]}, {count[1], stride[1]}, {count[2], stride[2]}}, width, es); }
+};
+// Whether two sets of blocks of the same strides, `delta` elements apart, share an element: delta = sum of q_i stride_i + e for steps
+// lo_i <= q_i <= hi_i and |e| < width.  From the largest stride on; what lies inside a stride rarely reaches past the next
+// multiple, so two or three steps come into question each.  Many of them (strides that are not nested) count as shared.
+struct Step { long long stride, lo, hi; };
+bool steps_meet(const Step* d, int n, long long delta, int width) {
+  if (n == 0) return std::abs(delta) < width;
+  long long reach = width - 1;
+  for (int i = 1; i < n; ++i) reach += d[i].stride * std::max(-d[i].lo, d[i].hi);
+  auto floor_div = [](long long a, long long b) { return a / b - (a % b < 0); };
+  const long long from = std::max(d->lo, -floor_div(reach - delta, d->stride)), to = std::min(d->hi, floor_div(delta + reach, d->stride));
+  if (to - from >= 8) return true;
+  for (long long q = from; q <= to; ++q)
+    if (steps_meet(d + 1, n - 1, delta - q * d->stride, width)) return true;
+  return false;
+}
+// No element in common: ranges that do not meet; blocks between each other's, at the same strides (q and k inside a fused projection, in
+// any order of its dimensions); or columns apart in rows of one pitch.
+bool apart(const Blocks& a, const Blocks& b, int es) {
+  if (!overlap(a.p, a.end(es), b.p, b.end(es))) return true;
+  const long long bytes = (const char*)b.p - (const char*)a.p;
   if (bytes % es) return false;
-  const long long d = ((bytes / es) % a_row + a_row) % a_row;
-  return d >= a_width && d + b_width <= a_row;
+  bool same = true;
+  int n = 0;
+  Step d[3];
+  for (int i = 0; i < 3; ++i) {
+    const long long s = a.count[i] > 1 ? a.stride[i] : b.stride[i];
+    if (a.count[i] > 1 && b.count[i] > 1 && a.stride[i] != b.stride[i]) same = false;
+    if ((a.count[i] > 1 || b.count[i] > 1) && s > 0) d[n++] = Step{s, -(b.count[i] - 1), a.count[i] - 1};
+  }
+  std::sort(d, d + n, [](const Step& x, const Step& y) { return x.stride > y.stride; });
+  if (same && !steps_meet(d, n, bytes / es, a.width)) return true;
+  const long long row = a.stride[1], a_width = (a.count[2] - 1) * a.stride[2] + a.width, b_width = (b.count[2] - 1) * b.stride[2] + b.width;
+  if (row != b.stride[1] || row < 1 || (a.count[0] > 1 && (a.stride[0] % row || b.stride[0] % row))) return false;
+  const long long at = ((bytes / es) % row + row) % row;
+  return at >= a_width && at + b_width <= row;
 }
 
 }  // namespace
@@ -159,16 +192,15 @@ extern "C" int vtc_rotary_heads(int device, int dtype, const vtc_rotary* r, int6
   if (length > 0x7fffffff || batch > 0x7fffffffffffll / length) return fail_handleless(VTC_ERR_ARG, "rotary: too many rows");
   int vec = 16 / esize(dtype);
   bool copy_tail = false;
-  const char* ends[2][2];
+  Blocks xs[2], ys[2];
   for (int i = 0; i < n_tensors; ++i) {
     const vtc_heads& t = tensors[i];
     const char* name = i ? "second tensor" : "first tensor";
     bool in_place = false;
     if (int rc = rotary_check_tensor(name, t, *r, batch, length, dtype, &in_place)) return rc;
-    ends[i][0] = end_of(t.x, {{batch, t.x_batch}, {length, t.x_row}, {t.heads, t.x_head}}, r->head_dim, esize(dtype));
-    ends[i][1] = end_of(t.y, {{batch, t.y_batch}, {length, t.y_row}, {t.heads, t.y_head}}, r->head_dim, esize(dtype));
-    if (!in_place && !apart(t.x, ends[i][0], t.x_batch, t.x_row, (t.heads - 1) * t.x_head + r->head_dim, t.y, ends[i][1], t.y_batch, t.y_row,
-                            (t.heads - 1) * t.y_head + r->head_dim, batch, esize(dtype)))
+    xs[i] = Blocks{t.x, {t.x_batch, t.x_row, t.x_head}, {batch, length, t.heads}, r->head_dim};
+    ys[i] = Blocks{t.y, {t.y_batch, t.y_row, t.y_head}, {batch, length, t.heads}, r->head_dim};
+    if (!in_place && !apart(xs[i], ys[i], esize(dtype)))
       return fail_handleless(VTC_ERR_ARG, "rotary: input and output of the %s overlap without being the same", name);
     copy_tail = copy_tail || !in_place;
     p.t[i] = RotaryTensor{t.x, t.y, t.x_batch, t.x_row, t.x_head, t.y_batch, t.y_row, t.y_head, t.heads};
@@ -177,14 +209,9 @@ extern "C" int vtc_rotary_heads(int device, int dtype, const vtc_rotary* r, int6
     vec = std::min(vec, vec_of(dtype, {half, r->head_dim - r->rotary_dim, eff(t.x_batch, batch), eff(t.x_row, length), eff(t.x_head, t.heads),
                                        eff(t.y_batch, batch), eff(t.y_row, length), eff(t.y_head, t.heads)}, {t.x, t.y}));
   }
-  for (int i = 0; n_tensors == 2 && i < 2; ++i) {   // what one tensor's blocks write, the other's must not read or write
-    const vtc_heads &a = tensors[i], &b = tensors[1 - i];
-    if (!apart(a.y, ends[i][1], a.y_batch, a.y_row, (a.heads - 1) * a.y_head + r->head_dim, b.x, ends[1 - i][0], b.x_batch, b.x_row,
-               (b.heads - 1) * b.x_head + r->head_dim, batch, esize(dtype)) ||
-        !apart(a.y, ends[i][1], a.y_batch, a.y_row, (a.heads - 1) * a.y_head + r->head_dim, b.y, ends[1 - i][1], b.y_batch, b.y_row,
-               (b.heads - 1) * b.y_head + r->head_dim, batch, esize(dtype)))
+  for (int i = 0; n_tensors == 2 && i < 2; ++i)   // what one tensor's blocks write, the other's must not read or write
+    if (!apart(ys[i], xs[1 - i], esize(dtype)) || !apart(ys[i], ys[1 - i], esize(dtype)))
       return fail_handleless(VTC_ERR_ARG, "rotary: an output shares memory with the other tensor");
-  }
   DeviceGuard guard(device);
   if (guard.rc) return guard.rc;
   p.pos = positions; p.pos64 = positions64 ? 1 : 0; p.pb = pos_batch; p.pt = pos_row; p.offset = offset;
