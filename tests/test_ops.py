@@ -1203,3 +1203,17 @@ def test_rotary_takes_what_is_apart_and_refuses_what_is_shared():
         assert got == (not shared), (base, strides, counts, heads, dim)
         seen[got] += 1
     assert min(seen.values()) > 300, seen
+
+
+@gpu
+def test_group_norm_statistics_of_samples_without_rows():
+    """A call on samples of length 0 still writes their mean and rstd, from C as from Python."""
+    mean, rstd = torch.full((2, 70000, 20), float("nan"), device="cuda")
+    t = C.byref(L.VtcRows3(None, 0, 40))
+    L.check(L.load().vtc_group_norm_act(0, 1, t, t, 70000, 0, 40, 20, None, None, 0, 1e-5, 0, None, mean.data_ptr(), rstd.data_ptr(), None, 0,
+                                        torch.cuda.current_stream().cuda_stream))
+    assert not mean.any() and not rstd.any()
+    x = torch.zeros((3, 0, 40), device="cuda")
+    y, mean, rstd = ops.group_norm_act_forward(x, 20)
+    assert y.shape == x.shape and mean.shape == (3, 20) and not mean.any() and not rstd.any()
+    assert ops.group_norm_act_forward(x[:0], 20)[1].shape == (0, 20)

@@ -358,8 +358,21 @@ extern "C" int vtc_group_norm_act(int device, int dtype, const vtc_rows3* x, con
   const vtc_rows3* ts[2] = {x, y};
   if (int rc = gn_check("group norm", dtype, affine_f32, ts, 2, batch, length, channels, groups, act)) return rc;
   if (!(eps >= 0.0) || !std::isfinite(eps)) return fail_handleless(VTC_ERR_ARG, "group norm: eps must be finite and not negative");
-  if (batch == 0 || length == 0) return VTC_OK;
+  if (batch == 0) return VTC_OK;
   if (!mean || !rstd) return fail_handleless(VTC_ERR_ARG, "group norm: mean and rstd are needed");
+  if (length == 0) {   // samples without rows: mean = rstd = 0
+    DeviceGuard guard(device);
+    if (guard.rc) return guard.rc;
+    GnParams p = gn_params(batch, 0, channels, groups, nullptr, nullptr, 0, nullptr);
+    p.mean = mean; p.rstd = rstd;
+    const int per16 = (groups + 15) / 16;
+    const long long slice = gn_slice(batch, 256ll * per16);
+    for (long long n0 = 0; n0 < batch; n0 += slice) {
+      const GnParams q = gn_from(p, dtype, n0, std::min(slice, batch - n0));
+      hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(q.N * per16)), dim3(256), 0, (hipStream_t)stream, q);
+    }
+    return launched("group norm");
+  }
   const size_t need = gn_forward_bytes(batch, length, channels, groups);
   if (!workspace || workspace_bytes < (int64_t)need) return fail_handleless(VTC_ERR_CAPACITY, "group norm: the workspace holds %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   if ((uintptr_t)workspace % 256) return fail_handleless(VTC_ERR_ARG, "group norm: the workspace is not aligned to 256 bytes");

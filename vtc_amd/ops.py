@@ -344,10 +344,6 @@ def group_norm_act_forward(x: torch.Tensor, groups: int, weight=None, bias=None,
     index, dt, f32, n, t, c = _gn_args(what, x, groups, weight, bias, lengths, act)
     given, out = out, _gn_out(what, x, out)
     mean, rstd = torch.empty((2, n, groups), dtype=torch.float32, device=x.device).unbind(0)
-    if n == 0 or t == 0:
-        mean.zero_()
-        rstd.zero_()
-        return out, mean, rstd
     so = _library()
     size = _bytes("vtc_group_norm_act_workspace", n, t, c, groups, 0)
     ws = _workspace(size, x)
