@@ -1217,3 +1217,22 @@ def test_group_norm_statistics_of_samples_without_rows():
     y, mean, rstd = ops.group_norm_act_forward(x, 20)
     assert y.shape == x.shape and mean.shape == (3, 20) and not mean.any() and not rstd.any()
     assert ops.group_norm_act_forward(x[:0], 20)[1].shape == (0, 20)
+
+
+@gpu
+def test_one_channel_and_one_column_have_no_stride():
+    """A single channel turned channel-last and weights of width one keep the stride of what they were; it means nothing."""
+    g = torch.Generator(device="cuda").manual_seed(51)
+    x, dy = (torch.randn((3, 1, 70), generator=g, device="cuda").transpose(1, 2) for _ in range(2))   # (3, 70, 1), strides (70, 1, 70)
+    w = torch.randn(1, generator=g, device="cuda")
+    assert x.stride(2) == 70
+    check_gn("f32", x, 1, w, w, "silu", None, dy, run_gn(x, 1, w, w, "silu", None, dy))
+    z = x.clone(memory_format=torch.preserve_format)
+    assert torch.equal(ops.group_norm_act_forward(z, 1, out=z)[0], ops.group_norm_act_forward(x, 1)[0])
+    leaf = x.detach().requires_grad_()
+    (dx,) = torch.autograd.grad(ops.group_norm_act(leaf, 1, w, w, act="silu"), leaf, dy)
+    assert torch.equal(dx, run_gn(x, 1, w, w, "silu", None, dy)[3])
+    x, w, b, dy = make_ffn(torch.float16, 130, 1, 24, 8, True)
+    turned = tuple(t.as_strided(t.shape, (1, t.shape[0])) for t in w[:2] + (x,))
+    y, saved = ops.gated_ffn_forward(turned[2], *turned[:2], w[2], *b, save=True)
+    check_ffn(torch.float16, x, w, b, "silu", dy, y, ops.gated_ffn_backward(dy, x, *turned[:2], w[2], saved))

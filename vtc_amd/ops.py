@@ -284,6 +284,11 @@ def rotary(x: torch.Tensor, spec: Rotary, positions: torch.Tensor | None = None,
     return _rotary_call((x,), spec, positions, offset, inverse, None)[0]
 
 
+def _dense_last(t) -> bool:
+    """Whether the elements of the last dimension are neighbours (one element has no stride, whatever the tensor says)."""
+    return t.stride(-1) == 1 or t.shape[-1] == 1 or not t.numel()
+
+
 # ------------------------------------------------------------------------------------------------ group norm + activation
 _GN_ACTS = ("none", "gelu", "silu")
 
@@ -295,7 +300,7 @@ def _gn_args(what, x, groups, weight, bias, lengths, act):
     if len(shape) != 3:
         raise ValueError(f"{what}: rows are (batch, length, channels), got {tuple(shape)}")
     n, t, c = shape
-    if x.stride(2) != 1 and n * t * c:
+    if not _dense_last(x):
         raise ValueError(f"{what}: the channels of a row must be contiguous")
     if groups < 1 or c < 1 or c % groups:
         raise ValueError(f"{what}: {c} channels do not divide into {groups} groups")
@@ -329,7 +334,7 @@ def _gn_out(what, x, out):
         return _empty(x)
     _same(what, x, "out", out)
     _check_out(what, out)
-    if out.shape != x.shape or (out.numel() and out.stride(2) != 1):
+    if out.shape != x.shape or not _dense_last(out):
         raise ValueError(f"{what}: out must have shape {tuple(x.shape)} with contiguous channels")
     return out
 
@@ -363,7 +368,7 @@ def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, groups: int, mean
     what = "group_norm_act_backward"
     index, dt, f32, n, t, c = _gn_args(what, x, groups, weight, bias, lengths, act)
     _same(what, x, "dy", dy)
-    if dy.shape != x.shape or (dy.stride(2) != 1 and dy.numel()):
+    if dy.shape != x.shape or not _dense_last(dy):
         raise ValueError(f"{what}: dy must have shape {tuple(x.shape)} with contiguous channels")
     for s in (mean, rstd):
         if not s.is_cuda or s.get_device() != index or s.dtype is not torch.float32 or s.shape != (n, groups) or not s.is_contiguous():
@@ -395,7 +400,7 @@ class _GroupNormActFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, bias, lengths, mean, rstd = ctx.saved_tensors
-        if dy.numel() and dy.stride(2) != 1:
+        if not _dense_last(dy):
             dy = dy.contiguous()
         dx, dw, db = group_norm_act_backward(dy, x, ctx.args[0], mean, rstd, weight, bias, ctx.args[1], lengths)
         return dx, None, dw, db, None, None, None
@@ -433,7 +438,7 @@ def _ffn_args(what, x, w_gate, w_up, w_down, biases, act):
                          f"{tuple(sg)}, {tuple(su)}, {tuple(sd)}")
     for name, t in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
         row, col = t.stride()
-        if col != 1 or (row < t.shape[1] and t.shape[0] > 1):
+        if (col != 1 and t.shape[1] > 1) or (row < t.shape[1] and t.shape[0] > 1):
             raise ValueError(f"{what}: {name} must be stored row by row")
     if act not in ACTS:
         raise ValueError(f"{what}: act must be one of {list(ACTS)}, got {act!r}")
