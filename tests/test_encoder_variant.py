@@ -80,6 +80,29 @@ def test_every_stage_of_a_variant_against_the_oracle(name, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("name", [n for n, v in VARIANTS.items() if not v.conv_norm_groups])
+def test_conv_layers_without_norms_keep_the_base_models_bf16_bar(name):
+    """One store per conv layer, as in HuBERT-base: 6e-2 on conv rows, not the bar of layers that store twice."""
+    variant = VARIANTS[name]
+    w = variant_state(variant)
+    B, W = 3, 16000
+    T = O.conv_out_len(W)
+    wav = np.random.default_rng(1).standard_normal((B, W), dtype=np.float32) * np.float32(0.1)
+    st = O.encoder_stages(as_torch(w), torch.from_numpy(wav), variant=variant)
+    eng = VtcEngine(w, 4, 1.0, max_batch=B, mfma_dtype="bf16", variant=variant)
+    arena = torch.from_numpy(wav.reshape(-1).copy()).cuda()
+    logits = torch.zeros((B * T, 4), device="cuda")
+    for stage in range(7):
+        eng.debug_stop_after(stage)
+        eng.forward_windows(arena, np.arange(B) * W, np.full(B, W), np.arange(B) * T, np.full(B, T), logits)
+        ref = st[f"conv{stage}"].transpose(1, 2).contiguous()
+        got = torch.from_numpy(eng.debug_stage(stage, B, ref.numel()).reshape(ref.shape))
+        err = (got - ref).abs().max().item()
+        assert err <= 6e-2 * max(1.0, float(ref.std())), f"conv{stage}: max abs err {err}"
+    eng.close()
+
+
+@gpu
 def test_variant_changes_the_result_and_the_base_model_is_untouched():
     w = synth.make_weights(seed=0, family="hubert")
     wav = torch.from_numpy(synth.synth_audio(3.0, 5)).cuda()
