@@ -502,7 +502,6 @@ namespace {
 
 constexpr int64_t kFfnMaxDim = 1 << 18;   // width, inner width: tile offsets stay far below 2^31 bytes
 constexpr int kSkinnyRows = 64;
-constexpr long long kMaxPitch = 1 << 20;  // elements between rows of a matrix (of more than one row)
 
 // Carves a workspace; with base == null it only measures.
 struct Arena {
@@ -527,7 +526,7 @@ struct FfnArgs {
 int ffn_check_mat(const char* what, const char* name, const vtc_mat* m, int64_t rows, int cols) {
   if (!m || !m->p) return fail_handleless(VTC_ERR_ARG, "%s: %s is null", what, name);
   if (rows > 1 && (m->row < cols || m->row > kMaxPitch))
-    return fail_handleless(VTC_ERR_ARG, "%s: %s has a row pitch of %lld for %d columns (at most %lld)", what, name, (long long)m->row, cols, kMaxPitch);
+    return fail_handleless(VTC_ERR_ARG, "%s: %s has a row pitch of %lld for %d columns (at most %d)", what, name, (long long)m->row, cols, kMaxPitch);
   if ((uintptr_t)m->p % 2) return fail_handleless(VTC_ERR_ARG, "%s: %s is not aligned to its type", what, name);
   return VTC_OK;
 }
