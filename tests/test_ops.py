@@ -1236,3 +1236,16 @@ def test_one_channel_and_one_column_have_no_stride():
     turned = tuple(t.as_strided(t.shape, (1, t.shape[0])) for t in w[:2] + (x,))
     y, saved = ops.gated_ffn_forward(turned[2], *turned[:2], w[2], *b, save=True)
     check_ffn(torch.float16, x, w, b, "silu", dy, y, ops.gated_ffn_backward(dy, x, *turned[:2], w[2], saved))
+
+
+@gpu
+@pytest.mark.parametrize("m", [2, 16, 17, 32, 33, 64])
+def test_gated_ffn_few_rows_do_not_reach_each_other(m):
+    """A row that is no number stays alone on both sides of the border between the kernels of few and of many rows."""
+    x, w, b, dy = make_ffn(torch.float16, m, 100, 132, 60, True)
+    want, saved = ops.gated_ffn_forward(x, *w, *b, save=True)
+    check_ffn(torch.float16, x, w, b, "silu", dy, want, ops.gated_ffn_backward(dy, x, *w, saved))
+    x[1] = float("nan")
+    got = ops.gated_ffn(x, *w, *b)
+    clean = torch.arange(m, device="cuda") != 1
+    assert got[1].isnan().all() and torch.equal(got[clean], want[clean])

@@ -8,7 +8,7 @@
 // forward pass keeps for the backward one (s = u act'(g) and a = act(g), so that no activation is computed twice) has 24 bits;
 // every sum is fp32 (column sums are joined in fp64).
 //
-// Few rows (at most 64: single frames, live streams) are bound by reading the weights once, and by latency: skinny_kernel
+// Few rows (at most 32: single frames, live streams) are bound by reading the weights once, and by latency: skinny_kernel
 // below.  Everything else runs on op_gemm_kernel or, where that would leave CUs idle, op_small_kernel.
 #pragma once
 #include "common.hip.h"
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(512) void skinny_kernel(const SkinnyParams p) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[w][m] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int steps = (p.K + 31) / 32;
-  constexpr int D = MT == 4 ? 2 : 4;            // K steps in flight; steps behind the end read as zero
+  constexpr int D = 4;                          // K steps in flight; steps behind the end read as zero
   for (int s0 = wave; s0 < steps; s0 += 8 * D) {
     u16x8 a[D][NW], b[D][MT];
 #pragma unroll

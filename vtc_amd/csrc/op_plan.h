@@ -23,6 +23,9 @@ inline int div_up(long long a, int b) { return (int)((a + b - 1) / b); }
 //   dx               512 rows 72 / 16   2048 74 / 30   8192 86 / 82   16384 109 / 173
 //   dg and du        512 rows 36 / 13   2048 37 / 20   8192 88 / 73   16384 149 / 162
 //   weights          512 rows 31 / 22   2048 46 / 44   8192 91 / 137  16384 165 / 290
+// Whole training steps at other widths, by this rule / all small / all 256-wide (bf16, us): 256 x 512, 8192 rows 66 / 65 / 121, 31936 rows 199 /
+// 198 / 207; 1024 x 4096, 2048 rows 229 / 264 / 349, 8192 rows 740 / 1018 / 742; 2048 x 8192, 512 rows 333 / 355 / 634, 2048 rows 772 / 1007 /
+// 906, 8192 rows 2445 / 3979 / 2461; 389 x 1031, 1024 rows 60 / 60 / 166, 8192 rows 198 / 189 / 228.
 struct OgPlan { bool small; int splits, kps; };
 struct OgCost { long long tiles_big, tiles_small; double width, end_big, end_small; };   // tiles; epilogue of a tile
 inline OgPlan og_plan(const OgCost& o, int nk, int splits_big, int splits_small, double out_elems) {

@@ -501,7 +501,10 @@ extern "C" int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows
 namespace {
 
 constexpr int64_t kFfnMaxDim = 1 << 18;   // width, inner width: tile offsets stay far below 2^31 bytes
-constexpr int kSkinnyRows = 64;
+// Most rows of skinny_kernel.  A forward pass, bf16, skinny / tiles (us): 768 x 2048, 1 row 8.3 / 15.0, 16 10.2 / 15.4, 32 13.0 / 15.8, 48 18.3 /
+// 16.2, 64 19.5 / 16.5; 256 x 512, 64 rows 9.9 / 11.0; 2048 x 8192, 16 rows 30.0 / 30.5, 32 40 / 31, 64 64 / 33: every
+// block of 16 columns reads all rows of x.
+constexpr int kSkinnyRows = 32;
 
 // Carves a workspace; with base == null it only measures.
 struct Arena {
@@ -638,8 +641,7 @@ template <bool F16> void launch_reduce(const ReduceParams& r, hipStream_t s) {
 template <bool F16, bool GATE> void launch_skinny(const SkinnyParams& p, hipStream_t s) {
   const dim3 grid((unsigned)((p.N + 15) / 16)), block(512);
   if (p.M <= 16) hipLaunchKernelGGL((skinny_kernel<F16, 1, GATE>), grid, block, 0, s, p);
-  else if (p.M <= 32) hipLaunchKernelGGL((skinny_kernel<F16, 2, GATE>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((skinny_kernel<F16, 4, GATE>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((skinny_kernel<F16, 2, GATE>), grid, block, 0, s, p);
 }
 template <typename F> void by_f16(int dtype, F&& f) {
   if (dtype == OP_F16) f(std::true_type{});
