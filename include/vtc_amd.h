@@ -244,8 +244,9 @@ const char* vtc_profile_class_name(int32_t cls);
  * `stream` (which belongs to that device), never allocate and never synchronise, so they may be captured into a graph and
  * called from several threads; the caller's current device is left as it was.  Scratch memory is the caller's: its size comes
  * from the matching _workspace call, it must be 256-byte aligned, and two calls that may run at the same time need two.
- * The message of a failure is vtc_last_error(NULL) on the calling thread.  Sizes of zero are valid and launch nothing that
- * reads them.  Bits of a result do not depend on the launch order (no atomics). */
+ * The message of a failure is vtc_last_error(NULL) on the calling thread.  No batch, no length and no rows are valid and launch
+ * nothing that reads them (vtc_gated_ffn_backward alone refuses rows == 0: its gradients are zeros, which the caller has).  Bits of a
+ * result do not depend on the launch order (no atomics). */
 typedef enum { VTC_F32 = 0, VTC_F16 = 1, VTC_BF16 = 2 } vtc_dtype;
 typedef enum { VTC_ACT_NONE = 0, VTC_ACT_GELU = 1 /* x Phi(x) */, VTC_ACT_SILU = 2, VTC_ACT_SIGMOID = 3 } vtc_act;
 

@@ -344,7 +344,8 @@ def group_norm_act_forward(x: torch.Tensor, groups: int, weight=None, bias=None,
     """(y, mean, rstd): y = act(group_norm(x)) on channel-last rows (batch, length, channels), statistics per sample and group of
     neighbouring channels over the first lengths[n] rows (int32 tensor, default all).  Rows behind a sample's length are not read
     and come out as zero.  weight / bias: of x's type or float32.  out: where y goes (x itself for in place).  mean and rstd
-    (batch, groups, float32) are what the backward call needs.  A sample's result does not depend on the rest of its batch."""
+    (batch, groups, float32) are what the backward call needs.  A sample's result does not depend on the rest of its batch (of tensors
+    with the same strides and alignment)."""
     what = "group_norm_act"
     index, dt, f32, n, t, c = _gn_args(what, x, groups, weight, bias, lengths, act)
     given, out = out, _gn_out(what, x, out)
@@ -469,7 +470,8 @@ def _rows2(t):
 def gated_ffn_forward(x: torch.Tensor, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu", save: bool = False):
     """(y, saved): y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down on rows x (.., width) in float16 or bfloat16,
     sums in fp32; w_gate, w_up (inner, width), w_down (out, inner); biases of x's type or float32.  With save, `saved` is what
-    gated_ffn_backward needs, an opaque buffer of vtc_gated_ffn_saved bytes; else None."""
+    gated_ffn_backward needs, an opaque buffer of vtc_gated_ffn_saved bytes; else None.  The order in which a row's products are added
+    follows the number of rows, so its last bits do."""
     what = "gated_ffn"
     index, dt, f32, k, f, n = _ffn_args(what, x, w_gate, w_up, w_down, (b_gate, b_up, b_down), act)
     rows = _rows2(x)
