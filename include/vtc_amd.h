@@ -299,10 +299,11 @@ int vtc_group_norm_act_backward(int device, int dtype, const vtc_rows3* dy, cons
 
 /* Gated feed-forward block on rows of f16 / bf16 (sums in fp32): g = x W_gate^T + b_gate, u = x W_up^T + b_up,
  * h = act(g) * u (NONE, GELU, SILU, SIGMOID), y = h W_down^T + b_down.  x [rows][width], W_gate and W_up [inner][width], W_down
- * [out_width][inner] (as torch.nn.Linear keeps them), y [rows][out_width]; any sizes, row pitches of up to 2^20 elements (of a
- * single row the pitch is not looked at; operands whose rows are not made of aligned 16-byte pieces are copied into the workspace first).  Biases may be NULL; of the operands' type, or
- * fp32 with bias_f32 = 1.  h is rounded to the operands' type.  `saved` (vtc_gated_ffn_saved bytes, 256-byte aligned; NULL: no
- * backward call follows) receives h and, in 24 bits, act(g) and u act'(g): the backward call needs no activation.
+ * [out_width][inner] (as torch.nn.Linear keeps them), y [rows][out_width]; any sizes, row pitches of up to 2^20 elements (that of a
+ * single row is not looked at); operands whose rows are not made of aligned 16-byte pieces are copied into the workspace first.
+ * Biases may be NULL; of the operands' type, or fp32 with bias_f32 = 1.  h is rounded to the operands' type.  `saved`
+ * (vtc_gated_ffn_saved bytes, 256-byte aligned; NULL: no backward call follows) receives h and, in 24 bits, act(g) and u act'(g):
+ * the backward call needs no activation.
  * Backward: dy [rows][out_width] -> any of dx (row pitch dx_row), the weights' gradients (all three or none; dense, in the weights'
  * layout and type) and the biases' (of the biases' type); NULL leaves one out.  dx may not overlap x or dy. */
 typedef struct {
