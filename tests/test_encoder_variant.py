@@ -103,6 +103,23 @@ def test_conv_layers_without_norms_keep_the_base_models_bf16_bar(name):
 
 
 @gpu
+@pytest.mark.parametrize("variant,inner", [(EncoderVariant(ffn="gated_sigmoid"), 256), (EncoderVariant(ffn="gated_gelu"), 8192), (EncoderVariant(conv_norm_groups=1), 0),
+                                           (EncoderVariant(conv_norm_groups=512), 0), (EncoderVariant(rotary=Rotary(2, layout="interleaved")), 0)])
+def test_logits_at_the_limits_of_a_variants_sizes(variant, inner):
+    """The narrowest and widest gated block, one group of all channels and one per channel, one rotated pair; the bar of the logits above."""
+    w = variant_state(variant, inner=inner or 2048)
+    B, W = 3, 16000
+    T = O.conv_out_len(W)
+    wav = np.random.default_rng(2).standard_normal((B, W), dtype=np.float32) * np.float32(0.1)
+    want = O.encoder_stages(as_torch(w), torch.from_numpy(wav), variant=variant)["logits"]
+    eng = VtcEngine(w, 4, 1.0, max_batch=B, variant=variant)
+    logits = torch.zeros((B * T, 4), device="cuda")
+    eng.forward_windows(torch.from_numpy(wav.reshape(-1).copy()).cuda(), np.arange(B) * W, np.full(B, W), np.arange(B) * T, np.full(B, T), logits)
+    assert (logits.cpu() - want.reshape(B * T, 4)).abs().max().item() <= 2e-2
+    eng.close()
+
+
+@gpu
 def test_variant_changes_the_result_and_the_base_model_is_untouched():
     w = synth.make_weights(seed=0, family="hubert")
     wav = torch.from_numpy(synth.synth_audio(3.0, 5)).cuda()
